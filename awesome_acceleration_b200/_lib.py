@@ -37,6 +37,13 @@ SIGNATURES: dict[str, tuple] = {
     "aacc_paged_decode_noalloc_capacity_bytes": (I64, []),
     "aacc_prefill_attention": (I32, [P, P, I64, P, P, I64, P, I64, P, P, P, I64, I64, I32, I32, I32, F32, P]),
     "aacc_prefill_attention_mma": (I32, [P, P, P, P, I64, P, I64, P, P, P, I64, I64, I32, I32, I32, F32, P]),
+    "aacc_build_block_tables": (I32, [P, I64, I32, P, I64, P, I64, P, P]),
+    "aacc_build_slot_maps": (I32, [P, P, P, I64, P, I64, I64, I32, I64, P, P, P, I64, P]),
+    "aacc_kv4_store": (I32, [P, P, I64, I64, I64, I64, I64, P, P, P, I64, I32, I32, P]),
+    "aacc_kv4_load": (I32, [P, P, I64, I32, I32, P, P, I64, P, P, I64, I32, P]),
+    "aacc_kv4_decode_workspace_bytes": (I64, [I32, I32]),
+    "aacc_kv4_decode_attention": (I32, [P, P, P, P, I64, P, I64, I64, P, P, I32, I64, I32, I32, I32, F32,
+                                        I64, P, I64, P]),
     "aacc_rmsnorm": (I32, [P, P, P, I64, I64, F32, P]),
     "aacc_add_rmsnorm": (I32, [P, P, P, P, I64, I64, F32, P]),
     "aacc_embed_rmsnorm": (I32, [P, P, I64, P, P, P, I64, I64, F32, P]),

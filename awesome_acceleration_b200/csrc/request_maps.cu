@@ -1,0 +1,194 @@
+// Block tables and slot maps from request lengths, on the device.
+//
+// Both are prefix sums over the requests followed by a write per output
+// element; the outputs are a few hundred KB at most, so launch latency and
+// the dependent loads of the scan are the cost.  Every CTA scans the lengths
+// itself (a few KB from L2) instead of waiting for another kernel or CTA.
+#include "common.cuh"
+#include "host.h"
+
+namespace aacc {
+
+constexpr int kMapThreads = 256;
+constexpr int kMapPer = 4;                             // requests a thread scans per chunk
+constexpr int kMapChunk = kMapThreads * kMapPer;       // requests per chunk
+constexpr int kMapTokens = 512;                        // packed tokens one CTA maps
+
+__device__ __forceinline__ int64_t warp_scan_incl(int64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+// Exclusive prefix of every thread's `v` over the CTA; *total is the sum.
+__device__ __forceinline__ int64_t block_scan_excl(int64_t v, int64_t* sh, int64_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t inc = warp_scan_incl(v, lane);
+  __syncthreads();  // sh of the previous call is read
+  if (lane == 31) sh[warp] = inc;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kMapThreads / 32; ++w) {
+    const int64_t x = sh[w];
+    if (w < warp) before += x;
+    all += x;
+  }
+  *total = all;
+  return before + inc - v;
+}
+
+__device__ __forceinline__ int64_t blocks_of(int32_t len, int bs, int64_t max_blocks) {
+  const int64_t need = len > 0 ? ((int64_t)len + bs - 1) / bs : 0;
+  return min(need, max_blocks);
+}
+
+// One CTA per request: its first block is the number of blocks that the
+// requests before it take.
+__global__ void __launch_bounds__(kMapThreads)
+    build_block_tables_kernel(const int32_t* __restrict__ lengths, int64_t n, int bs,
+                              const int32_t* __restrict__ free_blocks, int64_t num_free, int32_t* __restrict__ tables,
+                              int64_t max_blocks, int32_t* __restrict__ used, unsigned* err) {
+  __shared__ int64_t sh[kMapThreads / 32];
+  griddep_wait();
+  griddep_launch();
+  const int64_t i = blockIdx.x;
+  int64_t part = 0, off;
+  for (int64_t j = threadIdx.x; j < i; j += kMapThreads) part += blocks_of(lengths[j], bs, max_blocks);
+  block_scan_excl(part, sh, &off);
+  const int32_t len = lengths[i];
+  const int64_t need = blocks_of(len, bs, max_blocks);
+  for (int64_t j = threadIdx.x; j < max_blocks; j += kMapThreads) {
+    int32_t b = -1;
+    if (j < need) {
+      const int64_t at = off + j;
+      if (at >= num_free)
+        report(err, ERR_BLOCK_OOB);
+      else
+        b = free_blocks ? free_blocks[at] : (int32_t)at;
+    }
+    tables[i * max_blocks + j] = b;
+  }
+  if (threadIdx.x == 0) {
+    if ((int64_t)len > max_blocks * bs) report(err, ERR_CTX_OOB);
+    if (i == n - 1 && used) *used = (int32_t)min(off + need, (int64_t)0x7fffffff);
+  }
+}
+
+// One CTA per kMapTokens packed tokens.  It walks the requests in chunks; of
+// the chunk whose tokens meet its own it keeps the prefix sums in shared
+// memory, where every token finds its request by bisection.
+__global__ void __launch_bounds__(kMapThreads)
+    build_slot_maps_kernel(const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts,
+                           const int64_t* __restrict__ rows, int64_t n, const int32_t* __restrict__ bt,
+                           int64_t num_rows, int64_t max_blocks, int bs, int64_t num_blocks, int32_t* __restrict__ cu,
+                           int64_t* __restrict__ positions, int64_t* __restrict__ slots, int64_t num_tokens,
+                           unsigned* err) {
+  __shared__ int64_t sh[kMapThreads / 32];
+  __shared__ int64_t pre[kMapChunk + 1];
+  griddep_wait();
+  griddep_launch();
+  const int64_t t0 = (int64_t)blockIdx.x * kMapTokens;
+  const int64_t t1 = min(t0 + kMapTokens, num_tokens);
+  const bool first = blockIdx.x == 0;  // writes cu, so it walks every chunk
+  int64_t base = 0;
+  for (int64_t c0 = 0; c0 < n && (first || base < t1); c0 += kMapChunk) {
+    int32_t len[kMapPer];
+    int64_t mine = 0, total;
+#pragma unroll
+    for (int p = 0; p < kMapPer; ++p) {
+      const int64_t j = c0 + threadIdx.x * kMapPer + p;
+      len[p] = j < n ? max(lengths[j], 0) : 0;
+      mine += len[p];
+    }
+    int64_t at = base + block_scan_excl(mine, sh, &total);
+    const int m = (int)min((int64_t)kMapChunk, n - c0);
+#pragma unroll
+    for (int p = 0; p < kMapPer; ++p) {
+      const int q = threadIdx.x * kMapPer + p;
+      pre[q] = at;
+      if (first && q < m) cu[c0 + q] = (int32_t)min(at, (int64_t)0x7fffffff);
+      at += len[p];
+    }
+    if (threadIdx.x == 0) pre[kMapChunk] = base + total;
+    __syncthreads();
+    const int64_t lo = max(t0, base), hi = min(t1, base + total);
+    for (int64_t t = lo + threadIdx.x; t < hi; t += kMapThreads) {
+      int a = 0, b = m;  // the last request of the chunk that starts at or before t: pre[a] <= t < pre[b]
+      while (b - a > 1) {
+        const int mid = (a + b) >> 1;
+        if (pre[mid] <= t)
+          a = mid;
+        else
+          b = mid;
+      }
+      const int64_t req = c0 + a;
+      const int64_t pos = t - pre[a] + (starts ? (int64_t)starts[req] : 0);
+      const int64_t row = rows ? rows[req] : req;
+      int64_t slot = -1;
+      if (row >= num_rows) {
+        report(err, ERR_SLOT_OOB);
+      } else if (row >= 0) {  // negative rows are padding
+        const int64_t j = pos / bs;
+        if (pos < 0 || j >= max_blocks) {
+          report(err, ERR_CTX_OOB);
+        } else {
+          const int64_t blk = bt[row * max_blocks + j];
+          if (blk < 0 || blk >= num_blocks)
+            report(err, ERR_BLOCK_OOB);
+          else
+            slot = blk * bs + (pos - j * bs);
+        }
+      }
+      if (positions) positions[t] = pos;
+      slots[t] = slot;
+    }
+    base += total;
+    __syncthreads();  // pre is rewritten by the next chunk
+  }
+  if (first && threadIdx.x == 0) {
+    cu[n] = (int32_t)min(base, (int64_t)0x7fffffff);
+    if (base > num_tokens) report(err, ERR_CTX_OOB);
+  }
+  for (int64_t t = max(t0, base) + threadIdx.x; t < t1; t += kMapThreads) {  // behind the last request
+    if (positions) positions[t] = 0;
+    slots[t] = -1;
+  }
+}
+
+}  // namespace aacc
+
+using namespace aacc;
+
+extern "C" {
+
+int aacc_build_block_tables(const int32_t* lengths, int64_t num_requests, int block_size, const int32_t* free_blocks,
+                            int64_t num_free, int32_t* block_tables, int64_t max_blocks, int32_t* used,
+                            cudaStream_t stream) {
+  if (num_requests < 0 || num_requests > 0x7fffffff || block_size <= 0 || max_blocks <= 0 || num_free < 0)
+    return set_error(AACC_ERR_INVALID, "build_block_tables: bad sizes");
+  if (num_requests == 0) return AACC_OK;
+  return check_launch("build_block_tables",
+                      launch_k(build_block_tables_kernel, dim3((unsigned)num_requests), dim3(kMapThreads), 0, stream,
+                               lengths, num_requests, block_size, free_blocks, num_free, block_tables, max_blocks,
+                               used, device_error_ptr()));
+}
+
+int aacc_build_slot_maps(const int32_t* lengths, const int32_t* starts, const int64_t* rows, int64_t num_requests,
+                         const int32_t* block_tables, int64_t num_rows, int64_t max_blocks, int block_size,
+                         int64_t num_blocks, int32_t* cu_seqlens, int64_t* positions, int64_t* slots,
+                         int64_t num_tokens, cudaStream_t stream) {
+  if (num_requests < 0 || num_rows < 0 || max_blocks <= 0 || block_size <= 0 || num_blocks <= 0 || num_tokens < 0 ||
+      num_tokens > 0x7fffffff)
+    return set_error(AACC_ERR_INVALID, "build_slot_maps: bad sizes");
+  const int64_t ctas = num_tokens > 0 ? (num_tokens + kMapTokens - 1) / kMapTokens : 1;
+  return check_launch("build_slot_maps",
+                      launch_k(build_slot_maps_kernel, dim3((unsigned)ctas), dim3(kMapThreads), 0, stream, lengths,
+                               starts, rows, num_requests, block_tables, num_rows, max_blocks, block_size, num_blocks,
+                               cu_seqlens, positions, slots, num_tokens, device_error_ptr()));
+}
+
+}  // extern "C"

@@ -150,6 +150,81 @@ int aacc_prefill_attention_mma(const void* q, void* out, const void* k_cache, co
                                int64_t num_seqs, int64_t max_q_len, int num_q_heads, int num_kv_heads,
                                int block_size, float scale, cudaStream_t stream);
 
+/* ---- request maps ---------------------------------------------------------- */
+
+/* Block tables of new requests: request i takes need_i = ceil(lengths[i] /
+ * block_size) blocks (lengths <= 0: none) of the list free_blocks[num_free],
+ * in request order; row i of block_tables [num_requests][max_blocks] gets
+ * them, then -1.  free_blocks NULL is the list 0, 1, 2, ...  used (may be
+ * NULL) receives the number of blocks taken.  A request longer than
+ * max_blocks * block_size is cut there (error word bit 32); blocks past the
+ * end of the list are -1 (bit 1) and still counted in used.  The device form
+ * of the host's block bookkeeping for slots (llm.py:139-140). */
+int aacc_build_block_tables(const int32_t* lengths, int64_t num_requests, int block_size, const int32_t* free_blocks,
+                            int64_t num_free, int32_t* block_tables, int64_t max_blocks, int32_t* used,
+                            cudaStream_t stream);
+
+/* Packed positions and flat cache slots of tokens [starts[i], starts[i] +
+ * lengths[i]) of every request i (starts NULL: 0), the paged form of the
+ * packed prefill's scatter indices and cu_seqlens (llm.py:131-150):
+ *   cu_seqlens[num_requests + 1]  prefix sums of max(lengths, 0)
+ *   positions[num_tokens]         (may be NULL)
+ *   slots[num_tokens]             block_tables[rows[i]][pos / bs] * bs + pos % bs
+ * rows NULL: request i owns row i; a negative row is padding (slots -1).
+ * num_tokens is the size of the outputs: entries behind the last request get
+ * position 0 and slot -1 (which the stores skip).  A token without a valid
+ * block gets slot -1 and sets the error word, and so does a sum of lengths
+ * above num_tokens (the tokens that do not fit are dropped). */
+int aacc_build_slot_maps(const int32_t* lengths, const int32_t* starts, const int64_t* rows, int64_t num_requests,
+                         const int32_t* block_tables, int64_t num_rows, int64_t max_blocks, int block_size,
+                         int64_t num_blocks, int32_t* cu_seqlens, int64_t* positions, int64_t* slots,
+                         int64_t num_tokens, cudaStream_t stream);
+
+/* ---- 4-bit KV cache ---------------------------------------------------------
+ * A pool holds K or V of one layer as uint8
+ *   [num_blocks][num_kv_heads][block_size / 64][4608]:
+ * per 64 tokens of a kv head 4096 bytes of 4-bit codes, then 64 x 4 bf16
+ * scales.  32 consecutive dims of a (token, kv head) share the scale
+ * s = bf16(max|x| / 7); code u stands for (u - 8) * s, u - 8 =
+ * clamp(rint(x / s), -7, 7); a group with an infinity or NaN reads as NaN.
+ * 4.5 bits a value: 144 bytes per (token, kv head) for K and V, where the
+ * bf16 cache takes 512.  csrc/kv4.cuh gives the order of the codes.  A
+ * zero-filled pool reads as zeros.  No counterpart in the reference, whose
+ * cache is bf16 (model/model.py:324-336). */
+
+/* Quantise K/V rows into the pools: row t of k/v, [num_kv_heads][128] bf16
+ * with row and head strides in elements (multiples of 8), goes to flat slot
+ * slot_mapping[t]; negative slots skip.  Slots must be distinct: one named
+ * twice holds an undefined mix of the two rows. */
+int aacc_kv4_store(const void* k, const void* v, int64_t num_tokens, int64_t k_row_stride, int64_t k_head_stride,
+                   int64_t v_row_stride, int64_t v_head_stride, const int64_t* slot_mapping, void* k_cache,
+                   void* v_cache, int64_t num_blocks, int num_kv_heads, int block_size, cudaStream_t stream);
+
+/* Dequantise slots of the pools into bf16 caches [out_blocks][num_kv_heads]
+ * [out_block_size][128]: slot slots[t] goes to flat slot out_slots[t] there
+ * (out_slots NULL: t).  A token with a negative slot on either side is
+ * skipped.  out_block_size is any positive number: 1 makes the output plain
+ * rows [num_tokens][num_kv_heads][128]. */
+int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, int num_kv_heads, int block_size,
+                  const int64_t* slots, const int64_t* out_slots, int64_t num_tokens, void* k_out, void* v_out,
+                  int64_t out_blocks, int out_block_size, cudaStream_t stream);
+
+/* Workspace bytes of aacc_kv4_decode_attention on the current device for any
+ * batch and context (zero-fill it once, before its first use). */
+int64_t aacc_kv4_decode_workspace_bytes(int num_q_heads, int num_kv_heads);
+
+/* Decode attention of one query token per row over its context of
+ * seqlens[row] + ctx_add tokens in 4-bit pools; arguments as
+ * aacc_paged_decode_attention.  A context longer than max_context is cut
+ * there (error word bit 32); an empty one, a padding row (negative slot
+ * index) or one outside [0, num_rows) (bit 2) gives zeros.  Calls that share a workspace must be ordered on one
+ * stream. */
+int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, const void* v_cache, int64_t num_blocks,
+                              const int32_t* block_tables, int64_t num_rows, int64_t max_blocks,
+                              const int64_t* slot_indices, const int32_t* seqlens, int ctx_add, int64_t batch, int num_q_heads, int num_kv_heads,
+                              int block_size, float scale, int64_t max_context, void* workspace,
+                              int64_t workspace_bytes, cudaStream_t stream);
+
 /* ---- RMSNorm ------------------------------------------------------------- */
 
 /* y = w * bf16(x * rsqrt(mean(x^2) + eps)), rows of `hidden` (multiple of

@@ -1,0 +1,95 @@
+"""The 4-bit KV cache and request maps without a GPU: the oracle's storage format, and what the entry points
+refuse before any CUDA call."""
+import pytest
+import torch
+
+from awesome_acceleration_b200 import _lib
+from awesome_acceleration_b200 import kernels as K
+from oracle import kv4 as O
+
+BF = torch.bfloat16
+
+
+def test_every_nibble_has_one_place_and_packing_round_trips():
+    for value in (False, True):
+        assert sorted(O.nibble_places(value).flatten().tolist()) == list(range(2 * 4096))
+        x = torch.randn((3, 64, 128), generator=torch.Generator().manual_seed(int(value))).to(BF)
+        n, s = O.quantise(x)
+        rec = O.pack(x, value)
+        assert rec.shape == (3, 4608)
+        assert torch.equal(O.unpack(rec, value), n.double() * s.double().repeat_interleave(32, -1))
+        # a value is at most half a step of its group's scale off (7 s rounds within 2^-8 of max|x|)
+        step = s.double().repeat_interleave(32, -1)
+        assert ((O.unpack(rec, value) - x.double()).abs() <= step * (0.5 + 7 * 2.0 ** -8)).all()
+
+
+def test_cache_shape():
+    assert K.kv4_cache_shape(10, 8, 256) == (10, 8, 4, 4608)
+    for bs in (0, -64, 63, 100):
+        with pytest.raises(ValueError):
+            K.kv4_cache_shape(1, 1, bs)
+
+
+def test_wrappers_refuse_tensors_off_the_gpu_and_of_other_types_and_shapes():
+    pool = torch.zeros(K.kv4_cache_shape(2, 2, 64), dtype=torch.uint8)
+    rows, slots = torch.zeros((3, 2, 128), dtype=BF), torch.zeros(3, dtype=torch.int64)
+    i32 = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        K.kv4_store(rows, rows, slots, pool, pool)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        K.kv4_load(pool, pool, slots)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        K.kv4_decode_attention(rows, pool, pool, i32.view(1, 3), slots, i32, ctx_add=0, scale=1.0, max_context=64,
+                               workspace=None)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        K.build_block_tables(i32, 64, max_blocks=2)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        K.build_slot_maps(i32, i32.view(1, 3), block_size=64, num_blocks=1, num_tokens=3)
+    with pytest.raises(ValueError, match="k_cache"):
+        K.kv4_store(rows, rows, slots, pool.to(torch.int8), pool)
+    with pytest.raises(ValueError, match="lengths"):
+        K.build_block_tables(i32.long(), 64, max_blocks=2)
+    with pytest.raises(ValueError, match="lengths"):
+        K.build_slot_maps(i32.view(1, 3), i32.view(1, 3), block_size=64, num_blocks=1, num_tokens=3)
+
+
+def test_c_abi_checks_arguments_before_any_cuda_call():
+    lib = _lib.load()
+    st = lib.aacc_kv4_store
+
+    def store(T=3, ks=256, kh=128, nb=2, hkv=2, bs=64, k=16):
+        return st(k, 16, T, ks, kh, 256, 128, 16, 16, 16, nb, hkv, bs, None)
+    for kw in (dict(T=-1), dict(nb=0), dict(hkv=0), dict(bs=0), dict(bs=96), dict(ks=100), dict(kh=127), dict(k=8),
+               dict(T=2 ** 40, hkv=8)):
+        assert store(**kw) == 1, kw
+        assert b"kv4_store" in lib.aacc_last_error()
+    assert store(T=0) == 0
+
+    def load(T=3, nb=2, hkv=2, bs=64, ob=3, obs=1, k=16):
+        return lib.aacc_kv4_load(k, 16, nb, hkv, bs, 16, None, T, 16, 16, ob, obs, None)
+    for kw in (dict(T=-1), dict(nb=0), dict(hkv=0), dict(bs=100), dict(ob=-1), dict(obs=0), dict(k=8), dict(T=2 ** 40)):
+        assert load(**kw) == 1, kw
+        assert b"kv4_load" in lib.aacc_last_error()
+    assert load(T=0) == 0
+
+    def attend(B=2, hq=4, hkv=2, bs=64, nb=2, mb=2, rows=2, ctx=128, q=16):
+        return lib.aacc_kv4_decode_attention(q, 16, 16, 16, nb, 16, rows, mb, 16, 16, 1, B, hq, hkv, bs, 0.1, ctx, None,
+                                             0, None)
+    for kw in (dict(B=-1), dict(hkv=0), dict(hq=0), dict(hq=5), dict(bs=96), dict(bs=0), dict(nb=0), dict(mb=0),
+               dict(rows=-1), dict(ctx=0), dict(q=8)):
+        assert attend(**kw) == 1, kw
+        assert b"kv4_decode_attention" in lib.aacc_last_error()
+    for hq in (6, 32):
+        assert attend(hq=hq) == 3, hq  # 3 and 16 query heads per kv head
+    assert attend(B=0) == 0
+
+    def tables(S=2, bs=64, nf=4, mb=2):
+        return lib.aacc_build_block_tables(16, S, bs, None, nf, 16, mb, None, None)
+    for kw in (dict(S=-1), dict(S=2 ** 31), dict(bs=0), dict(nf=-1), dict(mb=0)):
+        assert tables(**kw) == 1, kw
+    assert tables(S=0) == 0
+
+    def maps(S=2, nr=2, mb=2, bs=64, nb=2, T=4):
+        return lib.aacc_build_slot_maps(16, None, None, S, 16, nr, mb, bs, nb, 16, None, 16, T, None)
+    for kw in (dict(S=-1), dict(nr=-1), dict(mb=0), dict(bs=0), dict(nb=0), dict(T=-1), dict(T=2 ** 31)):
+        assert maps(**kw) == 1, kw
