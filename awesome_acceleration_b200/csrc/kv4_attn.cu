@@ -6,26 +6,37 @@
 // has about 400 cycles per 64 tokens, so the expansion of the codes has to
 // stay near one instruction a value, and there is no time for barriers.
 //
-// Work: the unit is a tile of 64 tokens of one (row, kv head), an item is all
-// tiles of one (row, kv head).  The kernel is persistent: one CTA of 16 warps
-// per SM, grouped into teams of TEAM warps; the N units of the batch, which
-// every CTA counts itself from seqlens, are cut into equal runs, one per team,
-// whatever the rows' lengths are.  A run that ends inside an item leaves an
-// fp32 partial (max, sum, O); the last team of the item to arrive merges the
-// partials in order.
+// Work: the kernel is persistent, one CTA of 16 warps per SM, grouped into
+// teams of T = 1, 2, 4, 8 or 16 warps.  An item is one (row, kv head), a unit
+// a round of T tiles of 64 tokens of an item, one for each warp of a team.
+// Every CTA counts the batch's units itself from seqlens and takes the T
+// that leaves the longest run shortest (the largest such T: fewer partials);
+// the units are cut into equal runs, one per team, whatever the rows' lengths
+// are.  A run that ends inside an item leaves an fp32 partial (max, sum, O);
+// the last team of the item to arrive merges the partials in order.
 //
 // Tiles: each warp streams its own tiles through one K and one V buffer with
 // bulk copies (lane 0 issues; the next K is fetched during softmax and P.V,
-// the next V during the next Q.K), so warps never wait for one another.
+// the next V during the next Q.K), so warps never wait for one another but at
+// the end of a team's item.  A tile is worked on in halves of 32 tokens, in a
+// rolled loop: straight-line code for whole tiles spent a fifth of a small
+// call on instruction fetches.
 //
-// Q.K: the tile's tokens are the rows of m16n8k16's A operand, the G <= 8
-// query heads its 8 columns.  A code u becomes the bf16 16 + u by one shift
-// and one and-or; 24 sum(q) is taken off through the accumulator's start value,
-// which leaves sum(q n) in fp32.  The group's scale multiplies the fp32 sum.
-// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand, whose values
-// are 128 + u - 136, exact in bf16; the V scale of (token, group) multiplies p
-// in fp32, and the product is rounded once to bf16, the only rounding before
-// the output's (as P alone is in the bf16 kernels).
+// Q.K: the tokens are the rows of m16n8k16's A operand, the G <= 8 query heads
+// its 8 columns.  A code u becomes 1024 + u or 1024 + 16 u in fp16 by one
+// and-or where it lies, then u - 8 by one fp16x2 add or fma, exactly.  q is
+// scaled by a power of two per head to a largest element in [2^14, 2^15), so
+// that bf16 values go into fp16 unrounded down to 2^-28 of the largest.  The
+// group's scale multiplies the fp32 sum.
+// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand; the V scale of
+// (token, group) multiplies p in fp32, and the product is rounded once, to
+// fp16: 2^-12, an eighth of bf16's.  It is kept in range by a power of two,
+// 2^10 over the largest V scale so far, so that all products within 2^-24 of
+// the largest possible one keep their 11 bits.
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
 #include "host.h"
 #include "kv4.cuh"
 
@@ -34,14 +45,16 @@ namespace aacc {
 constexpr int kAttWarps = 16;
 constexpr int kAttThreads = kAttWarps * 32;
 
-template <int G, int TEAM>
+template <int G>
 struct Kv4Smem {
   uint8_t k[kAttWarps][kKv4Record];
   uint8_t v[kAttWarps][kKv4Record];
-  float red_o[TEAM > 1 ? kAttWarps : 1][G][128];
-  float red_ml[TEAM > 1 ? kAttWarps : 1][G][2];
-  int64_t pre[kAttThreads];
-  int64_t wsum[kAttWarps];
+  float red_o[kAttWarps][G][128];
+  float red_ml[kAttWarps][G][2];
+  uint32_t pre[kAttThreads];  // units before thread i's rows, per kv head
+  int row[kAttThreads];       // of batches up to kAttThreads rows
+  int ctx[kAttThreads];
+  uint32_t wsum[5][kAttWarps];
   uint64_t kfull[kAttWarps];
   uint64_t vfull[kAttWarps];
   int last[kAttWarps];
@@ -60,44 +73,61 @@ struct Kv4Args {
   float* ws_o;    // [2 * teams][G][128]
   float* ws_ml;   // [2 * teams][G][2]
   unsigned* err;
-  int64_t num_blocks, num_rows, max_blocks, batch;
-  int max_ctx, ctx_add, Hkv, tpb;  // tpb: tiles per block
+  int64_t num_blocks, max_blocks;
+  int num_rows, batch, max_ctx, ctx_add, Hkv, tpb;  // tpb: tiles per block
   float scale;
 };
 
 // A run of tiles [t0, t1) of item (b, h), whose row has n tiles; u is the unit number of t0.
 struct Kv4Seg {
-  int64_t u, b, row;
-  int h, n, t0, t1, ctx;
+  uint32_t u;
+  int b, row, h, n, t0, t1, ctx;
 };
 
 // Tokens of batch row b (0: padding, outside the tables, or empty).
-__device__ __forceinline__ int kv4_ctx(const Kv4Args& a, int64_t b, int64_t* row) {
+__device__ __forceinline__ int kv4_ctx(const Kv4Args& a, int b, int* row) {
   const int64_t r = a.rows[b];
-  *row = r;
-  if (r < 0 || r >= a.num_rows) return 0;
+  if (r < 0 || r >= a.num_rows) {
+    *row = r < 0 ? -1 : a.num_rows;
+    return 0;
+  }
+  *row = (int)r;
   const int64_t c = (int64_t)a.seqlens[r] + a.ctx_add;
   return (int)max((int64_t)0, min(c, (int64_t)a.max_ctx));
 }
 
-__device__ __forceinline__ void kv4_row(const Kv4Args& a, Kv4Seg& s) {
-  s.ctx = kv4_ctx(a, s.b, &s.row);
-  s.n = (s.ctx + kKv4Tile - 1) / kKv4Tile;
+__device__ __forceinline__ int tiles_of(int ctx) { return (int)(((unsigned)ctx + kKv4Tile - 1) / kKv4Tile); }
+
+template <int G>
+__device__ __forceinline__ void kv4_row(const Kv4Args& a, const Kv4Smem<G>& sm, Kv4Seg& s) {
+  if (a.batch <= kAttThreads) {
+    s.ctx = sm.ctx[s.b];
+    s.row = sm.row[s.b];
+  } else {
+    s.ctx = kv4_ctx(a, s.b, &s.row);
+  }
+  s.n = tiles_of(s.ctx);
+}
+
+// Tiles of a segment that starts at t0 with `units` units left in its run.
+__device__ __forceinline__ int seg_end(int n, int t0, uint32_t units, int tsh) {
+  return (int)min((uint64_t)n, (uint64_t)t0 + ((uint64_t)units << tsh));
 }
 
 // The run's next segment; false when the run is over.
-__device__ __forceinline__ bool kv4_next(const Kv4Args& a, Kv4Seg& s, int64_t uend) {
-  s.u += s.t1 - s.t0;
+template <int G>
+__device__ __forceinline__ bool kv4_next(const Kv4Args& a, const Kv4Smem<G>& sm, Kv4Seg& s, uint32_t uend, int tsh) {
+  s.u += (uint32_t)(s.t1 - s.t0 + (1 << tsh) - 1) >> tsh;
   if (s.u >= uend) return false;
-  s.t0 = 0;  // within a run only its end cuts an item short
-  if (++s.h == a.Hkv) {
+  if (++s.h == a.Hkv) {  // within a run only its end cuts an item short
     s.h = 0;
     do {
       ++s.b;
-      kv4_row(a, s);
+      kv4_row(a, sm, s);
     } while (s.n == 0);
   }
-  s.t1 = (int)min((int64_t)s.n, uend - s.u);
+  s.t0 = 0;
+  s.t1 = seg_end(s.n, 0, uend - s.u, tsh);
   return true;
 }
 
@@ -115,74 +145,76 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   return y;
 }
 
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Nibbles R and R + 4 of x as the bf16 pair (16 + u, 16 + u').
-template <int R>
-__device__ __forceinline__ uint32_t code16(uint32_t x) {
-  const uint32_t y = R == 0 ? x << 3 : x >> (4 * R - 3);
-  return (y & 0x00780078u) | 0x41804180u;
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Nibbles R and R + 4 of x as the bf16 pair (u - 8, u' - 8).
-template <int R>
-__device__ __forceinline__ uint32_t code_exact(uint32_t x) {
-  const uint32_t y = ((x >> (4 * R)) & 0x000f000fu) | 0x43004300u;  // 128 + u
-  const __nv_bfloat162 off = __float2bfloat162_rn(-136.f);
-  const __nv_bfloat162 r = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&y), off);
+// Bits 0-3 (HI: 4-7) of both halves of x, a code u each, as the fp16 pair (u - 8, u' - 8).
+template <bool HI>
+__device__ __forceinline__ uint32_t code(uint32_t x) {
+  const uint32_t y = (x & (HI ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;  // 1024 + u, or 1024 + 16 u
+  const __half2 h = *reinterpret_cast<const __half2*>(&y);
+  const __half2 r = HI ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f))
+                       : __hadd2(h, __float2half2_rn(-1032.f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-template <int TEAM>
-__device__ __forceinline__ void team_sync(int team) {
-  if constexpr (TEAM == 1)
+// bf16 pair W / 2 of `p`, member W % 2, as fp32.
+template <int W>
+__device__ __forceinline__ float scale_of(uint2 p) {
+  const uint32_t x = W < 2 ? p.x : p.y;
+  return __uint_as_float((W & 1) ? x & 0xffff0000u : x << 16);
+}
+
+__device__ __forceinline__ void team_sync(int team, int tsh) {
+  if (tsh == 0)
     __syncwarp();
   else
-    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM * 32) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(32 << tsh) : "memory");
 }
 
-// Merge the parts of an item (team k0's tail, then the heads of k0 + 1 .. k0 + parts - 1) in order.
-template <int G, int TEAM>
-__device__ __forceinline__ void kv4_merge(const Kv4Args& a, int64_t k0, int parts, int64_t qh0, int tid) {
-  for (int i = tid; i < G * 32; i += TEAM * 32) {
-    const int g = i >> 5, d4 = i & 31;
-    float M = -INFINITY;
-    for (int p = 0; p < parts; ++p) {
-      const int64_t slot = 2 * (k0 + p) + (p == 0);
-      M = fmaxf(M, __ldcg(a.ws_ml + (slot * G + g) * 2));
-    }
-    const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < parts; ++p) {
-      const int64_t slot = 2 * (k0 + p) + (p == 0);
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + slot * G + g);
-      const float4 o = __ldcg(reinterpret_cast<const float4*>(a.ws_o) + (slot * G + g) * 32 + d4);
-      const float f = ex2(ml.x - mu);
-      L += f * ml.y;
-      O.x += f * o.x;
-      O.y += f * o.y;
-      O.z += f * o.z;
-      O.w += f * o.w;
-    }
-    const float inv = 1.f / L;
-    reinterpret_cast<uint2*>(a.out + (qh0 + g) * 128)[d4] =
-        make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
+// Running (max, sum, O) of partial results that are weighted 2^max.
+struct Kv4Acc {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float pm, float pl, float4 po) {
+    const float n = fmaxf(m, pm);
+    const float u = n == -INFINITY ? 0.f : n;
+    const float f = ex2(m - u), g = ex2(pm - u);
+    m = n;
+    l = l * f + pl * g;
+    o.x = o.x * f + po.x * g;
+    o.y = o.y * f + po.y * g;
+    o.z = o.z * f + po.z * g;
+    o.w = o.w * f + po.w * g;
   }
-}
+  __device__ __forceinline__ uint2 result() const {
+    const float inv = 1.f / l;
+    return make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  }
+};
 
-template <int G, int TEAM>
+template <int G>
 __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Args a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  using Smem = Kv4Smem<G, TEAM>;
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  Kv4Smem<G>& sm = *reinterpret_cast<Kv4Smem<G>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int team = warp / TEAM, wt = warp % TEAM;
   if (lane == 0) {
     mbar_init(&sm.kfull[warp], 1);
     mbar_init(&sm.vfull[warp], 1);
@@ -192,41 +224,57 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   griddep_wait();
   griddep_launch();
 
-  // ---- count the batch's units: every thread sums a run of rows, then a scan over the CTA
-  const int64_t per = (a.batch + kAttThreads - 1) / kAttThreads;
-  int64_t mine = 0;
-  for (int64_t b = threadIdx.x * per; b < min(a.batch, (threadIdx.x + 1) * per); ++b) {
-    int64_t row;
-    mine += (kv4_ctx(a, b, &row) + kKv4Tile - 1) / kKv4Tile;
-  }
-  int64_t inc = mine;
+  // ---- count the batch's units for every team size: each thread sums a run of rows, then the CTA
+  const int per = (a.batch + kAttThreads - 1) / kAttThreads;
+  const int b_lo = min(a.batch, (int)threadIdx.x * per), b_hi = min(a.batch, b_lo + per);
+  uint32_t cnt[5] = {0, 0, 0, 0, 0};
+  for (int b = b_lo; b < b_hi; ++b) {
+    int row;
+    const int ctx = kv4_ctx(a, b, &row);
+    if (per == 1) {
+      sm.ctx[b] = ctx;
+      sm.row[b] = row;
+    }
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += y;
+    for (int i = 0; i < 5; ++i) cnt[i] += (uint32_t)(tiles_of(ctx) + (1 << i) - 1) >> i;
   }
-  if (lane == 31) sm.wsum[warp] = inc;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    const uint32_t x = __reduce_add_sync(0xffffffffu, cnt[i]);
+    if (lane == 0) sm.wsum[i][warp] = x;
+  }
   __syncthreads();
-  int64_t before = 0, total = 0;
+  int tsh = 0;
+  uint32_t N = 0, chunk = 0xffffffffu, before = 0;
 #pragma unroll
-  for (int w = 0; w < kAttWarps; ++w) {
-    const int64_t x = sm.wsum[w];
-    if (w < warp) before += x;
-    total += x;
+  for (int i = 0; i < 5; ++i) {
+    const uint32_t mine = lane < kAttWarps ? sm.wsum[i][lane] : 0;
+    const uint32_t n = __reduce_add_sync(0xffffffffu, mine) * a.Hkv;
+    const uint32_t teams = gridDim.x * (kAttWarps >> i);
+    const uint32_t ch = (n + teams - 1) / teams;
+    if (ch <= chunk) {
+      tsh = i;
+      N = n;
+      chunk = ch;
+      before = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    }
+  }
+  uint32_t mine = cnt[0];
+#pragma unroll
+  for (int i = 1; i < 5; ++i) mine = tsh == i ? cnt[i] : mine;
+  uint32_t inc = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += y;
   }
   sm.pre[threadIdx.x] = before + inc - mine;
   __syncthreads();
 
   // ---- this team's run of units
-  constexpr int kTeams = kAttWarps / TEAM;
-  const int64_t N = total * a.Hkv;
-  const int64_t teams = (int64_t)gridDim.x * kTeams;
-  const int64_t chunk = max((N + teams - 1) / teams, (int64_t)TEAM);
-  const int64_t k = (int64_t)team * gridDim.x + blockIdx.x;  // runs go round the SMs, so few runs use many of them
-  const int64_t u0 = k * chunk, uend = min(u0 + chunk, N);
-  uint32_t ph = 0;                 // parity of the tile in hand, for both buffers
-  bool dead = false;               // a copy did not come in time: no more loads, no more tiles
-  uint32_t kph = 0;                // then: the parity that the K buffer still waits for
+  const int team = warp >> tsh, wt = warp & ((1 << tsh) - 1), T = 1 << tsh;
+  const uint32_t k = (uint32_t)team * gridDim.x + blockIdx.x;  // runs go round the SMs: few runs use many of them
+  const uint32_t u0 = (uint32_t)min((uint64_t)k * chunk, (uint64_t)N), uend = min(u0 + chunk, N);
   volatile int* abort = &sm.abort;
 
   if (u0 < uend) {
@@ -240,34 +288,39 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         else
           hi = mid;
       }
-      int64_t u = sm.pre[lo] * a.Hkv;
+      uint32_t u = sm.pre[lo] * a.Hkv;
       cs.b = lo * per;
-      kv4_row(a, cs);
-      while (u + (int64_t)cs.n * a.Hkv <= u0) {
-        u += (int64_t)cs.n * a.Hkv;
+      kv4_row(a, sm, cs);
+      uint32_t rounds = (uint32_t)(cs.n + T - 1) >> tsh;
+      while (u + rounds * a.Hkv <= u0) {
+        u += rounds * a.Hkv;
         ++cs.b;
-        kv4_row(a, cs);
+        kv4_row(a, sm, cs);
+        rounds = (uint32_t)(cs.n + T - 1) >> tsh;
       }
       cs.u = u0;
-      cs.h = (int)((u0 - u) / cs.n);
-      cs.t0 = (int)((u0 - u) - (int64_t)cs.h * cs.n);
-      cs.t1 = (int)min((int64_t)cs.n, cs.t0 + (uend - u0));
+      cs.h = (int)((u0 - u) / rounds);
+      cs.t0 = (int)((u0 - u) - (uint32_t)cs.h * rounds) << tsh;
+      cs.t1 = seg_end(cs.n, cs.t0, uend - u0, tsh);
     }
-    // The loads run one tile ahead of the arithmetic, across segments.
+    // The loads run one tile ahead of the arithmetic, across segments: tile lt of segment ls, which is
+    // tile lti of entry lbi of the row's block table.
     Kv4Seg ls = cs;
     int lt = ls.t0 + wt;
     bool lhas = true;
     while (lhas && lt >= ls.t1) {
-      lhas = kv4_next(a, ls, uend);
+      lhas = kv4_next(a, sm, ls, uend, tsh);
       lt = ls.t0 + wt;
     }
-    auto record = [&](int32_t id) -> int64_t {
-      int64_t blk = id;
+    int lbi = lt / a.tpb, lti = lt - lbi * a.tpb;
+    int32_t lid = lhas ? a.bt[ls.row * a.max_blocks + lbi] : 0;
+    auto record = [&]() -> int64_t {
+      int64_t blk = lid;
       if (blk < 0 || blk >= a.num_blocks) {
         if (lane == 0) report(a.err, ERR_BLOCK_OOB);
         blk = 0;  // a valid address keeps the pipeline going; the result is flagged
       }
-      return kv4_record(blk, ls.h, lt % a.tpb, a.Hkv, a.tpb);
+      return kv4_record(blk, ls.h, lti, a.Hkv, a.tpb);
     };
     auto load_k = [&](int64_t rec) {
       if (lane == 0) {
@@ -282,279 +335,317 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       }
     };
     if (lhas) {
-      const int64_t rec = record(a.bt[ls.row * a.max_blocks + lt / a.tpb]);
+      const int64_t rec = record();
       load_k(rec);
       load_v(rec);
     }
-    const float sl = fabsf(a.scale) * kLog2e;
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns q's sign
+    uint32_t ph = 0;    // parity of the tile in hand, for both buffers
+    bool dead = false;  // a copy did not come in time: no more loads, no more tiles
+    uint32_t kph = 0;   // then: the parity that the K buffer still waits for
 
     while (true) {
       // ---- queries of the item: B operand, column g = query head (columns >= G are zero)
-      const int64_t qh0 = (cs.b * a.Hkv + cs.h) * G;
+      const int64_t qh0 = ((int64_t)cs.b * a.Hkv + cs.h) * G;
       uint32_t qf[4][4];
-      float corr[4][2];
+      float sl0, sl1;  // log2 softmax scale of the raw scores of heads 2c and 2c + 1
+      {
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns q's sign
+        uint32_t mx = 0;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (g < G) x = *reinterpret_cast<const uint4*>(a.q + (qh0 + g) * 128 + 32 * w + 8 * c);
-        qf[w][0] = x.x ^ flip;
-        qf[w][1] = x.y ^ flip;
-        qf[w][2] = x.z ^ flip;
-        qf[w][3] = x.w ^ flip;
-        float s = 0.f;
+        for (int w = 0; w < 4; ++w) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (g < G) x = *reinterpret_cast<const uint4*>(a.q + (qh0 + g) * 128 + 32 * w + 8 * c);
+          qf[w][0] = x.x ^ flip;
+          qf[w][1] = x.y ^ flip;
+          qf[w][2] = x.z ^ flip;
+          qf[w][3] = x.w ^ flip;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float2 f = unpack_bf16(qf[w][r]);
-          s += f.x + f.y;
+          for (int r = 0; r < 4; ++r) mx = max(mx, max(qf[w][r] & 0x7fffu, (qf[w][r] >> 16) & 0x7fffu));
         }
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        corr[w][0] = -24.f * __shfl_sync(0xffffffffu, s, 8 * c);      // head 2c
-        corr[w][1] = -24.f * __shfl_sync(0xffffffffu, s, 8 * c + 4);  // head 2c + 1
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^(14 - e) for a largest element in [2^e, 2^(e + 1)), as far as fp32 goes
+        const int f = min(268 - (int)(mx >> 7), 254);
+        const float up = __uint_as_float((uint32_t)f << 23);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float2 y = unpack_bf16(qf[w][r]);
+            qf[w][r] = pack_f16(y.x * up, y.y * up);
+          }
+        const float down = fabsf(a.scale) * kLog2e * (f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23));
+        sl0 = __shfl_sync(0xffffffffu, down, 8 * c);
+        sl1 = __shfl_sync(0xffffffffu, down, 8 * c + 4);
       }
       float o[8][4];
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      int ev = 10;  // biased exponent of the largest V scale so far (at least 10): O is kept times 2^(264 - 127 - ev)
 
-      for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += TEAM) {
+      for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += T) {
         // the next tile's block id, in flight during Q.K
-        lt += TEAM;
-        while (lhas && lt >= ls.t1) {
-          lhas = kv4_next(a, ls, uend);
-          lt = ls.t0 + wt;
+        if (lhas) {
+          lt += T;
+          lti += T;
+          if (lt >= ls.t1) {
+            do {
+              lhas = kv4_next(a, sm, ls, uend, tsh);
+              lt = ls.t0 + wt;
+            } while (lhas && lt >= ls.t1);
+            lbi = lt / a.tpb;
+            lti = lt - lbi * a.tpb;
+            if (lhas) lid = a.bt[ls.row * a.max_blocks + lbi];
+          } else if (lti >= a.tpb) {
+            const int d = lti / a.tpb;
+            lbi += d;
+            lti -= d * a.tpb;
+            lid = a.bt[ls.row * a.max_blocks + lbi];
+          }
         }
-        const int32_t next_id = lhas ? a.bt[ls.row * a.max_blocks + lt / a.tpb] : 0;
-
-        // ---- S = K Q^T
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.kfull[warp], ph, a.err, abort))) {
           dead = true;
           kph = ph;
           lhas = false;
           break;
         }
-        const uint8_t* kb = sm.k[warp];
-        float s[4][4];
+        int64_t next_rec = 0;
+        int lim = cs.ctx - t * kKv4Tile;  // tokens from here to the end of the context
+        float cv = 0.f;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, lim -= 32) {
+          // ---- S = K Q^T for 32 tokens; lane (g, c): tokens 16 sb + g (+ 8), heads 2c and 2c + 1
+          const uint8_t* kb = sm.k[warp] + half * 2048;
+          const uint8_t* ksc = sm.k[warp] + kKv4Codes + half * 256;
+          float s[2][4];
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          const uint4 x4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + lane * 16);        // token g
-          const uint4 y4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + 512 + lane * 16);  // token g + 8
-          const uint2 sx = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + g) * 8);
-          const uint2 sy = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + g + 8) * 8);
-          const uint32_t xw[4] = {x4.x, x4.y, x4.z, x4.w}, yw[4] = {y4.x, y4.y, y4.z, y4.w};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            float acc[4] = {corr[w][0], corr[w][1], corr[w][0], corr[w][1]};
-            const uint32_t a0[4] = {code16<0>(xw[w]), code16<0>(yw[w]), code16<1>(xw[w]), code16<1>(yw[w])};
-            mma_bf16_16816(acc, a0, qf[w][0], qf[w][1]);
-            const uint32_t a1[4] = {code16<2>(xw[w]), code16<2>(yw[w]), code16<3>(xw[w]), code16<3>(yw[w])};
-            mma_bf16_16816(acc, a1, qf[w][2], qf[w][3]);
-            const uint32_t px = w < 2 ? sx.x : sx.y, py = w < 2 ? sy.x : sy.y;
-            const float fx = __uint_as_float((w & 1) ? px & 0xffff0000u : px << 16);
-            const float fy = __uint_as_float((w & 1) ? py & 0xffff0000u : py << 16);
-            if (w == 0) {
-              s[sb][0] = acc[0] * fx;
-              s[sb][1] = acc[1] * fx;
-              s[sb][2] = acc[2] * fy;
-              s[sb][3] = acc[3] * fy;
-            } else {
-              s[sb][0] += acc[0] * fx;
-              s[sb][1] += acc[1] * fx;
-              s[sb][2] += acc[2] * fy;
-              s[sb][3] += acc[3] * fy;
+          for (int sb = 0; sb < 2; ++sb) {
+            const uint4 x4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + lane * 16);        // token g
+            const uint4 y4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + 512 + lane * 16);  // token g + 8
+            const uint2 sx = *reinterpret_cast<const uint2*>(ksc + (16 * sb + g) * 8);
+            const uint2 sy = *reinterpret_cast<const uint2*>(ksc + (16 * sb + g + 8) * 8);
+            auto group = [&](auto W, uint32_t x, uint32_t y) {
+              constexpr int w = decltype(W)::value;
+              float acc[4] = {0.f, 0.f, 0.f, 0.f};
+              const uint32_t a0[4] = {code<false>(x), code<false>(y), code<true>(x), code<true>(y)};
+              mma_f16_16816(acc, a0, qf[w][0], qf[w][1]);
+              x >>= 8;
+              y >>= 8;
+              const uint32_t a1[4] = {code<false>(x), code<false>(y), code<true>(x), code<true>(y)};
+              mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
+              const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
+              if (w == 0) s[sb][0] = s[sb][1] = s[sb][2] = s[sb][3] = 0.f;
+              s[sb][0] = fmaf(acc[0], fx, s[sb][0]);
+              s[sb][1] = fmaf(acc[1], fx, s[sb][1]);
+              s[sb][2] = fmaf(acc[2], fy, s[sb][2]);
+              s[sb][3] = fmaf(acc[3], fy, s[sb][3]);
+            };
+            group(std::integral_constant<int, 0>{}, x4.x, y4.x);
+            group(std::integral_constant<int, 1>{}, x4.y, y4.y);
+            group(std::integral_constant<int, 2>{}, x4.z, y4.z);
+            group(std::integral_constant<int, 3>{}, x4.w, y4.w);
+          }
+          const bool done = half == 1 || lim <= 32;  // no more tokens in this tile
+          if (done) {
+            __syncwarp();  // every lane has read the K buffer
+            if (lhas) {
+              next_rec = record();
+              load_k(next_rec);
             }
           }
-        }
-        __syncwarp();  // every lane has read the K buffer
-        int64_t next_rec = 0;
-        if (lhas) {
-          next_rec = record(next_id);
-          load_k(next_rec);
-        }
 
-        // ---- online softmax, log2 domain; lane (g, c): tokens 16 sb + g (+ 8), heads 2c and 2c + 1
-        const int lim = cs.ctx - t * kKv4Tile;
-        if (lim < kKv4Tile) {
+          // ---- online softmax in the log2 domain
+          if (lim < 32) {
 #pragma unroll
-          for (int sb = 0; sb < 4; ++sb) {
-            if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = -INFINITY;
-            if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = -INFINITY;
+            for (int sb = 0; sb < 2; ++sb) {
+              if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = -INFINITY;
+              if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = -INFINITY;
+            }
           }
-        }
-        float x0 = s[0][0], x1 = s[0][1];
+          float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
+          float x1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          x0 = fmaxf(x0, fmaxf(s[sb][0], s[sb][2]));
-          x1 = fmaxf(x1, fmaxf(s[sb][1], s[sb][3]));
-        }
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-        }
-        const float n0 = fmaxf(m0, x0 * sl), n1 = fmaxf(m1, x1 * sl);  // a tile has a token: finite
-        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-          const float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
-          l0 *= a0;
-          l1 *= a1;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            o[j][0] *= a0;
-            o[j][1] *= a1;
-            o[j][2] *= a0;
-            o[j][3] *= a1;
+          for (int d = 4; d < 32; d <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
           }
+          const float n0 = fmaxf(m0, x0 * sl0), n1 = fmaxf(m1, x1 * sl1);  // these tokens are in the context: finite
+          float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
           m0 = n0;
           m1 = n1;
-        }
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          s[sb][0] = ex2(fmaf(s[sb][0], sl, -m0));
-          s[sb][1] = ex2(fmaf(s[sb][1], sl, -m1));
-          s[sb][2] = ex2(fmaf(s[sb][2], sl, -m0));
-          s[sb][3] = ex2(fmaf(s[sb][3], sl, -m1));
-        }
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.vfull[warp], ph, a.err, abort))) {
-          dead = true;
-          kph = lhas ? ph ^ 1 : ph;
-          lhas = false;
-          break;
-        }
-        ph ^= 1;
-        if (lim < kKv4Tile) {
-          // Behind the context: no weight (also where sl = 0 makes -inf * sl a NaN), and no V scale,
-          // which may be anything there.
-#pragma unroll
-          for (int sb = 0; sb < 4; ++sb) {
-            if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = 0.f;
-            if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = 0.f;
+          for (int sb = 0; sb < 2; ++sb) {
+            s[sb][0] = ex2(fmaf(s[sb][0], sl0, -m0));
+            s[sb][1] = ex2(fmaf(s[sb][1], sl1, -m1));
+            s[sb][2] = ex2(fmaf(s[sb][2], sl0, -m0));
+            s[sb][3] = ex2(fmaf(s[sb][3], sl1, -m1));
           }
-          for (int i = lane; i < kKv4Tile; i += 32)
-            if (i >= lim) *reinterpret_cast<uint2*>(sm.v[warp] + kKv4Codes + 8 * i) = make_uint2(0, 0);
-          fence_proxy_async();  // before the bulk copy that overwrites the buffer
-          __syncwarp();
-        }
+          if (lim < 32) {  // also where a scale of 0 makes -inf * 0 a NaN
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          l0 += s[sb][0] + s[sb][2];
-          l1 += s[sb][1] + s[sb][3];
-        }
+            for (int sb = 0; sb < 2; ++sb) {
+              if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = 0.f;
+              if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = 0.f;
+            }
+          }
+          l0 = l0 * a0 + (s[0][0] + s[0][2]) + (s[1][0] + s[1][2]);
+          l1 = l1 * a1 + (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
 
-        // ---- O^T += V^T P^T
-        const uint8_t* vb = sm.v[warp];
-#pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
-          const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
-          const uint2 sx = *reinterpret_cast<const uint2*>(vb + kKv4Codes + (16 * sb + g) * 8);
-          const uint2 sy = *reinterpret_cast<const uint2*>(vb + kKv4Codes + (16 * sb + g + 8) * 8);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {  // 32 dims: j = 2w and 2w + 1
-            const uint32_t px = w < 2 ? sx.x : sx.y, py = w < 2 ? sy.x : sy.y;
-            const float fx = __uint_as_float((w & 1) ? px & 0xffff0000u : px << 16);
-            const float fy = __uint_as_float((w & 1) ? py & 0xffff0000u : py << 16);
-            const uint32_t b0 = movmatrix_trans(pack_bf16(s[sb][0] * fx, s[sb][1] * fx));
-            const uint32_t b1 = movmatrix_trans(pack_bf16(s[sb][2] * fy, s[sb][3] * fy));
-            // the words' 16 bits of tokens 2c | 2c + 1: four nibbles = dims 16 j + 2g, + 1 of j = 2w, 2w + 1
-            const uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
-            const uint32_t lo = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
-            const uint32_t hi = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
-            const uint32_t a0[4] = {code_exact<0>(lo), code_exact<1>(lo), code_exact<0>(hi), code_exact<1>(hi)};
-            mma_bf16_16816(o[2 * w], a0, b0, b1);
-            const uint32_t a1[4] = {code_exact<2>(lo), code_exact<3>(lo), code_exact<2>(hi), code_exact<3>(hi)};
-            mma_bf16_16816(o[2 * w + 1], a1, b0, b1);
+          if (half == 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&sm.vfull[warp], ph, a.err, abort))) {
+              dead = true;
+              kph = lhas && done ? ph ^ 1 : ph;
+              lhas = false;
+              break;
+            }
+            // The tile's largest V scale (they are not negative: their bits order as they do); lane: tokens
+            // 2 lane and 2 lane + 1.  Behind the context a scale may be anything: it becomes zero.
+            uint4* vs = reinterpret_cast<uint4*>(sm.v[warp] + kKv4Codes) + lane;
+            uint4 x = *vs;
+            if (lim < kKv4Tile) {
+              if (2 * lane >= lim) x.x = x.y = 0;
+              if (2 * lane + 1 >= lim) x.z = x.w = 0;
+              *vs = x;
+              fence_proxy_async();  // before the bulk copy that overwrites the buffer
+              __syncwarp();
+            }
+            const uint32_t hi = max(max(x.x, x.y), max(x.z, x.w)) >> 16;
+            const uint32_t lo = max(max(x.x & 0xffffu, x.y & 0xffffu), max(x.z & 0xffffu, x.w & 0xffffu));
+            const int e = (int)(__reduce_max_sync(0xffffffffu, max(hi, lo)) >> 7);
+            if (e > ev) {
+              const float f = ex2((float)(ev - e));
+              a0 *= f;
+              a1 *= f;
+              ev = e;
+            }
+            cv = __uint_as_float((uint32_t)(264 - ev) << 23);
           }
+          if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              o[j][0] *= a0;
+              o[j][1] *= a1;
+              o[j][2] *= a0;
+              o[j][3] *= a1;
+            }
+          }
+
+          // ---- O^T += V^T P^T
+          const uint8_t* vb = sm.v[warp] + half * 2048;
+          const uint8_t* vsc = sm.v[warp] + kKv4Codes + half * 256;
+#pragma unroll
+          for (int sb = 0; sb < 2; ++sb) {
+            const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
+            const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
+            const uint2 sx = *reinterpret_cast<const uint2*>(vsc + (16 * sb + g) * 8);
+            const uint2 sy = *reinterpret_cast<const uint2*>(vsc + (16 * sb + g + 8) * 8);
+            const float p0 = s[sb][0] * cv, p1 = s[sb][1] * cv, p2 = s[sb][2] * cv, p3 = s[sb][3] * cv;
+            auto group = [&](auto W) {  // 32 dims: j = 2w and 2w + 1
+              constexpr int w = decltype(W)::value;
+              const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
+              const uint32_t b0 = movmatrix_trans(pack_f16(p0 * fx, p1 * fx));
+              const uint32_t b1 = movmatrix_trans(pack_f16(p2 * fy, p3 * fy));
+              // 16 bits of tokens 2c | 2c + 1 each: four nibbles = dims 16 j + 2g, + 1 of j = 2w, 2w + 1
+              constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
+              uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
+              uint32_t y = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
+              const uint32_t a0[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
+              mma_f16_16816(o[2 * w], a0, b0, b1);
+              x >>= 8;
+              y >>= 8;
+              const uint32_t a1[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
+              mma_f16_16816(o[2 * w + 1], a1, b0, b1);
+            };
+            group(std::integral_constant<int, 0>{});
+            group(std::integral_constant<int, 1>{});
+            group(std::integral_constant<int, 2>{});
+            group(std::integral_constant<int, 3>{});
+          }
+          if (done) break;
         }
+        if (dead) break;
+        ph ^= 1;
         __syncwarp();  // every lane has read the V buffer
         if (lhas) load_v(next_rec);
       }
 
-      // ---- end of the segment
+      // ---- end of the segment: the team's warps meet in shared memory
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
       }
+      const float down = __uint_as_float((uint32_t)max(ev - 10, 0) << 23) + (ev == 10 ? 0x1p-127f : 0.f);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // o[j][e], o[j][2 + e]: dims 16 j + 2g and + 1 of head 2c + e
+        const int hd = 2 * c + e;
+        if (hd < G) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float2*>(&sm.red_o[warp][hd][16 * j + 2 * g]) =
+                make_float2(o[j][e] * down, o[j][2 + e] * down);
+          if (g == 0) *reinterpret_cast<float2*>(sm.red_ml[warp][hd]) = make_float2(e ? m1 : m0, e ? l1 : l0);
+        }
+      }
+      team_sync(team, tsh);
       const bool whole = cs.t0 == 0 && cs.t1 == cs.n;
-      const int64_t slot = 2 * k + (cs.t0 == 0);
-      if constexpr (TEAM == 1) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {  // heads 2c and 2c + 1; o[j][e], o[j][2 + e] are dims 16 j + 2g, + 1
-          const int hd = 2 * c + e;
-          if (hd < G) {
-            const float inv = 1.f / (e ? l1 : l0);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int d = 16 * j + 2 * g;
-              if (whole)
-                *reinterpret_cast<uint32_t*>(a.out + (qh0 + hd) * 128 + d) = pack_bf16(o[j][e] * inv, o[j][2 + e] * inv);
-              else
-                *reinterpret_cast<float2*>(a.ws_o + (slot * G + hd) * 128 + d) = make_float2(o[j][e], o[j][2 + e]);
-            }
-            if (!whole && g == 0)
-              reinterpret_cast<float2*>(a.ws_ml)[slot * G + hd] = make_float2(e ? m1 : m0, e ? l1 : l0);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int hd = 2 * c + e;
-          if (hd < G) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<float2*>(&sm.red_o[warp][hd][16 * j + 2 * g]) = make_float2(o[j][e], o[j][2 + e]);
-            if (g == 0) {
-              sm.red_ml[warp][hd][0] = e ? m1 : m0;
-              sm.red_ml[warp][hd][1] = e ? l1 : l0;
-            }
-          }
-        }
-        team_sync<TEAM>(team);
-        for (int i = wt * 32 + lane; i < G * 32; i += TEAM * 32) {
-          const int hd = i >> 5, d4 = i & 31;
-          float M = -INFINITY;
-#pragma unroll
-          for (int w = 0; w < TEAM; ++w) M = fmaxf(M, sm.red_ml[team * TEAM + w][hd][0]);
-          const float mu = M == -INFINITY ? 0.f : M;
-          float L = 0.f;
-          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int w = 0; w < TEAM; ++w) {
-            const float f = ex2(sm.red_ml[team * TEAM + w][hd][0] - mu);
-            const float4 x = reinterpret_cast<const float4*>(sm.red_o[team * TEAM + w][hd])[d4];
-            L += f * sm.red_ml[team * TEAM + w][hd][1];
-            O.x += f * x.x;
-            O.y += f * x.y;
-            O.z += f * x.z;
-            O.w += f * x.w;
-          }
-          if (whole) {
-            const float inv = 1.f / L;
-            reinterpret_cast<uint2*>(a.out + (qh0 + hd) * 128)[d4] =
-                make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
-          } else {
-            reinterpret_cast<float4*>(a.ws_o)[(slot * G + hd) * 32 + d4] = O;
-            if (d4 == 0) reinterpret_cast<float2*>(a.ws_ml)[slot * G + hd] = make_float2(M, L);
-          }
+      const uint32_t slot = 2 * k + (cs.t0 == 0);
+      for (int hd = wt; hd < G; hd += T) {
+        Kv4Acc acc;
+        for (int w = team << tsh; w < (team + 1) << tsh; ++w)
+          acc.add(sm.red_ml[w][hd][0], sm.red_ml[w][hd][1], reinterpret_cast<const float4*>(sm.red_o[w][hd])[lane]);
+        if (whole) {
+          reinterpret_cast<uint2*>(a.out + (qh0 + hd) * 128)[lane] = acc.result();
+        } else {
+          reinterpret_cast<float4*>(a.ws_o)[((int64_t)slot * G + hd) * 32 + lane] = acc.o;
+          if (lane == 0) reinterpret_cast<float2*>(a.ws_ml)[(int64_t)slot * G + hd] = make_float2(acc.m, acc.l);
         }
       }
       if (!whole) {
-        // The item's first unit lies in run k0, its last in run k1; the last of them to get here merges.
-        const int64_t first = cs.u - cs.t0;
-        const int64_t k0 = first / chunk;
-        const int parts = (int)((first + cs.n - 1) / chunk - k0) + 1;
+        // The item's first unit lies in run k0, its last in run k0 + parts - 1; the last of them to get
+        // here merges: run k0's tail (slot 2 k0 + 1), then the heads of the others (2 k), in this order
+        // within each of `sl` slices that the team's warps share out.
+        const uint32_t first = cs.u - (cs.t0 >> tsh);
+        const uint32_t k0 = first / chunk;
+        const int parts = (int)((first + ((uint32_t)(cs.n + T - 1) >> tsh) - 1) / chunk - k0) + 1;
         __threadfence();
-        team_sync<TEAM>(team);
-        if (wt == 0 && lane == 0) sm.last[warp] = atomicInc(a.cnt + k0, parts - 1) == (unsigned)(parts - 1);
-        team_sync<TEAM>(team);
-        if (sm.last[team * TEAM]) {
+        team_sync(team, tsh);
+        if (wt == 0 && lane == 0) sm.last[team] = atomicInc(a.cnt + k0, parts - 1) == (unsigned)(parts - 1);
+        team_sync(team, tsh);
+        if (sm.last[team]) {
           __threadfence();
-          kv4_merge<G, TEAM>(a, k0, parts, qh0, wt * 32 + lane);
+          const int sl = max(T / G, 1);  // a power of two, as T and G are
+          for (int hs = wt; hs < G * sl; hs += T) {
+            const int hd = hs % G;
+            Kv4Acc acc;
+#pragma unroll 4
+            for (int p = hs / G; p < parts; p += sl) {
+              const int64_t at = (int64_t)(2 * (k0 + p) + (p == 0)) * G + hd;
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + at);
+              acc.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(a.ws_o) + at * 32 + lane));
+            }
+            if (sl == 1) {
+              reinterpret_cast<uint2*>(a.out + (qh0 + hd) * 128)[lane] = acc.result();
+            } else {
+              reinterpret_cast<float4*>(sm.red_o[warp][0])[lane] = acc.o;
+              if (lane == 0) *reinterpret_cast<float2*>(sm.red_ml[warp][0]) = make_float2(acc.m, acc.l);
+            }
+          }
+          if (sl > 1) {
+            team_sync(team, tsh);
+            if (wt < G) {
+              Kv4Acc acc;
+              for (int i = 0; i < sl; ++i) {
+                const int w = warp + i * G;
+                acc.add(sm.red_ml[w][0][0], sm.red_ml[w][0][1], reinterpret_cast<const float4*>(sm.red_o[w][0])[lane]);
+              }
+              reinterpret_cast<uint2*>(a.out + (qh0 + wt) * 128)[lane] = acc.result();
+            }
+          }
         }
       }
-      team_sync<TEAM>(team);  // the team's shared buffers are read
-      if (!kv4_next(a, cs, uend)) break;
+      team_sync(team, tsh);  // the team's shared buffers are read
+      if (!kv4_next(a, sm, cs, uend, tsh)) break;
     }
     if (dead) {  // copies in flight land (or run out of time once more) before the CTA ends
       mbar_wait(&sm.kfull[warp], kph, a.err, nullptr);
@@ -563,34 +654,26 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   }
 
   // ---- rows without tokens are zero; rows out of bounds are reported
-  for (int64_t b = blockIdx.x + (int64_t)warp * gridDim.x; b < a.batch; b += (int64_t)kAttWarps * gridDim.x) {
-    int64_t row;
+  for (int b = blockIdx.x + warp * gridDim.x; b < a.batch; b += kAttWarps * gridDim.x) {
+    int row;
     const int ctx = kv4_ctx(a, b, &row);
-    if (lane == 0 && row >= a.num_rows) report(a.err, ERR_SLOT_OOB);
+    if (lane == 0 && row == a.num_rows) report(a.err, ERR_SLOT_OOB);
     if (lane == 0 && ctx > 0 && (int64_t)a.seqlens[row] + a.ctx_add > a.max_ctx) report(a.err, ERR_CTX_OOB);
     if (ctx == 0)
       for (int i = lane; i < a.Hkv * G * 16; i += 32)
-        reinterpret_cast<uint4*>(a.out + b * a.Hkv * G * 128)[i] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(a.out + (int64_t)b * a.Hkv * G * 128)[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// Workspace: counters of every team a device can have (TEAM = 1), then two partials per team.
+// Workspace: counters of every team a device can have (T = 1), then two partials per team.
 static int64_t kv4_teams() { return (int64_t)sm_count() * kAttWarps; }
 static int64_t kv4_counter_bytes() { return (kv4_teams() * 4 + 255) / 256 * 256; }
 
-template <int G, int TEAM>
-static cudaError_t kv4_launch(const Kv4Args& a, cudaStream_t stream) {
-  const size_t smem = sizeof(Kv4Smem<G, TEAM>);
-  set_smem_once<kv4_decode_kernel<G, TEAM>>((int)smem);
-  return launch_k(kv4_decode_kernel<G, TEAM>, dim3(sm_count()), dim3(kAttThreads), smem, stream, a);
-}
-
 template <int G>
-static cudaError_t kv4_pick(const Kv4Args& a, cudaStream_t stream) {
-  const int64_t items = a.batch * a.Hkv;
-  if (items >= 256) return kv4_launch<G, 1>(a, stream);
-  if (items >= 64) return kv4_launch<G, 4>(a, stream);
-  return kv4_launch<G, 16>(a, stream);
+static cudaError_t kv4_launch(const Kv4Args& a, cudaStream_t stream) {
+  const size_t smem = sizeof(Kv4Smem<G>);
+  set_smem_once<kv4_decode_kernel<G>>((int)smem);
+  return launch_k(kv4_decode_kernel<G>, dim3(sm_count()), dim3(kAttThreads), smem, stream, a);
 }
 
 }  // namespace aacc
@@ -625,6 +708,11 @@ int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, con
                      (long long)need);
   if (max_context > max_blocks * block_size) max_context = max_blocks * block_size;
   if (max_context > 0x7fffffc0) max_context = 0x7fffffc0;
+  // Units are counted in 32 bits.
+  if (batch > 0x7fffffff || num_rows > 0x7ffffffe ||
+      (double)batch * num_kv_heads * (double)((max_context + kKv4Tile - 1) / kKv4Tile) > 2147483647.0)
+    return set_error(AACC_ERR_UNSUPPORTED, "kv4_decode_attention: %lld rows of up to %lld tokens are too many",
+                     (long long)batch, (long long)max_context);
   Kv4Args a;
   a.q = (const bf16*)q;
   a.out = (bf16*)out;
@@ -638,9 +726,9 @@ int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, con
   a.ws_ml = a.ws_o + 2 * kv4_teams() * G * 128;
   a.err = device_error_ptr();
   a.num_blocks = num_blocks;
-  a.num_rows = num_rows;
+  a.num_rows = (int)num_rows;
   a.max_blocks = max_blocks;
-  a.batch = batch;
+  a.batch = (int)batch;
   a.max_ctx = (int)max_context;
   a.ctx_add = ctx_add;
   a.Hkv = num_kv_heads;
@@ -648,10 +736,10 @@ int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, con
   a.scale = scale;
   cudaError_t le;
   switch (G) {
-    case 1: le = kv4_pick<1>(a, stream); break;
-    case 2: le = kv4_pick<2>(a, stream); break;
-    case 4: le = kv4_pick<4>(a, stream); break;
-    default: le = kv4_pick<8>(a, stream); break;
+    case 1: le = kv4_launch<1>(a, stream); break;
+    case 2: le = kv4_launch<2>(a, stream); break;
+    case 4: le = kv4_launch<4>(a, stream); break;
+    default: le = kv4_launch<8>(a, stream); break;
   }
   return check_launch("kv4_decode_kernel", le);
 }
