@@ -73,8 +73,8 @@ struct Kv4Args {
   float* ws_o;    // [2 * teams][G][128]
   float* ws_ml;   // [2 * teams][G][2]
   unsigned* err;
-  int64_t num_blocks, max_blocks;
-  int num_rows, batch, max_ctx, ctx_add, Hkv, tpb;  // tpb: tiles per block
+  int64_t max_blocks;
+  int num_blocks, num_rows, batch, max_ctx, ctx_add, Hkv, tpb;  // tpb: tiles per block
   float scale;
 };
 
@@ -145,6 +145,14 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   return y;
 }
 
+// d = a b, with no accumulator to clear.
+__device__ __forceinline__ void mma_f16_16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -167,7 +175,9 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // Bits 0-3 (HI: 4-7) of both halves of x, a code u each, as the fp16 pair (u - 8, u' - 8).
 template <bool HI>
 __device__ __forceinline__ uint32_t code(uint32_t x) {
-  const uint32_t y = (x & (HI ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;  // 1024 + u, or 1024 + 16 u
+  // 1024 + u, or 1024 + 16 u.  Written out, because (x & m) | c comes out as two operations otherwise.
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(HI ? 0x00f000f0 : 0x000f000f), "r"(0x64006400));
   const __half2 h = *reinterpret_cast<const __half2*>(&y);
   const __half2 r = HI ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f))
                        : __hadd2(h, __float2half2_rn(-1032.f));
@@ -179,6 +189,12 @@ template <int W>
 __device__ __forceinline__ float scale_of(uint2 p) {
   const uint32_t x = W < 2 ? p.x : p.y;
   return __uint_as_float((W & 1) ? x & 0xffff0000u : x << 16);
+}
+
+// All lanes' bounded wait; the first try is the common case.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* err, volatile int* abort) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, abort));
 }
 
 __device__ __forceinline__ void team_sync(int team, int tsh) {
@@ -315,12 +331,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     int lbi = lt / a.tpb, lti = lt - lbi * a.tpb;
     int32_t lid = lhas ? a.bt[ls.row * a.max_blocks + lbi] : 0;
     auto record = [&]() -> int64_t {
-      int64_t blk = lid;
-      if (blk < 0 || blk >= a.num_blocks) {
+      if ((uint32_t)lid >= (uint32_t)a.num_blocks) {
         if (lane == 0) report(a.err, ERR_BLOCK_OOB);
-        blk = 0;  // a valid address keeps the pipeline going; the result is flagged
+        lid = 0;  // a valid address keeps the pipeline going; the result is flagged
       }
-      return kv4_record(blk, ls.h, lti, a.Hkv, a.tpb);
+      return kv4_record(lid, ls.h, lti, a.Hkv, a.tpb);
     };
     auto load_k = [&](int64_t rec) {
       if (lane == 0) {
@@ -404,7 +419,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
             lid = a.bt[ls.row * a.max_blocks + lbi];
           }
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.kfull[warp], ph, a.err, abort))) {
+        if (!warp_wait(&sm.kfull[warp], ph, a.err, abort)) {
           dead = true;
           kph = ph;
           lhas = false;
@@ -427,19 +442,18 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
             const uint2 sy = *reinterpret_cast<const uint2*>(ksc + (16 * sb + g + 8) * 8);
             auto group = [&](auto W, uint32_t x, uint32_t y) {
               constexpr int w = decltype(W)::value;
-              float acc[4] = {0.f, 0.f, 0.f, 0.f};
+              float acc[4];
               const uint32_t a0[4] = {code<false>(x), code<false>(y), code<true>(x), code<true>(y)};
-              mma_f16_16816(acc, a0, qf[w][0], qf[w][1]);
+              mma_f16_16816_first(acc, a0, qf[w][0], qf[w][1]);
               x >>= 8;
               y >>= 8;
               const uint32_t a1[4] = {code<false>(x), code<false>(y), code<true>(x), code<true>(y)};
               mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
               const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
-              if (w == 0) s[sb][0] = s[sb][1] = s[sb][2] = s[sb][3] = 0.f;
-              s[sb][0] = fmaf(acc[0], fx, s[sb][0]);
-              s[sb][1] = fmaf(acc[1], fx, s[sb][1]);
-              s[sb][2] = fmaf(acc[2], fy, s[sb][2]);
-              s[sb][3] = fmaf(acc[3], fy, s[sb][3]);
+              s[sb][0] = w == 0 ? acc[0] * fx : fmaf(acc[0], fx, s[sb][0]);
+              s[sb][1] = w == 0 ? acc[1] * fx : fmaf(acc[1], fx, s[sb][1]);
+              s[sb][2] = w == 0 ? acc[2] * fy : fmaf(acc[2], fy, s[sb][2]);
+              s[sb][3] = w == 0 ? acc[3] * fy : fmaf(acc[3], fy, s[sb][3]);
             };
             group(std::integral_constant<int, 0>{}, x4.x, y4.x);
             group(std::integral_constant<int, 1>{}, x4.y, y4.y);
@@ -492,7 +506,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
           l1 = l1 * a1 + (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
 
           if (half == 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sm.vfull[warp], ph, a.err, abort))) {
+            if (!warp_wait(&sm.vfull[warp], ph, a.err, abort)) {
               dead = true;
               kph = lhas && done ? ph ^ 1 : ph;
               lhas = false;
@@ -725,7 +739,7 @@ int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, con
   a.ws_o = reinterpret_cast<float*>((uint8_t*)workspace + kv4_counter_bytes());
   a.ws_ml = a.ws_o + 2 * kv4_teams() * G * 128;
   a.err = device_error_ptr();
-  a.num_blocks = num_blocks;
+  a.num_blocks = (int)(num_blocks < 0x7fffffff ? num_blocks : 0x7fffffff);  // ids are 32-bit
   a.num_rows = (int)num_rows;
   a.max_blocks = max_blocks;
   a.batch = (int)batch;
