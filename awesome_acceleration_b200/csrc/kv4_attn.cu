@@ -28,11 +28,13 @@
 // scaled by a power of two per head to a largest element in [2^14, 2^15), so
 // that bf16 values go into fp16 unrounded down to 2^-28 of the largest.  The
 // group's scale multiplies the fp32 sum.
-// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand; the V scale of
-// (token, group) multiplies p in fp32, and the product is rounded once, to
-// fp16: 2^-12, an eighth of bf16's.  It is kept in range by a power of two,
-// 2^10 over the largest V scale so far, so that all products within 2^-24 of
-// the largest possible one keep their 11 bits.
+// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand.  P^T is 2^10 p
+// in fp16 (the 2^10 also in the sum it is divided by), transposed in
+// registers and multiplied by the V scales of its two tokens in fp16: two
+// roundings of 2^-12, a quarter of what one to bf16 costs.  The scales are
+// held relative to the largest so far, at [2^4, 2^5): a p down to 2^-24 and a
+// scale down to 2^-21 of the largest are exact but for those two roundings.
+// Once per tile each lane turns the scales of its two tokens into such pairs.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -49,6 +51,7 @@ template <int G>
 struct Kv4Smem {
   uint8_t k[kAttWarps][kKv4Record];
   uint8_t v[kAttWarps][kKv4Record];
+  uint4 vpair[kAttWarps][32];  // V scales of tokens 2 i and 2 i + 1, fp16 pairs of groups 0..3
   float red_o[kAttWarps][G][128];
   float red_ml[kAttWarps][G][2];
   uint32_t pre[kAttThreads];  // units before thread i's rows, per kv head
@@ -170,6 +173,11 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // Bits 0-3 (HI: 4-7) of both halves of x, a code u each, as the fp16 pair (u - 8, u' - 8).
@@ -397,7 +405,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-      int ev = 10;  // biased exponent of the largest V scale so far (at least 10): O is kept times 2^(264 - 127 - ev)
+      int ev = 4;  // biased exponent of the largest V scale so far (at least 4): O is kept times 2^(131 - ev)
 
       for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += T) {
         // the next tile's block id, in flight during Q.K
@@ -427,7 +435,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         }
         int64_t next_rec = 0;
         int lim = cs.ctx - t * kKv4Tile;  // tokens from here to the end of the context
-        float cv = 0.f;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half, lim -= 32) {
           // ---- S = K Q^T for 32 tokens; lane (g, c): tokens 16 sb + g (+ 8), heads 2c and 2c + 1
@@ -488,12 +495,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
           float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
           m0 = n0;
           m1 = n1;
+          const float r0 = 10.f - m0, r1 = 10.f - m1;  // 2^10 p
 #pragma unroll
           for (int sb = 0; sb < 2; ++sb) {
-            s[sb][0] = ex2(fmaf(s[sb][0], sl0, -m0));
-            s[sb][1] = ex2(fmaf(s[sb][1], sl1, -m1));
-            s[sb][2] = ex2(fmaf(s[sb][2], sl0, -m0));
-            s[sb][3] = ex2(fmaf(s[sb][3], sl1, -m1));
+            s[sb][0] = ex2(fmaf(s[sb][0], sl0, r0));
+            s[sb][1] = ex2(fmaf(s[sb][1], sl1, r1));
+            s[sb][2] = ex2(fmaf(s[sb][2], sl0, r0));
+            s[sb][3] = ex2(fmaf(s[sb][3], sl1, r1));
           }
           if (lim < 32) {  // also where a scale of 0 makes -inf * 0 a NaN
 #pragma unroll
@@ -514,25 +522,27 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
             }
             // The tile's largest V scale (they are not negative: their bits order as they do); lane: tokens
             // 2 lane and 2 lane + 1.  Behind the context a scale may be anything: it becomes zero.
-            uint4* vs = reinterpret_cast<uint4*>(sm.v[warp] + kKv4Codes) + lane;
-            uint4 x = *vs;
+            uint4 x = *(reinterpret_cast<const uint4*>(sm.v[warp] + kKv4Codes) + lane);
             if (lim < kKv4Tile) {
               if (2 * lane >= lim) x.x = x.y = 0;
               if (2 * lane + 1 >= lim) x.z = x.w = 0;
-              *vs = x;
-              fence_proxy_async();  // before the bulk copy that overwrites the buffer
-              __syncwarp();
             }
-            const uint32_t hi = max(max(x.x, x.y), max(x.z, x.w)) >> 16;
-            const uint32_t lo = max(max(x.x & 0xffffu, x.y & 0xffffu), max(x.z & 0xffffu, x.w & 0xffffu));
-            const int e = (int)(__reduce_max_sync(0xffffffffu, max(hi, lo)) >> 7);
+            const uint32_t big = max(max(max(x.x, x.y), max(x.z, x.w)),
+                                     max(max(x.x << 16, x.y << 16), max(x.z << 16, x.w << 16)));
+            const int e = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
             if (e > ev) {
               const float f = ex2((float)(ev - e));
               a0 *= f;
               a1 *= f;
               ev = e;
             }
-            cv = __uint_as_float((uint32_t)(264 - ev) << 23);
+            const float cv = __uint_as_float((uint32_t)(258 - ev) << 23);
+            const uint2 ta = make_uint2(x.x, x.y), tb = make_uint2(x.z, x.w);
+            sm.vpair[warp][lane] = make_uint4(pack_f16(scale_of<0>(ta) * cv, scale_of<0>(tb) * cv),
+                                              pack_f16(scale_of<1>(ta) * cv, scale_of<1>(tb) * cv),
+                                              pack_f16(scale_of<2>(ta) * cv, scale_of<2>(tb) * cv),
+                                              pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
+            __syncwarp();
           }
           if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
 #pragma unroll
@@ -546,19 +556,17 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
 
           // ---- O^T += V^T P^T
           const uint8_t* vb = sm.v[warp] + half * 2048;
-          const uint8_t* vsc = sm.v[warp] + kKv4Codes + half * 256;
 #pragma unroll
           for (int sb = 0; sb < 2; ++sb) {
             const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
             const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
-            const uint2 sx = *reinterpret_cast<const uint2*>(vsc + (16 * sb + g) * 8);
-            const uint2 sy = *reinterpret_cast<const uint2*>(vsc + (16 * sb + g + 8) * 8);
-            const float p0 = s[sb][0] * cv, p1 = s[sb][1] * cv, p2 = s[sb][2] * cv, p3 = s[sb][3] * cv;
+            const uint4 sx = sm.vpair[warp][(2 * half + sb) * 8 + c], sy = sm.vpair[warp][(2 * half + sb) * 8 + 4 + c];
+            const uint32_t px = movmatrix_trans(pack_f16(s[sb][0], s[sb][1]));  // head g, tokens 2c, 2c + 1
+            const uint32_t py = movmatrix_trans(pack_f16(s[sb][2], s[sb][3]));  // ... + 8
             auto group = [&](auto W) {  // 32 dims: j = 2w and 2w + 1
               constexpr int w = decltype(W)::value;
-              const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
-              const uint32_t b0 = movmatrix_trans(pack_f16(p0 * fx, p1 * fx));
-              const uint32_t b1 = movmatrix_trans(pack_f16(p2 * fy, p3 * fy));
+              const uint32_t b0 = mul_f16(px, w == 0 ? sx.x : w == 1 ? sx.y : w == 2 ? sx.z : sx.w);
+              const uint32_t b1 = mul_f16(py, w == 0 ? sy.x : w == 1 ? sy.y : w == 2 ? sy.z : sy.w);
               // 16 bits of tokens 2c | 2c + 1 each: four nibbles = dims 16 j + 2g, + 1 of j = 2w, 2w + 1
               constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
               uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
@@ -589,7 +597,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
       }
-      const float down = __uint_as_float((uint32_t)max(ev - 10, 0) << 23) + (ev == 10 ? 0x1p-127f : 0.f);
+      const float down = __uint_as_float((uint32_t)(ev - 4) << 23) + (ev == 4 ? 0x1p-127f : 0.f);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {  // o[j][e], o[j][2 + e]: dims 16 j + 2g and + 1 of head 2c + e
         const int hd = 2 * c + e;
