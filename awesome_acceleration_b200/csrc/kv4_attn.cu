@@ -28,12 +28,13 @@
 // scaled by a power of two per head to a largest element in [2^14, 2^15), so
 // that bf16 values go into fp16 unrounded down to 2^-28 of the largest.  The
 // group's scale multiplies the fp32 sum.
-// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand.  P^T is 2^10 p
-// in fp16 (the 2^10 also in the sum it is divided by), transposed in
+// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand.  P^T is 2^4 p
+// in fp16 (the 2^4 also in the sum it is divided by), p < 2^6, transposed in
 // registers and multiplied by the V scales of its two tokens in fp16: two
 // roundings of 2^-12, a quarter of what one to bf16 costs.  The scales are
-// held relative to the largest so far, at [2^4, 2^5): a p down to 2^-24 and a
-// scale down to 2^-21 of the largest are exact but for those two roundings.
+// held relative to the largest so far, at [2^4, 2^5): products reach 2^15, and
+// a p down to 2^-18 and a scale down to 2^-21 of the largest have no other
+// rounding than those two.
 // Once per tile each lane turns the scales of its two tokens into such pairs.
 #include <cuda_fp16.h>
 
@@ -144,20 +145,20 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // 8x8 transpose of b16 values over the warp.
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
 // d = a b, with no accumulator to clear.
 __device__ __forceinline__ void mma_f16_16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -484,18 +485,29 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
               if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = -INFINITY;
             }
           }
-          float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
-          float x1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+          // The reference of the exponentials follows the maximum only when a score passes it by 2^6: p stays
+          // below 2^6, and most halves need no shuffles and no rescaling.
+          const float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * sl0;
+          const float x1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * sl1;
+          float a0 = 1.f, a1 = 1.f;
+          bool grow = __any_sync(0xffffffffu, x0 > m0 + 6.f || x1 > m1 + 6.f);
+          if (grow) {
+            float n0 = x0, n1 = x1;
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+            for (int d = 4; d < 32; d <<= 1) {
+              n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
+              n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
+            }
+            n0 = fmaxf(m0, n0);
+            n1 = fmaxf(m1, n1);
+            a0 = ex2(m0 - n0);
+            a1 = ex2(m1 - n1);
+            m0 = n0;
+            m1 = n1;
+            l0 *= a0;
+            l1 *= a1;
           }
-          const float n0 = fmaxf(m0, x0 * sl0), n1 = fmaxf(m1, x1 * sl1);  // these tokens are in the context: finite
-          float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
-          m0 = n0;
-          m1 = n1;
-          const float r0 = 10.f - m0, r1 = 10.f - m1;  // 2^10 p
+          const float r0 = 4.f - m0, r1 = 4.f - m1;  // 2^4 p
 #pragma unroll
           for (int sb = 0; sb < 2; ++sb) {
             s[sb][0] = ex2(fmaf(s[sb][0], sl0, r0));
@@ -510,8 +522,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
               if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = 0.f;
             }
           }
-          l0 = l0 * a0 + (s[0][0] + s[0][2]) + (s[1][0] + s[1][2]);
-          l1 = l1 * a1 + (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
+          l0 += (s[0][0] + s[0][2]) + (s[1][0] + s[1][2]);
+          l1 += (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
 
           if (half == 0) {
             if (!warp_wait(&sm.vfull[warp], ph, a.err, abort)) {
@@ -535,6 +547,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
               a0 *= f;
               a1 *= f;
               ev = e;
+              grow = true;
             }
             const float cv = __uint_as_float((uint32_t)(258 - ev) << 23);
             const uint2 ta = make_uint2(x.x, x.y), tb = make_uint2(x.z, x.w);
@@ -544,7 +557,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
                                               pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
             __syncwarp();
           }
-          if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
+          if (grow) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               o[j][0] *= a0;
