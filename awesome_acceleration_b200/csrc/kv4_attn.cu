@@ -89,14 +89,15 @@ struct Kv4Seg {
 };
 
 // Tokens of batch row b (0: padding, outside the tables, or empty).
-__device__ __forceinline__ int kv4_ctx(const Kv4Args& a, int b, int* row) {
+__device__ __forceinline__ int kv4_ctx(const Kv4Args& a, int b, int* row, unsigned* err = nullptr) {
   const int64_t r = a.rows[b];
+  *row = (int)r;
   if (r < 0 || r >= a.num_rows) {
-    *row = r < 0 ? -1 : a.num_rows;
+    if (r >= 0) report(err, ERR_SLOT_OOB);
     return 0;
   }
-  *row = (int)r;
   const int64_t c = (int64_t)a.seqlens[r] + a.ctx_add;
+  if (c > a.max_ctx) report(err, ERR_CTX_OOB);
   return (int)max((int64_t)0, min(c, (int64_t)a.max_ctx));
 }
 
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   uint32_t cnt[5] = {0, 0, 0, 0, 0};
   for (int b = b_lo; b < b_hi; ++b) {
     int row;
-    const int ctx = kv4_ctx(a, b, &row);
+    const int ctx = kv4_ctx(a, b, &row, blockIdx.x == 0 ? a.err : nullptr);
     if (per == 1) {
       sm.ctx[b] = ctx;
       sm.row[b] = row;
@@ -688,13 +689,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     }
   }
 
-  // ---- rows without tokens are zero; rows out of bounds are reported
+  // ---- rows without tokens are zero
   for (int b = blockIdx.x + warp * gridDim.x; b < a.batch; b += kAttWarps * gridDim.x) {
     int row;
-    const int ctx = kv4_ctx(a, b, &row);
-    if (lane == 0 && row == a.num_rows) report(a.err, ERR_SLOT_OOB);
-    if (lane == 0 && ctx > 0 && (int64_t)a.seqlens[row] + a.ctx_add > a.max_ctx) report(a.err, ERR_CTX_OOB);
-    if (ctx == 0)
+    if ((per == 1 ? sm.ctx[b] : kv4_ctx(a, b, &row)) == 0)
       for (int i = lane; i < a.Hkv * G * 16; i += 32)
         reinterpret_cast<uint4*>(a.out + (int64_t)b * a.Hkv * G * 128)[i] = make_uint4(0, 0, 0, 0);
   }

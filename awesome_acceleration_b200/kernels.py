@@ -99,18 +99,24 @@ def prefill_attention(q, k_cache, v_cache, block_tables, seq_rows, cu_q, ctx_sta
 
 
 # ---------------------------------------------------------------- request maps
-def _here(t: torch.Tensor, dtype, ndim: int, name: str):
-    """`t` must be a contiguous `ndim`-d `dtype` tensor on the current CUDA device (the kernels launch on that
-    device's current stream)."""
-    if t.dtype != dtype or t.dim() != ndim or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {ndim}-d {dtype} tensor, got {tuple(t.shape)} {t.dtype} "
-                         f"contiguous={t.is_contiguous()}")
-    _on_device(t, name)
+def _device_of(t: torch.Tensor, what: str, name: str) -> int:
+    """The index of the current CUDA device, which `t` must be on: the kernels launch on its current stream."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{what}: {name} is on {t.device}, expected the current CUDA device")
+    return dev
 
 
-def _on_device(t: torch.Tensor, name: str):
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name}: is on {t.device}, expected the current CUDA device")
+def _here(t: torch.Tensor, dtype, ndim: int, dev: int, what: str, name: str) -> None:
+    """`t` must be a contiguous `ndim`-d `dtype` tensor on device `dev`."""
+    if t.dtype is not dtype or t.dim() != ndim or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {ndim}-d {dtype} tensor on cuda:{dev}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}, contiguous={t.is_contiguous()}")
+
+
+def _raw_stream(dev: int) -> int:
+    """The current stream of device `dev`, without a Stream object around it (a tenth of the cost)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def build_block_tables(lengths, block_size: int, *, max_blocks: int | None = None, free_blocks=None, out=None,
@@ -119,25 +125,30 @@ def build_block_tables(lengths, block_size: int, *, max_blocks: int | None = Non
     tokens: request i takes ceil(lengths[i] / block_size) blocks of
     `free_blocks` (int32; None: 0, 1, 2, ...) in request order, the rest of
     its row is -1.  `used` (int32 [1]) receives the number of blocks taken."""
-    _here(lengths, torch.int32, 1, "build_block_tables: lengths")
+    what = "build_block_tables"
+    dev = _device_of(lengths, what, "lengths")
+    _here(lengths, torch.int32, 1, dev, what, "lengths")
     S = lengths.shape[0]
     if out is None:
         if max_blocks is None:
-            raise ValueError("build_block_tables: give max_blocks or out")
+            raise ValueError(f"{what}: give max_blocks or out")
         out = torch.empty((S, max_blocks), dtype=torch.int32, device=lengths.device)
     else:
-        _here(out, torch.int32, 2, "build_block_tables: out")
+        _here(out, torch.int32, 2, dev, what, "out")
         if out.shape[0] != S or (max_blocks is not None and out.shape[1] != max_blocks):
-            raise ValueError(f"build_block_tables: out is {tuple(out.shape)} for {S} requests")
+            raise ValueError(f"{what}: out is {tuple(out.shape)} for {S} requests")
+    num_free = 0x7fffffff
     if free_blocks is not None:
-        _here(free_blocks, torch.int32, 1, "build_block_tables: free_blocks")
+        _here(free_blocks, torch.int32, 1, dev, what, "free_blocks")
+        num_free = free_blocks.shape[0]
     if used is not None:
-        _here(used, torch.int32, 1, "build_block_tables: used")
+        _here(used, torch.int32, 1, dev, what, "used")
         if used.shape[0] != 1:
-            raise ValueError("build_block_tables: used holds one value")
-    _lib.check(_lib_().aacc_build_block_tables(
-        _p(lengths), S, block_size, _p(free_blocks), 0x7fffffff if free_blocks is None else free_blocks.shape[0],
-        _p(out), out.shape[1], _p(used), _stream()), "build_block_tables")
+            raise ValueError(f"{what}: used holds one value")
+    rc = _lib_().aacc_build_block_tables(lengths.data_ptr(), S, block_size, _p(free_blocks), num_free, out.data_ptr(),
+                                         out.shape[1], _p(used), _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
     return out
 
 
@@ -150,28 +161,35 @@ def build_slot_maps(lengths, block_tables, *, block_size: int, num_blocks: int, 
     negative: padding).  Entries behind the last request get position 0 and
     slot -1; `num_tokens` may exceed the sum of the lengths."""
     what = "build_slot_maps"
-    _here(lengths, torch.int32, 1, f"{what}: lengths")
-    _here(block_tables, torch.int32, 2, f"{what}: block_tables")
-    S, dev = lengths.shape[0], lengths.device
-    for t, dt, name in ((starts, torch.int32, "starts"), (rows, torch.int64, "rows")):
-        if t is not None:
-            _here(t, dt, 1, f"{what}: {name}")
-            if t.shape[0] != S:
-                raise ValueError(f"{what}: {name} has {t.shape[0]} entries for {S} requests")
-    outs = []
-    for t, dt, n, name in ((cu, torch.int32, S + 1, "cu"), (positions, torch.int64, num_tokens, "positions"),
-                           (slots, torch.int64, num_tokens, "slots")):
+    dev = _device_of(lengths, what, "lengths")
+    _here(lengths, torch.int32, 1, dev, what, "lengths")
+    _here(block_tables, torch.int32, 2, dev, what, "block_tables")
+    S = lengths.shape[0]
+    if starts is not None:
+        _here(starts, torch.int32, 1, dev, what, "starts")
+        if starts.shape[0] != S:
+            raise ValueError(f"{what}: {starts.shape[0]} starts for {S} requests")
+    if rows is not None:
+        _here(rows, torch.int64, 1, dev, what, "rows")
+        if rows.shape[0] != S:
+            raise ValueError(f"{what}: {rows.shape[0]} rows for {S} requests")
+
+    def output(t, dtype, n, name):
         if t is None:
-            t = torch.empty(n, dtype=dt, device=dev)
-        else:
-            _here(t, dt, 1, f"{what}: {name}")
-            if t.shape[0] != n:
-                raise ValueError(f"{what}: {name} has {t.shape[0]} entries, expected {n}")
-        outs.append(t)
-    cu, positions, slots = outs
-    _lib.check(_lib_().aacc_build_slot_maps(
-        _p(lengths), _p(starts), _p(rows), S, _p(block_tables), block_tables.shape[0], block_tables.shape[1],
-        block_size, num_blocks, _p(cu), _p(positions), _p(slots), num_tokens, _stream()), what)
+            return torch.empty(n, dtype=dtype, device=lengths.device)
+        _here(t, dtype, 1, dev, what, name)
+        if t.shape[0] != n:
+            raise ValueError(f"{what}: {name} has {t.shape[0]} entries, expected {n}")
+        return t
+    cu = output(cu, torch.int32, S + 1, "cu")
+    positions = output(positions, torch.int64, num_tokens, "positions")
+    slots = output(slots, torch.int64, num_tokens, "slots")
+    num_rows, max_blocks = block_tables.shape
+    rc = _lib_().aacc_build_slot_maps(lengths.data_ptr(), _p(starts), _p(rows), S, block_tables.data_ptr(), num_rows,
+                                      max_blocks, block_size, num_blocks, cu.data_ptr(), positions.data_ptr(),
+                                      slots.data_ptr(), num_tokens, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
     return cu, positions, slots
 
 
@@ -188,24 +206,26 @@ def kv4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int) -> tupl
 
 
 def _kv4_pools(k_cache, v_cache, what: str):
-    """(num_blocks, Hkv, block_size) of a layer's pools, checked."""
-    _here(k_cache, torch.uint8, 4, f"{what}: k_cache")
-    _here(v_cache, torch.uint8, 4, f"{what}: v_cache")
-    nb, hkv, tiles, rec = k_cache.shape
-    if rec != KV4_RECORD_BYTES or v_cache.shape != k_cache.shape:
-        raise ValueError(f"{what}: pools are {tuple(k_cache.shape)} and {tuple(v_cache.shape)}, expected two of "
+    """(device, num_blocks, Hkv, block_size) of a layer's pools, checked."""
+    dev = _device_of(k_cache, what, "k_cache")
+    _here(k_cache, torch.uint8, 4, dev, what, "k_cache")
+    _here(v_cache, torch.uint8, 4, dev, what, "v_cache")
+    shape = k_cache.shape
+    if shape[3] != KV4_RECORD_BYTES or v_cache.shape != shape:
+        raise ValueError(f"{what}: pools are {tuple(shape)} and {tuple(v_cache.shape)}, expected two of "
                          f"[blocks, heads, block_size / {KV4_TILE}, {KV4_RECORD_BYTES}]")
-    return nb, hkv, tiles * KV4_TILE
+    return dev, shape[0], shape[1], shape[2] * KV4_TILE
 
 
-def _kv_rows(x, hkv: int, T: int, name: str):
+def _kv_rows(x, hkv: int, T: int, dev: int, what: str, name: str):
     """(row stride, head stride) in elements of bf16 rows [T, hkv, 128] or [T, hkv * 128]."""
-    if x.dtype != BF16 or x.shape[0] != T or x.stride(-1) != 1 or tuple(x.shape[1:]) not in ((hkv, 128), (hkv * 128,)):
-        raise ValueError(f"{name}: expected bf16 rows [{T}, {hkv}, 128] with contiguous dims, got {tuple(x.shape)} "
-                         f"{x.dtype} strides {tuple(x.stride())}")
-    _on_device(x, name)
+    shape, strides = tuple(x.shape), x.stride()
+    if (x.dtype is not BF16 or x.get_device() != dev or strides[-1] != 1
+            or shape not in ((T, hkv, 128), (T, hkv * 128))):
+        raise ValueError(f"{what}: {name} must be bf16 rows [{T}, {hkv}, 128] with contiguous dims on cuda:{dev}, got "
+                         f"{shape} {x.dtype} strides {strides} on {x.device}")
     # a dimension of size 1 may carry any stride: it is never stepped over
-    return x.stride(0) if T > 1 else 0, (x.stride(1) if x.dim() == 3 else 128) if hkv > 1 else 0
+    return strides[0] if T > 1 else 0, (strides[1] if len(shape) == 3 else 128) if hkv > 1 else 0
 
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_cache: torch.Tensor,
@@ -213,39 +233,47 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     """Quantise k/v [T, Hkv, 128] bf16 (strided rows and heads allowed) into
     flat slots of the 4-bit pools (see kv4_cache_shape); negative slots skip,
     the others must be distinct."""
-    nb, hkv, bs = _kv4_pools(k_cache, v_cache, "kv4_store")
-    _here(slot_mapping, torch.int64, 1, "kv4_store: slot_mapping")
+    what = "kv4_store"
+    dev, nb, hkv, bs = _kv4_pools(k_cache, v_cache, what)
+    _here(slot_mapping, torch.int64, 1, dev, what, "slot_mapping")
     T = slot_mapping.shape[0]
-    ks, kh = _kv_rows(k, hkv, T, "kv4_store: k")
-    vs, vh = _kv_rows(v, hkv, T, "kv4_store: v")
-    _lib.check(_lib_().aacc_kv4_store(_p(k), _p(v), T, ks, kh, vs, vh, _p(slot_mapping), _p(k_cache), _p(v_cache), nb,
-                                      hkv, bs, _stream()), "kv4_store")
+    ks, kh = _kv_rows(k, hkv, T, dev, what, "k")
+    vs, vh = _kv_rows(v, hkv, T, dev, what, "v")
+    rc = _lib_().aacc_kv4_store(k.data_ptr(), v.data_ptr(), T, ks, kh, vs, vh, slot_mapping.data_ptr(),
+                                k_cache.data_ptr(), v_cache.data_ptr(), nb, hkv, bs, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
 
 
 def kv4_load(k_cache, v_cache, slots, k_out=None, v_out=None, *, out_slots=None):
     """Dequantise flat slots (int64 [T]) of the 4-bit pools into bf16: rows
     k_out/v_out [n, Hkv, 128], or paged caches [blocks, Hkv, bs, 128] of any
     block size; token t goes to row / flat slot out_slots[t] (None: t).  A
-    negative slot on either side skips the token.  Returns (k_out, v_out)."""
-    nb, hkv, bs = _kv4_pools(k_cache, v_cache, "kv4_load")
-    _here(slots, torch.int64, 1, "kv4_load: slots")
+    negative slot on either side skips the token.  Returns (k_out, v_out);
+    outputs made here are zero where a token is skipped."""
+    what = "kv4_load"
+    dev, nb, hkv, bs = _kv4_pools(k_cache, v_cache, what)
+    _here(slots, torch.int64, 1, dev, what, "slots")
     T = slots.shape[0]
     if out_slots is not None:
-        _here(out_slots, torch.int64, 1, "kv4_load: out_slots")
+        _here(out_slots, torch.int64, 1, dev, what, "out_slots")
         if out_slots.shape[0] != T:
-            raise ValueError(f"kv4_load: {out_slots.shape[0]} out_slots for {T} slots")
+            raise ValueError(f"{what}: {out_slots.shape[0]} out_slots for {T} slots")
     if k_out is None or v_out is None:
         if out_slots is not None or k_out is not None or v_out is not None:
-            raise ValueError("kv4_load: give both k_out and v_out (or neither and no out_slots)")
-        k_out, v_out = torch.zeros((2, T, hkv, 128), dtype=BF16, device=k_cache.device)  # a skipped token reads as zeros
-    _here(k_out, BF16, k_out.dim(), "kv4_load: k_out")
-    _here(v_out, BF16, v_out.dim(), "kv4_load: v_out")
-    if v_out.shape != k_out.shape or k_out.dim() not in (3, 4) or k_out.shape[1] != hkv or k_out.shape[-1] != 128:
-        raise ValueError(f"kv4_load: outputs are {tuple(k_out.shape)} and {tuple(v_out.shape)}, expected two of "
+            raise ValueError(f"{what}: give both k_out and v_out (or neither and no out_slots)")
+        k_out, v_out = torch.zeros((2, T, hkv, 128), dtype=BF16, device=k_cache.device)
+    shape = k_out.shape
+    _here(k_out, BF16, len(shape), dev, what, "k_out")
+    _here(v_out, BF16, len(shape), dev, what, "v_out")
+    if v_out.shape != shape or len(shape) not in (3, 4) or shape[1] != hkv or shape[-1] != 128:
+        raise ValueError(f"{what}: outputs are {tuple(shape)} and {tuple(v_out.shape)}, expected two of "
                          f"[rows, {hkv}, 128] or [blocks, {hkv}, block_size, 128]")
-    out_bs = 1 if k_out.dim() == 3 else k_out.shape[2]
-    _lib.check(_lib_().aacc_kv4_load(_p(k_cache), _p(v_cache), nb, hkv, bs, _p(slots), _p(out_slots), T, _p(k_out),
-                                     _p(v_out), k_out.shape[0], out_bs, _stream()), "kv4_load")
+    rc = _lib_().aacc_kv4_load(k_cache.data_ptr(), v_cache.data_ptr(), nb, hkv, bs, slots.data_ptr(), _p(out_slots), T,
+                               k_out.data_ptr(), v_out.data_ptr(), shape[0], 1 if len(shape) == 3 else shape[2],
+                               _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
     return k_out, v_out
 
 
@@ -255,35 +283,34 @@ def kv4_decode_workspace_bytes(num_q_heads: int, num_kv_heads: int) -> int:
 
 
 def kv4_decode_attention(q, k_cache, v_cache, block_tables, rows, seqlens, *, ctx_add: int, scale: float,
-                         max_context: int, workspace: torch.Tensor | None, out=None) -> torch.Tensor:
+                         max_context: int, workspace: torch.Tensor, out=None) -> torch.Tensor:
     """q [B, Hq, 128] -> out [B, Hq, 128] over seqlens[rows[b]] + ctx_add
     tokens of the 4-bit pools (paged_decode_attention over the bf16 cache).
     Calls that share `workspace` must be ordered on one stream."""
     what = "kv4_decode_attention"
-    nb, hkv, bs = _kv4_pools(k_cache, v_cache, what)
-    _here(q, BF16, 3, f"{what}: q")
-    _here(block_tables, torch.int32, 2, f"{what}: block_tables")
-    _here(rows, torch.int64, 1, f"{what}: rows")
-    _here(seqlens, torch.int32, 1, f"{what}: seqlens")
+    dev, nb, hkv, bs = _kv4_pools(k_cache, v_cache, what)
+    _here(q, BF16, 3, dev, what, "q")
+    _here(block_tables, torch.int32, 2, dev, what, "block_tables")
+    _here(rows, torch.int64, 1, dev, what, "rows")
+    _here(seqlens, torch.int32, 1, dev, what, "seqlens")
+    _here(workspace, torch.uint8, 1, dev, what, "workspace")
     B, hq, d = q.shape
-    if d != 128 or rows.shape[0] != B or seqlens.shape[0] > block_tables.shape[0]:
-        raise ValueError(f"{what}: q {tuple(q.shape)}, {rows.shape[0]} rows, {seqlens.shape[0]} seqlens, "
-                         f"{block_tables.shape[0]} block table rows")
+    num_rows, max_blocks = block_tables.shape
+    if d != 128 or rows.shape[0] != B or seqlens.shape[0] != num_rows:
+        raise ValueError(f"{what}: q {tuple(q.shape)} with {rows.shape[0]} rows; {seqlens.shape[0]} seqlens with "
+                         f"{num_rows} block table rows")
     if out is None:
         out = torch.empty_like(q)
     else:
-        _here(out, BF16, 3, f"{what}: out")
+        _here(out, BF16, 3, dev, what, "out")
         if out.shape != q.shape:
             raise ValueError(f"{what}: out is {tuple(out.shape)}, expected {tuple(q.shape)}")
-    ws_bytes = 0
-    if workspace is not None:
-        if not workspace.is_contiguous():
-            raise ValueError(f"{what}: workspace must be contiguous")
-        _on_device(workspace, f"{what}: workspace")
-        ws_bytes = workspace.numel() * workspace.element_size()
-    _lib.check(_lib_().aacc_kv4_decode_attention(
-        _p(q), _p(out), _p(k_cache), _p(v_cache), nb, _p(block_tables), seqlens.shape[0], block_tables.shape[1],
-        _p(rows), _p(seqlens), ctx_add, B, hq, hkv, bs, scale, max_context, _p(workspace), ws_bytes, _stream()), what)
+    rc = _lib_().aacc_kv4_decode_attention(
+        q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), nb, block_tables.data_ptr(), num_rows,
+        max_blocks, rows.data_ptr(), seqlens.data_ptr(), ctx_add, B, hq, hkv, bs, scale, max_context,
+        workspace.data_ptr(), workspace.shape[0], _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
     return out
 
 

@@ -30,7 +30,7 @@ def test_cache_shape():
             K.kv4_cache_shape(1, 1, bs)
 
 
-def test_wrappers_refuse_tensors_off_the_gpu_and_of_other_types_and_shapes():
+def test_wrappers_refuse_tensors_off_the_gpu():
     pool = torch.zeros(K.kv4_cache_shape(2, 2, 64), dtype=torch.uint8)
     rows, slots = torch.zeros((3, 2, 128), dtype=BF), torch.zeros(3, dtype=torch.int64)
     i32 = torch.zeros(3, dtype=torch.int32)
@@ -45,12 +45,6 @@ def test_wrappers_refuse_tensors_off_the_gpu_and_of_other_types_and_shapes():
         K.build_block_tables(i32, 64, max_blocks=2)
     with pytest.raises(ValueError, match="current CUDA device"):
         K.build_slot_maps(i32, i32.view(1, 3), block_size=64, num_blocks=1, num_tokens=3)
-    with pytest.raises(ValueError, match="k_cache"):
-        K.kv4_store(rows, rows, slots, pool.to(torch.int8), pool)
-    with pytest.raises(ValueError, match="lengths"):
-        K.build_block_tables(i32.long(), 64, max_blocks=2)
-    with pytest.raises(ValueError, match="lengths"):
-        K.build_slot_maps(i32.view(1, 3), i32.view(1, 3), block_size=64, num_blocks=1, num_tokens=3)
 
 
 def test_c_abi_checks_arguments_before_any_cuda_call():

@@ -166,6 +166,61 @@ def test_store_and_load_skip_slots_outside_the_pool(cuda):
     assert dev_err() & 2 and not out.any()
 
 
+def test_wrappers_refuse_other_types_shapes_and_layouts(cuda):
+    pool = torch.zeros(K().kv4_cache_shape(2, 2, 64), dtype=torch.uint8, device=cuda)
+    rows = torch.zeros((3, 2, 128), dtype=BF, device=cuda)
+    i64, i32 = torch.zeros(3, dtype=torch.int64, device=cuda), torch.zeros(3, dtype=torch.int32, device=cuda)
+    bt = torch.zeros((3, 2), dtype=torch.int32, device=cuda)
+    ws = torch.zeros(K().kv4_decode_workspace_bytes(4, 2), dtype=torch.uint8, device=cuda)
+    q = torch.zeros((3, 4, 128), dtype=BF, device=cuda)
+
+    def store(k=rows, v=rows, s=i64, kc=pool, vc=pool):
+        K().kv4_store(k, v, s, kc, vc)
+
+    def load(kc=pool, vc=pool, s=i64, ko=rows, vo=rows.clone(), os=None):
+        K().kv4_load(kc, vc, s, ko, vo, out_slots=os)
+
+    def attend(q=q, kc=pool, vc=pool, bt=bt, r=i64, sl=i32, ws=ws, out=None):
+        K().kv4_decode_attention(q, kc, vc, bt, r, sl, ctx_add=0, scale=1.0, max_context=64, workspace=ws, out=out)
+
+    def maps(n=i32, bt=bt, st=None, r=None, cu=None, pos=None, sl=None):
+        K().build_slot_maps(n, bt, block_size=64, num_blocks=2, num_tokens=5, starts=st, rows=r, cu=cu, positions=pos,
+                            slots=sl)
+
+    def tables(n=i32, out=None, fr=None, used=None, mb=2):
+        K().build_block_tables(n, 64, max_blocks=mb, out=out, free_blocks=fr, used=used)
+    half = torch.zeros((2, 2, 1, 4600), dtype=torch.uint8, device=cuda)
+    wide = torch.zeros((3, 2, 256), dtype=BF, device=cuda)
+    for f, kw in [
+        (store, dict(kc=pool.to(torch.int8))), (store, dict(kc=half, vc=half)), (store, dict(vc=pool[:1])),
+        (store, dict(kc=pool.transpose(0, 1))), (store, dict(k=rows.float())), (store, dict(v=rows[:2])),
+        (store, dict(k=wide[..., ::2])), (store, dict(k=rows[:, :1])), (store, dict(s=i32)), (store, dict(s=i64[:2])),
+        (store, dict(k=rows.cpu())), (store, dict(s=i64.cpu())),
+        (load, dict(kc=half, vc=half)), (load, dict(s=i32)), (load, dict(os=i64[:2])), (load, dict(ko=None)),
+        (load, dict(ko=rows.half())), (load, dict(ko=rows[:2])), (load, dict(ko=wide[..., :128], vo=wide[..., 128:])),
+        (load, dict(ko=rows[:, :1].contiguous(), vo=rows[:, :1].contiguous())), (load, dict(ko=None, vo=None, os=i64)),
+        (attend, dict(q=q.half())), (attend, dict(q=wide)), (attend, dict(r=i64[:2])), (attend, dict(r=i32)),
+        (attend, dict(sl=i64)), (attend, dict(bt=bt[:2])), (attend, dict(bt=bt.long())), (attend, dict(ws=None)),
+        (attend, dict(ws=ws[:-16])), (attend, dict(ws=ws.view(torch.int8))), (attend, dict(out=q[:2])),
+        (attend, dict(out=q.float())), (attend, dict(kc=pool[:1], vc=pool)),
+        (maps, dict(n=i64)), (maps, dict(n=i32.view(1, 3))), (maps, dict(bt=bt.long())), (maps, dict(st=i32[:2])),
+        (maps, dict(r=i64[:2])), (maps, dict(r=i32)), (maps, dict(cu=i32)), (maps, dict(pos=i64)),
+        (maps, dict(sl=i32)), (maps, dict(bt=bt.t())),
+        (tables, dict(n=i64)), (tables, dict(mb=None)), (tables, dict(out=bt[:2])), (tables, dict(out=bt, mb=3)),
+        (tables, dict(fr=i64)), (tables, dict(used=i32)),
+    ]:
+        with pytest.raises((ValueError, RuntimeError, AttributeError)):
+            f(**kw)
+    for f in (store, load, attend, maps, tables):
+        f()
+    with pytest.raises(RuntimeError, match="head ratio"):
+        attend(q=torch.zeros((3, 6, 128), dtype=BF, device=cuda))
+    with pytest.raises(RuntimeError, match="aligned"):
+        buf = torch.zeros(3 * 256 + 4, dtype=BF, device=cuda)
+        store(k=buf[4:].view(3, 2, 128))
+    assert dev_err() == 0
+
+
 def test_empty_calls(cuda):
     kd = torch.zeros(K().kv4_cache_shape(2, 2, 64), dtype=torch.uint8, device=cuda)
     none = torch.empty(0, dtype=torch.int64, device=cuda)
