@@ -16,29 +16,47 @@ __device__ __forceinline__ uint32_t transpose4(uint32_t w, int lane) {
   return (lane & 2) ? __byte_perm(w, y, 0x3715) : __byte_perm(w, y, 0x6240);
 }
 
-// One warp per (token, kv head): lanes 0-15 quantise the K row, lanes 16-31
-// the V row, 8 dims each; four lanes share a group of 32.
-__global__ void kv4_store_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t T, int64_t ks,
-                                 int64_t kh, int64_t vs, int64_t vh, const int64_t* __restrict__ slots,
-                                 uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, int64_t num_slots, int Hkv, int bs,
-                                 unsigned* err) {
-  griddep_wait();
-  griddep_launch();
-  const int64_t warp = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (warp >= T * Hkv) return;
-  const int64_t t = warp / Hkv;
-  const int h = (int)(warp % Hkv);
-  const int64_t slot = slots[t];
-  if (slot < 0) return;
+// Work of both kernels: a warp takes two tokens, lanes 0-15 the first and
+// 16-31 the second, and `hpw` heads of them, 8 dims a lane.  Two tokens that
+// follow one another share the 16-byte pieces of V's layout, so each store
+// instruction fills them whole.
+struct Kv4Pair {
+  int64_t t, rec0;  // token of this half warp; byte offset of its record for head 0
+  int tt, h0, h1;
+  bool on;
+};
+
+__device__ __forceinline__ Kv4Pair kv4_pair(int64_t T, int Hkv, int hpw, int bs, uint32_t num_slots,
+                                            const int64_t* slots, unsigned* err) {
+  Kv4Pair p;
+  const uint32_t groups = (uint32_t)(Hkv + hpw - 1) / hpw;
+  const uint32_t warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const uint32_t pair = warp / groups;
+  p.h0 = (int)(warp - pair * groups) * hpw;
+  p.h1 = min(p.h0 + hpw, Hkv);
+  p.t = 2 * (int64_t)pair + ((threadIdx.x >> 4) & 1);
+  int64_t slot = p.t < T ? slots[p.t] : -1;
   if (slot >= num_slots) {
-    if (lane == 0) report(err, ERR_SLOT_OOB);
-    return;
+    report(err, ERR_SLOT_OOB);
+    slot = -1;
   }
-  const bool is_v = lane >= 16;
-  const int i = lane & 15;
-  const bf16* src = is_v ? v + t * vs + h * vh : k + t * ks + h * kh;
-  const uint4 x4 = reinterpret_cast<const uint4*>(src)[i];
+  p.on = slot >= 0;
+  const uint32_t u = p.on ? (uint32_t)slot : 0, blk = u / bs, off = u - blk * bs;
+  p.rec0 = kv4_record(blk, 0, off / kKv4Tile, Hkv, bs / kKv4Tile);
+  p.tt = off % kKv4Tile;
+  return p;
+}
+
+// Offset of lane i's word of token tt: K word 4 (i % 4) + i / 4 (dims 8 i ..), V word i / 8 of octet
+// 4 (i % 2) + (i / 2) % 4 (after transpose4: dims 8 i ..).
+__device__ __forceinline__ int kv4_k_word(int tt, int i) { return 64 * tt + 4 * (4 * (i & 3) + (i >> 2)); }
+__device__ __forceinline__ int kv4_v_word(int tt, int i) {
+  return kv4_v_base(tt) + 64 * (4 * (i & 1) + ((i >> 1) & 3)) + 4 * (i >> 3);
+}
+
+// 8 bf16 of a group of 32 that four lanes hold together: the group's scale, and each value's code u as bits
+// 0-3 of code[e] (higher bits: those of 12582912.0f).
+__device__ __forceinline__ uint32_t kv4_quantise(uint4 x4, uint32_t (&code)[8]) {
   const uint32_t x2[4] = {x4.x, x4.y, x4.z, x4.w};
   // max |x| on the bit patterns: they order as the values do, infinities and NaN above every finite one.
   uint32_t mx = 0;
@@ -49,82 +67,118 @@ __global__ void kv4_store_kernel(const bf16* __restrict__ k, const bf16* __restr
   const bool finite = mx < 0x7f80u;
   const uint32_t sbits = finite ? (uint32_t)__bfloat16_as_ushort(tobf(__fdiv_rn(bf16_bits(mx), 7.f))) : 0x7fc0u;
   const float s = bf16_bits(sbits);
-  // x has 8 significant bits and s 8, so x / s is either exactly on a rounding border or at least 2^-9 off
-  // it: the fp32 quotient rounds as the exact one does.
-  uint32_t code[8];
+  // n = rint(x / s) as exact arithmetic has it.  x and s have 8 significant bits, so x / s >= 1/2 is exactly
+  // k + 1/2 or at least 1/510 off it.  x times the rounded 1 / s is within 2^-20 of x / s; rounded to
+  // multiples of 2^-12 an exact k + 1/2 is back in place and no other value crosses one.  |x / s| <= 7 + 2^-5
+  // needs no clamp.  A subnormal s (or none) has fewer bits: divide and clamp there.
+  if (finite && sbits >= 0x80u) {
+    const float r = __fdiv_rn(1.f, s);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = bf16_bits((e & 1) ? x2[e >> 1] >> 16 : x2[e >> 1] & 0xffffu);
-    const float n = (finite && s > 0.f) ? fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.f), 7.f) : 0.f;
-    code[e] = (uint32_t)((int)n + 8);
-  }
-  uint32_t w = 0;
-  if (!is_v) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w |= code[e] << (4 * ((e >> 1) + 4 * (e & 1)));
+    for (int e = 0; e < 8; ++e) {
+      const float x = __uint_as_float((e & 1) ? x2[e >> 1] & 0xffff0000u : x2[e >> 1] << 16);
+      const float y = __fadd_rn(__fmaf_rn(x, r, 0x1.8p11f), -0x1.8p11f);
+      code[e] = __float_as_uint(__fadd_rn(y, 12582920.f));  // 1.5 * 2^23 + 8
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w |= code[e] << (4 * e);
+    for (int e = 0; e < 8; ++e) {
+      const float x = __uint_as_float((e & 1) ? x2[e >> 1] & 0xffff0000u : x2[e >> 1] << 16);
+      const float n = (finite && s > 0.f) ? fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.f), 7.f) : 0.f;
+      code[e] = __float_as_uint(n + 12582920.f);
+    }
   }
-  const uint32_t wt = transpose4(w, lane);
-  const int64_t blk = slot / bs;
-  const int off = (int)(slot - blk * bs);
-  const int64_t rec = kv4_record(blk, h, off / kKv4Tile, Hkv, bs / kKv4Tile);
-  const int tt = off % kKv4Tile;
-  if (!is_v) {
-    *reinterpret_cast<uint32_t*>(kc + rec + 64 * tt + 4 * (4 * (i & 3) + (i >> 2))) = w;
-  } else {
-    const int g = 4 * (i & 1) + ((i >> 1) & 3), u = i >> 3;
-    *reinterpret_cast<uint32_t*>(vc + rec + kv4_v_base(tt) + 64 * g + 4 * u) = wt;
-  }
-  if ((i & 3) == 0)
-    *reinterpret_cast<uint16_t*>((is_v ? vc : kc) + rec + kKv4Codes + 8 * tt + 2 * (i >> 2)) = (uint16_t)sbits;
+  return sbits;
 }
 
-// One warp per (token, kv head): lanes 0-15 expand the K row, lanes 16-31 the V row, 8 dims each.
-__global__ void kv4_load_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, int64_t num_slots,
-                                int Hkv, int bs, const int64_t* __restrict__ slots,
-                                const int64_t* __restrict__ out_slots, int64_t T, bf16* __restrict__ ko,
-                                bf16* __restrict__ vo, int64_t out_total, int out_bs, unsigned* err) {
+__global__ void __launch_bounds__(256)
+    kv4_store_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t T, int64_t ks, int64_t kh,
+                     int64_t vs, int64_t vh, const int64_t* __restrict__ slots, uint8_t* __restrict__ kc,
+                     uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv, int hpw, int bs, unsigned* err) {
   griddep_wait();
   griddep_launch();
-  const int64_t warp = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (warp >= T * Hkv) return;
-  const int64_t t = warp / Hkv;
-  const int h = (int)(warp % Hkv);
-  const int64_t slot = slots[t], dst = out_slots ? out_slots[t] : t;
-  if (slot < 0 || dst < 0) return;
-  if (slot >= num_slots || dst >= out_total) {
-    if (lane == 0) report(err, ERR_SLOT_OOB);
-    return;
-  }
-  const bool is_v = lane >= 16;
-  const int i = lane & 15;
-  const int64_t blk = slot / bs;
-  const int off = (int)(slot - blk * bs);
-  const int64_t rec = kv4_record(blk, h, off / kKv4Tile, Hkv, bs / kKv4Tile);
-  const int tt = off % kKv4Tile;
-  uint32_t w;
-  if (!is_v) {
-    w = *reinterpret_cast<const uint32_t*>(kc + rec + 64 * tt + 4 * (4 * (i & 3) + (i >> 2)));
-  } else {
-    const int g = 4 * (i & 1) + ((i >> 1) & 3), u = i >> 3;
-    w = *reinterpret_cast<const uint32_t*>(vc + rec + kv4_v_base(tt) + 64 * g + 4 * u);
-  }
-  const uint32_t wt = transpose4(w, lane);
-  const float s = bf16_bits(
-      *reinterpret_cast<const uint16_t*>((is_v ? vc : kc) + rec + kKv4Codes + 8 * tt + 2 * (i >> 2)));
-  uint32_t y[4];
+  const int lane = threadIdx.x & 31, i = lane & 15;
+  const Kv4Pair p = kv4_pair(T, Hkv, hpw, bs, num_slots, slots, err);
+  const int64_t head_bytes = (int64_t)(bs / kKv4Tile) * kKv4Record;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 2
+  for (int h = p.h0; h < p.h1; ++h) {
+    const uint4 xk = p.on ? reinterpret_cast<const uint4*>(k + p.t * ks + h * kh)[i] : zero;
+    const uint4 xv = p.on ? reinterpret_cast<const uint4*>(v + p.t * vs + h * vh)[i] : zero;
+    const int64_t rec = p.rec0 + h * head_bytes;
+    uint32_t code[8];
+    // sum_e code[e] 16^place(e) carries 0x4b400000 16^0..7 along: take it off at the end
+    constexpr uint32_t carried = 0x4b400000u * 0x11111111u;
+    const uint32_t sk = kv4_quantise(xk, code);
+    uint32_t w = 0;  // nibble n holds dim 8 i + 2 (n % 4) + n / 4
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {  // dims 8 i + 2 p and + 1
-    const uint32_t lo = is_v ? wt >> (8 * p) : w >> (4 * p);
-    const uint32_t hi = is_v ? wt >> (8 * p + 4) : w >> (4 * p + 16);
-    y[p] = pack_bf16((float)((int)(lo & 15u) - 8) * s, (float)((int)(hi & 15u) - 8) * s);
+    for (int n = 7; n >= 0; --n) w = w * 16 + code[2 * (n & 3) + (n >> 2)];
+    w -= carried;
+    if (p.on) {
+      *reinterpret_cast<uint32_t*>(kc + rec + kv4_k_word(p.tt, i)) = w;
+      if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(kc + rec + kKv4Codes + 8 * p.tt + (i >> 1)) = (uint16_t)sk;
+    }
+    const uint32_t sv = kv4_quantise(xv, code);
+    w = 0;  // byte b holds dims 8 i + 2 b and + 1
+#pragma unroll
+    for (int e = 7; e >= 0; --e) w = w * 16 + code[e];
+    w = transpose4(w - carried, lane);
+    if (p.on) {
+      *reinterpret_cast<uint32_t*>(vc + rec + kv4_v_word(p.tt, i)) = w;
+      if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(vc + rec + kKv4Codes + 8 * p.tt + (i >> 1)) = (uint16_t)sv;
+    }
   }
-  const int64_t ob = dst / out_bs, oo = dst - ob * out_bs;
-  bf16* out = (is_v ? vo : ko) + ((ob * Hkv + h) * out_bs + oo) * 128;
-  reinterpret_cast<uint4*>(out)[i] = make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+__global__ void __launch_bounds__(256)
+    kv4_load_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv,
+                    int hpw, int bs, const int64_t* __restrict__ slots, const int64_t* __restrict__ out_slots,
+                    int64_t T, bf16* __restrict__ ko, bf16* __restrict__ vo, uint32_t out_total, int out_bs,
+                    unsigned* err) {
+  griddep_wait();
+  griddep_launch();
+  const int lane = threadIdx.x & 31, i = lane & 15;
+  Kv4Pair p = kv4_pair(T, Hkv, hpw, bs, num_slots, slots, err);
+  int64_t dst = p.on ? (out_slots ? out_slots[p.t] : p.t) : -1;
+  if (dst >= out_total) {
+    report(err, ERR_SLOT_OOB);
+    dst = -1;
+  }
+  p.on = dst >= 0;
+  const uint32_t u = p.on ? (uint32_t)dst : 0, ob = u / out_bs, oo = u - ob * out_bs;
+  const int64_t out0 = ((int64_t)ob * Hkv * out_bs + oo) * 16 + i;  // in 16-byte pieces
+  const int64_t head_bytes = (int64_t)(bs / kKv4Tile) * kKv4Record;
+#pragma unroll 4
+  for (int h = p.h0; h < p.h1; ++h) {
+    const int64_t rec = p.rec0 + h * head_bytes;
+    uint32_t wk = 0, wv = 0;
+    float fk = 0.f, fv = 0.f;
+    if (p.on) {
+      wk = *reinterpret_cast<const uint32_t*>(kc + rec + kv4_k_word(p.tt, i));
+      wv = *reinterpret_cast<const uint32_t*>(vc + rec + kv4_v_word(p.tt, i));
+      fk = bf16_bits(*reinterpret_cast<const uint16_t*>(kc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2)));
+      fv = bf16_bits(*reinterpret_cast<const uint16_t*>(vc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2)));
+    }
+    wv = transpose4(wv, lane);
+    uint32_t yk[4], yv[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {  // dims 8 i + 2 b and + 1
+      yk[b] = pack_bf16((float)((int)((wk >> (4 * b)) & 15u) - 8) * fk,
+                        (float)((int)((wk >> (4 * b + 16)) & 15u) - 8) * fk);
+      yv[b] = pack_bf16((float)((int)((wv >> (8 * b)) & 15u) - 8) * fv,
+                        (float)((int)((wv >> (8 * b + 4)) & 15u) - 8) * fv);
+    }
+    if (p.on) {
+      const int64_t at = out0 + (int64_t)h * out_bs * 16;
+      reinterpret_cast<uint4*>(ko)[at] = make_uint4(yk[0], yk[1], yk[2], yk[3]);
+      reinterpret_cast<uint4*>(vo)[at] = make_uint4(yv[0], yv[1], yv[2], yv[3]);
+    }
+  }
+}
+
+// Heads a warp walks: as many as leave every SM its fill of warps (64).
+static int kv4_heads_per_warp(int64_t T, int Hkv) {
+  const int64_t rows = (T + 1) / 2 * Hkv, want = (int64_t)sm_count() * 64;
+  return (int)(rows <= want ? 1 : rows / want < 4 ? rows / want : 4);
 }
 
 }  // namespace aacc
@@ -138,17 +192,19 @@ int aacc_kv4_store(const void* k, const void* v, int64_t num_tokens, int64_t k_r
                    void* v_cache, int64_t num_blocks, int num_kv_heads, int block_size, cudaStream_t stream) {
   if (num_tokens < 0 || num_kv_heads <= 0 || num_blocks <= 0 || block_size <= 0 || block_size % kKv4Tile)
     return set_error(AACC_ERR_INVALID, "kv4_store: bad sizes");
+  if (num_blocks > 0x7fffffff / block_size || num_tokens > 0x7fffffff / num_kv_heads)
+    return set_error(AACC_ERR_UNSUPPORTED, "kv4_store: pool or token count too large");
   if (num_tokens == 0) return AACC_OK;
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache) ||
       (k_row_stride | k_head_stride | v_row_stride | v_head_stride) % 8)
     return set_error(AACC_ERR_INVALID, "kv4_store: pointers/strides must be 16-byte aligned");
-  const int64_t blocks = (num_tokens * num_kv_heads + 7) / 8;
-  if (blocks > 0x7fffffff) return set_error(AACC_ERR_INVALID, "kv4_store: too many rows");
+  const int hpw = kv4_heads_per_warp(num_tokens, num_kv_heads);
+  const int64_t warps = (num_tokens + 1) / 2 * ((num_kv_heads + hpw - 1) / hpw);
   return check_launch("kv4_store",
-                      launch_k(kv4_store_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (const bf16*)k,
-                               (const bf16*)v, num_tokens, k_row_stride, k_head_stride, v_row_stride, v_head_stride,
-                               slot_mapping, (uint8_t*)k_cache, (uint8_t*)v_cache, num_blocks * block_size,
-                               num_kv_heads, block_size, device_error_ptr()));
+                      launch_k(kv4_store_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream,
+                               (const bf16*)k, (const bf16*)v, num_tokens, k_row_stride, k_head_stride, v_row_stride,
+                               v_head_stride, slot_mapping, (uint8_t*)k_cache, (uint8_t*)v_cache,
+                               (uint32_t)(num_blocks * block_size), num_kv_heads, hpw, block_size, device_error_ptr()));
 }
 
 int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, int num_kv_heads, int block_size,
@@ -157,16 +213,19 @@ int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, 
   if (num_tokens < 0 || num_kv_heads <= 0 || num_blocks <= 0 || block_size <= 0 || block_size % kKv4Tile ||
       out_blocks < 0 || out_block_size <= 0)
     return set_error(AACC_ERR_INVALID, "kv4_load: bad sizes");
+  if (num_blocks > 0x7fffffff / block_size || out_blocks > 0x7fffffff / out_block_size ||
+      num_tokens > 0x7fffffff / num_kv_heads)
+    return set_error(AACC_ERR_UNSUPPORTED, "kv4_load: pool or token count too large");
   if (num_tokens == 0) return AACC_OK;
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_out) || !aligned16(v_out))
     return set_error(AACC_ERR_INVALID, "kv4_load: pointers must be 16-byte aligned");
-  const int64_t blocks = (num_tokens * num_kv_heads + 7) / 8;
-  if (blocks > 0x7fffffff) return set_error(AACC_ERR_INVALID, "kv4_load: too many rows");
+  const int hpw = kv4_heads_per_warp(num_tokens, num_kv_heads);
+  const int64_t warps = (num_tokens + 1) / 2 * ((num_kv_heads + hpw - 1) / hpw);
   return check_launch(
-      "kv4_load", launch_k(kv4_load_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (const uint8_t*)k_cache,
-                           (const uint8_t*)v_cache, num_blocks * block_size, num_kv_heads, block_size, slots, out_slots,
-                           num_tokens, (bf16*)k_out, (bf16*)v_out, out_blocks * out_block_size, out_block_size,
-                           device_error_ptr()));
+      "kv4_load", launch_k(kv4_load_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream,
+                           (const uint8_t*)k_cache, (const uint8_t*)v_cache, (uint32_t)(num_blocks * block_size),
+                           num_kv_heads, hpw, block_size, slots, out_slots, num_tokens, (bf16*)k_out, (bf16*)v_out,
+                           (uint32_t)(out_blocks * out_block_size), out_block_size, device_error_ptr()));
 }
 
 }  // extern "C"

@@ -109,6 +109,8 @@ def _device_of(t: torch.Tensor, what: str, name: str) -> int:
 
 def _here(t: torch.Tensor, dtype, ndim: int, dev: int, what: str, name: str) -> None:
     """`t` must be a contiguous `ndim`-d `dtype` tensor on device `dev`."""
+    if t is None:
+        raise ValueError(f"{what}: {name} is missing")
     if t.dtype is not dtype or t.dim() != ndim or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {ndim}-d {dtype} tensor on cuda:{dev}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}, contiguous={t.is_contiguous()}")
