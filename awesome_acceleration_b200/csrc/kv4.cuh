@@ -40,6 +40,14 @@ __device__ __forceinline__ int kv4_v_base(int t) {
   return ((t >> 4) << 10) + ((r >> 3) << 9) + (((r & 7) >> 1) << 4) + ((r & 1) << 3);
 }
 
+// (x & M) | c in one operation; the compiler makes two of it.
+template <uint32_t M>
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t c) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(M), "r"(c));
+  return y;
+}
+
 // bf16 pattern -> fp32.
 __device__ __forceinline__ float bf16_bits(uint32_t u) { return __uint_as_float(u << 16); }
 

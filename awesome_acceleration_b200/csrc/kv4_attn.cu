@@ -185,9 +185,7 @@ __device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
 // Bits 0-3 (HI: 4-7) of both halves of x, a code u each, as the fp16 pair (u - 8, u' - 8).
 template <bool HI>
 __device__ __forceinline__ uint32_t code(uint32_t x) {
-  // 1024 + u, or 1024 + 16 u.  Written out, because (x & m) | c comes out as two operations otherwise.
-  uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(HI ? 0x00f000f0 : 0x000f000f), "r"(0x64006400));
+  const uint32_t y = and_or<HI ? 0x00f000f0u : 0x000f000fu>(x, 0x64006400u);  // 1024 + u, or 1024 + 16 u
   const __half2 h = *reinterpret_cast<const __half2*>(&y);
   const __half2 r = HI ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f))
                        : __hadd2(h, __float2half2_rn(-1032.f));

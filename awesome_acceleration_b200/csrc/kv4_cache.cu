@@ -58,21 +58,28 @@ __device__ __forceinline__ int kv4_v_word(int tt, int i) {
 // 0-3 of code[e] (higher bits: those of 12582912.0f).
 __device__ __forceinline__ uint32_t kv4_quantise(uint4 x4, uint32_t (&code)[8]) {
   const uint32_t x2[4] = {x4.x, x4.y, x4.z, x4.w};
-  // max |x| on the bit patterns: they order as the values do, infinities and NaN above every finite one.
-  uint32_t mx = 0;
+  // max |x|; a NaN stays one.
+  const __nv_bfloat162* xh = reinterpret_cast<const __nv_bfloat162*>(x2);
+  __nv_bfloat162 m2 = __hmax2_nan(__hmax2_nan(__habs2(xh[0]), __habs2(xh[1])),
+                                  __hmax2_nan(__habs2(xh[2]), __habs2(xh[3])));
 #pragma unroll
-  for (int n = 0; n < 4; ++n) mx = max(mx, max(x2[n] & 0x7fffu, (x2[n] >> 16) & 0x7fffu));
-  mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-  mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  const bool finite = mx < 0x7f80u;
-  const uint32_t sbits = finite ? (uint32_t)__bfloat16_as_ushort(tobf(__fdiv_rn(bf16_bits(mx), 7.f))) : 0x7fc0u;
+  for (int d = 1; d < 4; d <<= 1) {
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&m2), d);
+    m2 = __hmax2_nan(m2, *reinterpret_cast<const __nv_bfloat162*>(&y));
+  }
+  const float mx = bf(__hmax_nan(__low2bfloat16(m2), __high2bfloat16(m2)));
+  const bool finite = mx < INFINITY;
+  // max / 7 has 8 bits over 7: it is exact or at least 1/14 of bf16's step off a rounding border, so the
+  // product with the rounded 1/7 rounds as the quotient does.
+  const uint32_t sbits = finite ? (uint32_t)__bfloat16_as_ushort(tobf(mx * (1.f / 7.f))) : 0x7fc0u;
   const float s = bf16_bits(sbits);
   // n = rint(x / s) as exact arithmetic has it.  x and s have 8 significant bits, so x / s >= 1/2 is exactly
-  // k + 1/2 or at least 1/510 off it.  x times the rounded 1 / s is within 2^-20 of x / s; rounded to
+  // k + 1/2 or at least 1/510 off it.  x times the approximate 1 / s is within 2^-19 of x / s; rounded to
   // multiples of 2^-12 an exact k + 1/2 is back in place and no other value crosses one.  |x / s| <= 7 + 2^-5
   // needs no clamp.  A subnormal s (or none) has fewer bits: divide and clamp there.
   if (finite && sbits >= 0x80u) {
-    const float r = __fdiv_rn(1.f, s);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));  // 2^-126 <= s < 2^126: within 1 ulp
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = __uint_as_float((e & 1) ? x2[e >> 1] & 0xffff0000u : x2[e >> 1] << 16);
@@ -129,6 +136,15 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Codes u in bits 0-3 and 16-19 of x times the bf16 pair `s`: 128 + u - 136 is exact in bf16, so
+// the product is rounded once, to the bf16 that n s rounds to.
+__device__ __forceinline__ uint32_t kv4_value(uint32_t x, uint32_t s) {
+  const uint32_t u = and_or<0x000f000fu>(x, 0x43004300u);
+  const __nv_bfloat162 n = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(-136.f));
+  const __nv_bfloat162 y = __hmul2(n, *reinterpret_cast<const __nv_bfloat162*>(&s));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
 __global__ void __launch_bounds__(256)
     kv4_load_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv,
                     int hpw, int bs, const int64_t* __restrict__ slots, const int64_t* __restrict__ out_slots,
@@ -150,22 +166,22 @@ __global__ void __launch_bounds__(256)
 #pragma unroll 4
   for (int h = p.h0; h < p.h1; ++h) {
     const int64_t rec = p.rec0 + h * head_bytes;
-    uint32_t wk = 0, wv = 0;
-    float fk = 0.f, fv = 0.f;
+    uint32_t wk = 0, wv = 0, sk = 0, sv = 0;
     if (p.on) {
       wk = *reinterpret_cast<const uint32_t*>(kc + rec + kv4_k_word(p.tt, i));
       wv = *reinterpret_cast<const uint32_t*>(vc + rec + kv4_v_word(p.tt, i));
-      fk = bf16_bits(*reinterpret_cast<const uint16_t*>(kc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2)));
-      fv = bf16_bits(*reinterpret_cast<const uint16_t*>(vc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2)));
+      sk = *reinterpret_cast<const uint16_t*>(kc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2));
+      sv = *reinterpret_cast<const uint16_t*>(vc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2));
     }
     wv = transpose4(wv, lane);
+    sk = __byte_perm(sk, 0, 0x1010);
+    sv = __byte_perm(sv, 0, 0x1010);
     uint32_t yk[4], yv[4];
+    const uint32_t lo = wv & 0x0f0f0f0fu, hi = (wv >> 4) & 0x0f0f0f0fu;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {  // dims 8 i + 2 b and + 1
-      yk[b] = pack_bf16((float)((int)((wk >> (4 * b)) & 15u) - 8) * fk,
-                        (float)((int)((wk >> (4 * b + 16)) & 15u) - 8) * fk);
-      yv[b] = pack_bf16((float)((int)((wv >> (8 * b)) & 15u) - 8) * fv,
-                        (float)((int)((wv >> (8 * b + 4)) & 15u) - 8) * fv);
+      yk[b] = kv4_value(wk >> (4 * b), sk);
+      yv[b] = kv4_value(__byte_perm(lo, hi, b | (4 + b) << 8), sv);
     }
     if (p.on) {
       const int64_t at = out0 + (int64_t)h * out_bs * 16;
