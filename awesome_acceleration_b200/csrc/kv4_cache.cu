@@ -16,23 +16,41 @@ __device__ __forceinline__ uint32_t transpose4(uint32_t w, int lane) {
   return (lane & 2) ? __byte_perm(w, y, 0x3715) : __byte_perm(w, y, 0x6240);
 }
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994): with 2^(L-1) < d <= 2^L and
+// m = ceil(2^(31+L) / d), floor(n / d) = floor(n m / 2^(31+L)).
+struct Divide {
+  uint32_t d, m, sh;
+  explicit Divide(uint32_t d_) : d(d_), m(0), sh(0) {
+    if (d == 1) return;
+    uint32_t L = 1;
+    while ((uint64_t(1) << L) < d) ++L;
+    m = (uint32_t)(((uint64_t(1) << (31 + L)) + d - 1) / d);
+    sh = L - 1;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return m ? __umulhi(n, m) >> sh : n; }
+};
+
 // Work of both kernels: a warp takes two tokens, lanes 0-15 the first and
-// 16-31 the second, and `hpw` heads of them, 8 dims a lane.  Two tokens that
-// follow one another share the 16-byte pieces of V's layout, so each store
-// instruction fills them whole.
+// 16-31 the second, and `hpw` heads of them, 8 dims a lane; the loads of
+// several heads are in flight together.  Two tokens that follow one another
+// share the 16-byte pieces of V's layout, so each store instruction fills
+// them whole.
+constexpr int kStoreHeads = 2;  // heads whose loads are issued together (registers: 8 a head)
+constexpr int kLoadHeads = 4;   // (4 a head)
+
 struct Kv4Pair {
   int64_t t, rec0;  // token of this half warp; byte offset of its record for head 0
   int tt, h0, h1;
   bool on;
 };
 
-__device__ __forceinline__ Kv4Pair kv4_pair(int64_t T, int Hkv, int hpw, int bs, uint32_t num_slots,
-                                            const int64_t* slots, unsigned* err) {
+__device__ __forceinline__ Kv4Pair kv4_pair(int64_t T, int Hkv, int hpw, Divide groups, Divide bs,
+                                            uint32_t num_slots, const int64_t* slots, unsigned* err) {
   Kv4Pair p;
-  const uint32_t groups = (uint32_t)(Hkv + hpw - 1) / hpw;
   const uint32_t warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const uint32_t pair = warp / groups;
-  p.h0 = (int)(warp - pair * groups) * hpw;
+  const uint32_t pair = groups(warp);
+  p.h0 = (int)(warp - pair * groups.d) * hpw;
   p.h1 = min(p.h0 + hpw, Hkv);
   p.t = 2 * (int64_t)pair + ((threadIdx.x >> 4) & 1);
   int64_t slot = p.t < T ? slots[p.t] : -1;
@@ -41,8 +59,8 @@ __device__ __forceinline__ Kv4Pair kv4_pair(int64_t T, int Hkv, int hpw, int bs,
     slot = -1;
   }
   p.on = slot >= 0;
-  const uint32_t u = p.on ? (uint32_t)slot : 0, blk = u / bs, off = u - blk * bs;
-  p.rec0 = kv4_record(blk, 0, off / kKv4Tile, Hkv, bs / kKv4Tile);
+  const uint32_t u = p.on ? (uint32_t)slot : 0, blk = bs(u), off = u - blk * bs.d;
+  p.rec0 = kv4_record(blk, 0, off / kKv4Tile, Hkv, bs.d / kKv4Tile);
   p.tt = off % kKv4Tile;
   return p;
 }
@@ -100,38 +118,50 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint4 x4, uint32_t (&code)[8]) 
 __global__ void __launch_bounds__(256)
     kv4_store_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t T, int64_t ks, int64_t kh,
                      int64_t vs, int64_t vh, const int64_t* __restrict__ slots, uint8_t* __restrict__ kc,
-                     uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv, int hpw, int bs, unsigned* err) {
+                     uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv, int hpw, Divide groups, Divide bs,
+                     unsigned* err) {
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31, i = lane & 15;
-  const Kv4Pair p = kv4_pair(T, Hkv, hpw, bs, num_slots, slots, err);
-  const int64_t head_bytes = (int64_t)(bs / kKv4Tile) * kKv4Record;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
-  for (int h = p.h0; h < p.h1; ++h) {
-    const uint4 xk = p.on ? reinterpret_cast<const uint4*>(k + p.t * ks + h * kh)[i] : zero;
-    const uint4 xv = p.on ? reinterpret_cast<const uint4*>(v + p.t * vs + h * vh)[i] : zero;
-    const int64_t rec = p.rec0 + h * head_bytes;
-    uint32_t code[8];
-    // sum_e code[e] 16^place(e) carries 0x4b400000 16^0..7 along: take it off at the end
-    constexpr uint32_t carried = 0x4b400000u * 0x11111111u;
-    const uint32_t sk = kv4_quantise(xk, code);
-    uint32_t w = 0;  // nibble n holds dim 8 i + 2 (n % 4) + n / 4
+  const Kv4Pair p = kv4_pair(T, Hkv, hpw, groups, bs, num_slots, slots, err);
+  const int64_t head_bytes = (int64_t)(bs.d / kKv4Tile) * kKv4Record;
+  const int scale_at = kKv4Codes + 8 * p.tt + (i >> 1);
+  kc += p.rec0;
+  vc += p.rec0;
+  k += p.t * ks + 8 * i;
+  v += p.t * vs + 8 * i;
+  for (int h0 = p.h0; h0 < p.h1; h0 += kStoreHeads) {
+    uint4 xk[kStoreHeads], xv[kStoreHeads];
 #pragma unroll
-    for (int n = 7; n >= 0; --n) w = w * 16 + code[2 * (n & 3) + (n >> 2)];
-    w -= carried;
-    if (p.on) {
-      *reinterpret_cast<uint32_t*>(kc + rec + kv4_k_word(p.tt, i)) = w;
-      if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(kc + rec + kKv4Codes + 8 * p.tt + (i >> 1)) = (uint16_t)sk;
+    for (int q = 0; q < kStoreHeads; ++q) {
+      const bool on = p.on && h0 + q < p.h1;
+      xk[q] = on ? *reinterpret_cast<const uint4*>(k + (h0 + q) * kh) : make_uint4(0, 0, 0, 0);
+      xv[q] = on ? *reinterpret_cast<const uint4*>(v + (h0 + q) * vh) : make_uint4(0, 0, 0, 0);
     }
-    const uint32_t sv = kv4_quantise(xv, code);
-    w = 0;  // byte b holds dims 8 i + 2 b and + 1
 #pragma unroll
-    for (int e = 7; e >= 0; --e) w = w * 16 + code[e];
-    w = transpose4(w - carried, lane);
-    if (p.on) {
-      *reinterpret_cast<uint32_t*>(vc + rec + kv4_v_word(p.tt, i)) = w;
-      if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(vc + rec + kKv4Codes + 8 * p.tt + (i >> 1)) = (uint16_t)sv;
+    for (int q = 0; q < kStoreHeads; ++q) {
+      const bool on = p.on && h0 + q < p.h1;
+      const int64_t rec = (h0 + q) * head_bytes;
+      uint32_t code[8];
+      // sum_e code[e] 16^place(e) carries 0x4b400000 16^0..7 along: take it off at the end
+      constexpr uint32_t carried = 0x4b400000u * 0x11111111u;
+      const uint32_t sk = kv4_quantise(xk[q], code);
+      uint32_t w = 0;  // nibble n holds dim 8 i + 2 (n % 4) + n / 4
+#pragma unroll
+      for (int n = 7; n >= 0; --n) w = w * 16 + code[2 * (n & 3) + (n >> 2)];
+      if (on) {
+        *reinterpret_cast<uint32_t*>(kc + rec + kv4_k_word(p.tt, i)) = w - carried;
+        if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(kc + rec + scale_at) = (uint16_t)sk;
+      }
+      const uint32_t sv = kv4_quantise(xv[q], code);
+      w = 0;  // byte b holds dims 8 i + 2 b and + 1
+#pragma unroll
+      for (int e = 7; e >= 0; --e) w = w * 16 + code[e];
+      w = transpose4(w - carried, lane);
+      if (on) {
+        *reinterpret_cast<uint32_t*>(vc + rec + kv4_v_word(p.tt, i)) = w;
+        if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(vc + rec + scale_at) = (uint16_t)sv;
+      }
     }
   }
 }
@@ -147,46 +177,56 @@ __device__ __forceinline__ uint32_t kv4_value(uint32_t x, uint32_t s) {
 
 __global__ void __launch_bounds__(256)
     kv4_load_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv,
-                    int hpw, int bs, const int64_t* __restrict__ slots, const int64_t* __restrict__ out_slots,
-                    int64_t T, bf16* __restrict__ ko, bf16* __restrict__ vo, uint32_t out_total, int out_bs,
-                    unsigned* err) {
+                    int hpw, Divide groups, Divide bs, const int64_t* __restrict__ slots,
+                    const int64_t* __restrict__ out_slots, int64_t T, bf16* __restrict__ ko, bf16* __restrict__ vo,
+                    uint32_t out_total, Divide out_bs, unsigned* err) {
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31, i = lane & 15;
-  Kv4Pair p = kv4_pair(T, Hkv, hpw, bs, num_slots, slots, err);
+  Kv4Pair p = kv4_pair(T, Hkv, hpw, groups, bs, num_slots, slots, err);
   int64_t dst = p.on ? (out_slots ? out_slots[p.t] : p.t) : -1;
   if (dst >= out_total) {
     report(err, ERR_SLOT_OOB);
     dst = -1;
   }
   p.on = dst >= 0;
-  const uint32_t u = p.on ? (uint32_t)dst : 0, ob = u / out_bs, oo = u - ob * out_bs;
-  const int64_t out0 = ((int64_t)ob * Hkv * out_bs + oo) * 16 + i;  // in 16-byte pieces
-  const int64_t head_bytes = (int64_t)(bs / kKv4Tile) * kKv4Record;
-#pragma unroll 4
-  for (int h = p.h0; h < p.h1; ++h) {
-    const int64_t rec = p.rec0 + h * head_bytes;
-    uint32_t wk = 0, wv = 0, sk = 0, sv = 0;
-    if (p.on) {
-      wk = *reinterpret_cast<const uint32_t*>(kc + rec + kv4_k_word(p.tt, i));
-      wv = *reinterpret_cast<const uint32_t*>(vc + rec + kv4_v_word(p.tt, i));
-      sk = *reinterpret_cast<const uint16_t*>(kc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2));
-      sv = *reinterpret_cast<const uint16_t*>(vc + rec + kKv4Codes + 8 * p.tt + 2 * (i >> 2));
-    }
-    wv = transpose4(wv, lane);
-    sk = __byte_perm(sk, 0, 0x1010);
-    sv = __byte_perm(sv, 0, 0x1010);
-    uint32_t yk[4], yv[4];
-    const uint32_t lo = wv & 0x0f0f0f0fu, hi = (wv >> 4) & 0x0f0f0f0fu;
+  const uint32_t u = p.on ? (uint32_t)dst : 0, ob = out_bs(u), oo = u - ob * out_bs.d;
+  const int64_t out0 = ((int64_t)ob * Hkv * out_bs.d + oo) * 16 + i;  // in 16-byte pieces
+  const int64_t head_bytes = (int64_t)(bs.d / kKv4Tile) * kKv4Record;
+  const int scale_at = kKv4Codes + 8 * p.tt + 2 * (i >> 2);
+  const uint8_t* kr = kc + p.rec0;
+  const uint8_t* vr = vc + p.rec0;
+  uint4* ow = reinterpret_cast<uint4*>(ko) + out0;
+  uint4* vw = reinterpret_cast<uint4*>(vo) + out0;
+  for (int h0 = p.h0; h0 < p.h1; h0 += kLoadHeads) {
+    uint32_t wk[kLoadHeads], wv[kLoadHeads], sk[kLoadHeads], sv[kLoadHeads];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {  // dims 8 i + 2 b and + 1
-      yk[b] = kv4_value(wk >> (4 * b), sk);
-      yv[b] = kv4_value(__byte_perm(lo, hi, b | (4 + b) << 8), sv);
+    for (int q = 0; q < kLoadHeads; ++q) {
+      wk[q] = wv[q] = sk[q] = sv[q] = 0;
+      if (p.on && h0 + q < p.h1) {
+        const int64_t rec = (h0 + q) * head_bytes;
+        wk[q] = *reinterpret_cast<const uint32_t*>(kr + rec + kv4_k_word(p.tt, i));
+        wv[q] = *reinterpret_cast<const uint32_t*>(vr + rec + kv4_v_word(p.tt, i));
+        sk[q] = *reinterpret_cast<const uint16_t*>(kr + rec + scale_at);
+        sv[q] = *reinterpret_cast<const uint16_t*>(vr + rec + scale_at);
+      }
     }
-    if (p.on) {
-      const int64_t at = out0 + (int64_t)h * out_bs * 16;
-      reinterpret_cast<uint4*>(ko)[at] = make_uint4(yk[0], yk[1], yk[2], yk[3]);
-      reinterpret_cast<uint4*>(vo)[at] = make_uint4(yv[0], yv[1], yv[2], yv[3]);
+#pragma unroll
+    for (int q = 0; q < kLoadHeads; ++q) {
+      const uint32_t x = transpose4(wv[q], lane);
+      const uint32_t lo = x & 0x0f0f0f0fu, hi = (x >> 4) & 0x0f0f0f0fu;
+      const uint32_t fk = __byte_perm(sk[q], 0, 0x1010), fv = __byte_perm(sv[q], 0, 0x1010);
+      uint32_t yk[4], yv[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {  // dims 8 i + 2 b and + 1
+        yk[b] = kv4_value(wk[q] >> (4 * b), fk);
+        yv[b] = kv4_value(__byte_perm(lo, hi, b | (4 + b) << 8), fv);
+      }
+      if (p.on && h0 + q < p.h1) {
+        const int64_t at = (int64_t)(h0 + q) * out_bs.d * 16;
+        ow[at] = make_uint4(yk[0], yk[1], yk[2], yk[3]);
+        vw[at] = make_uint4(yv[0], yv[1], yv[2], yv[3]);
+      }
     }
   }
 }
@@ -220,7 +260,8 @@ int aacc_kv4_store(const void* k, const void* v, int64_t num_tokens, int64_t k_r
                       launch_k(kv4_store_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream,
                                (const bf16*)k, (const bf16*)v, num_tokens, k_row_stride, k_head_stride, v_row_stride,
                                v_head_stride, slot_mapping, (uint8_t*)k_cache, (uint8_t*)v_cache,
-                               (uint32_t)(num_blocks * block_size), num_kv_heads, hpw, block_size, device_error_ptr()));
+                               (uint32_t)(num_blocks * block_size), num_kv_heads, hpw,
+                               Divide((num_kv_heads + hpw - 1) / hpw), Divide(block_size), device_error_ptr()));
 }
 
 int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, int num_kv_heads, int block_size,
@@ -240,8 +281,9 @@ int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, 
   return check_launch(
       "kv4_load", launch_k(kv4_load_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream,
                            (const uint8_t*)k_cache, (const uint8_t*)v_cache, (uint32_t)(num_blocks * block_size),
-                           num_kv_heads, hpw, block_size, slots, out_slots, num_tokens, (bf16*)k_out, (bf16*)v_out,
-                           (uint32_t)(out_blocks * out_block_size), out_block_size, device_error_ptr()));
+                           num_kv_heads, hpw, Divide((num_kv_heads + hpw - 1) / hpw), Divide(block_size), slots,
+                           out_slots, num_tokens, (bf16*)k_out, (bf16*)v_out, (uint32_t)(out_blocks * out_block_size),
+                           Divide(out_block_size), device_error_ptr()));
 }
 
 }  // extern "C"
