@@ -42,40 +42,54 @@ __device__ __forceinline__ int64_t block_scan_excl(int64_t v, int64_t* sh, int64
 }
 
 __device__ __forceinline__ int64_t blocks_of(int32_t len, int bs, int64_t max_blocks) {
-  const int64_t need = len > 0 ? ((int64_t)len + bs - 1) / bs : 0;
+  const int64_t need = len > 0 ? ((uint32_t)len - 1) / (uint32_t)bs + 1 : 0;  // 32-bit: a 64-bit division is a loop
   return min(need, max_blocks);
 }
 
-// One CTA per request: its first block is the number of blocks that the
-// requests before it take.
+// One CTA per run of `per` requests: the first one's first block is the number
+// of blocks that all requests before it take, the others' follow by a scan.
+// A warp writes a row.
 __global__ void __launch_bounds__(kMapThreads)
-    build_block_tables_kernel(const int32_t* __restrict__ lengths, int64_t n, int bs,
+    build_block_tables_kernel(const int32_t* __restrict__ lengths, int64_t n, int64_t per, int bs,
                               const int32_t* __restrict__ free_blocks, int64_t num_free, int32_t* __restrict__ tables,
                               int64_t max_blocks, int32_t* __restrict__ used, unsigned* err) {
   __shared__ int64_t sh[kMapThreads / 32];
+  __shared__ int64_t first[kMapThreads], count[kMapThreads];
   griddep_wait();
   griddep_launch();
-  const int64_t i = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t i0 = blockIdx.x * per, i1 = min(n, i0 + per);
   int64_t part = 0, off;
-  for (int64_t j = threadIdx.x; j < i; j += kMapThreads) part += blocks_of(lengths[j], bs, max_blocks);
+  for (int64_t j = threadIdx.x; j < i0; j += kMapThreads) part += blocks_of(lengths[j], bs, max_blocks);
   block_scan_excl(part, sh, &off);
-  const int32_t len = lengths[i];
-  const int64_t need = blocks_of(len, bs, max_blocks);
-  for (int64_t j = threadIdx.x; j < max_blocks; j += kMapThreads) {
-    int32_t b = -1;
-    if (j < need) {
-      const int64_t at = off + j;
-      if (at >= num_free)
-        report(err, ERR_BLOCK_OOB);
-      else
-        b = free_blocks ? free_blocks[at] : (int32_t)at;
-    }
-    tables[i * max_blocks + j] = b;
-  }
-  if (threadIdx.x == 0) {
+  for (int64_t r0 = i0; r0 < i1; r0 += kMapThreads) {
+    const int64_t i = r0 + threadIdx.x;
+    const int32_t len = i < i1 ? lengths[i] : 0;
+    const int64_t need = blocks_of(len, bs, max_blocks);
     if ((int64_t)len > max_blocks * bs) report(err, ERR_CTX_OOB);
-    if (i == n - 1 && used) *used = (int32_t)min(off + need, (int64_t)0x7fffffff);
+    int64_t total;
+    first[threadIdx.x] = off + block_scan_excl(need, sh, &total);
+    count[threadIdx.x] = need;
+    off += total;
+    __syncthreads();
+    const int m = (int)min((int64_t)kMapThreads, i1 - r0);
+    for (int r = warp; r < m; r += kMapThreads / 32) {
+      const int64_t at0 = first[r], c = count[r];
+      int32_t* row = tables + (r0 + r) * max_blocks;
+      for (int64_t j = lane; j < max_blocks; j += 32) {
+        int32_t b = -1;
+        if (j < c) {
+          if (at0 + j >= num_free)
+            report(err, ERR_BLOCK_OOB);
+          else
+            b = free_blocks ? free_blocks[at0 + j] : (int32_t)(at0 + j);
+        }
+        row[j] = b;
+      }
+    }
+    __syncthreads();  // first and count are rewritten
   }
+  if (i1 == n && threadIdx.x == 0 && used) *used = (int32_t)min(off, (int64_t)0x7fffffff);
 }
 
 // One CTA per kMapTokens packed tokens.  It walks the requests in chunks; of
@@ -132,8 +146,8 @@ __global__ void __launch_bounds__(kMapThreads)
       if (row >= num_rows) {
         report(err, ERR_SLOT_OOB);
       } else if (row >= 0) {  // negative rows are padding
-        const int64_t j = pos / bs;
-        if (pos < 0 || j >= max_blocks) {
+        const int64_t j = (uint32_t)pos / (uint32_t)bs;
+        if (pos < 0 || pos > 0x7fffffff || j >= max_blocks) {
           report(err, ERR_CTX_OOB);
         } else {
           const int64_t blk = bt[row * max_blocks + j];
@@ -171,10 +185,12 @@ int aacc_build_block_tables(const int32_t* lengths, int64_t num_requests, int bl
   if (num_requests < 0 || num_requests > 0x7fffffff || block_size <= 0 || max_blocks <= 0 || num_free < 0)
     return set_error(AACC_ERR_INVALID, "build_block_tables: bad sizes");
   if (num_requests == 0) return AACC_OK;
+  // A CTA per SM at most twice over: each reads all the lengths before its own.
+  const int64_t per = (num_requests + 2 * sm_count() - 1) / (2 * sm_count());
   return check_launch("build_block_tables",
-                      launch_k(build_block_tables_kernel, dim3((unsigned)num_requests), dim3(kMapThreads), 0, stream,
-                               lengths, num_requests, block_size, free_blocks, num_free, block_tables, max_blocks,
-                               used, device_error_ptr()));
+                      launch_k(build_block_tables_kernel, dim3((unsigned)((num_requests + per - 1) / per)),
+                               dim3(kMapThreads), 0, stream, lengths, num_requests, per, block_size, free_blocks,
+                               num_free, block_tables, max_blocks, used, device_error_ptr()));
 }
 
 int aacc_build_slot_maps(const int32_t* lengths, const int32_t* starts, const int64_t* rows, int64_t num_requests,
