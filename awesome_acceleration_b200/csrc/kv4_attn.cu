@@ -23,18 +23,22 @@
 // call on instruction fetches.
 //
 // Q.K: the tokens are the rows of m16n8k16's A operand, the G <= 8 query heads
-// its 8 columns.  A code u becomes 1024 + u or 1024 + 16 u in fp16 by one
-// and-or where it lies, then u - 8 by one fp16x2 add or fma, exactly.  q is
-// scaled by a power of two per head to a largest element in [2^14, 2^15), so
-// that bf16 values go into fp16 unrounded down to 2^-28 of the largest.  The
-// group's scale multiplies the fp32 sum.
-// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand.  P^T is 2^4 p
-// in fp16 (the 2^4 also in the sum it is divided by), p < 2^6, transposed in
-// registers and multiplied by the V scales of its two tokens in fp16: two
-// roundings of 2^-12, a quarter of what one to bf16 costs.  The scales are
-// held relative to the largest so far, at [2^4, 2^5): products reach 2^15, and
-// a p down to 2^-18 and a scale down to 2^-21 of the largest have no other
-// rounding than those two.
+// its 8 columns.  With all else masked off, four bits at the foot of an fp16
+// are the subnormal 2^-24 u, or 2^-20 u one nibble higher, and the tensor
+// cores take subnormals as they are: an AND makes two operands.  The 2^24 is
+// put right in the softmax scale, the 16 in q, and the offset of 8 through the
+// accumulator's start, -8 sum(q) of the group; the group's scale multiplies
+// the fp32 sum.  q is scaled by a power of two per head to a largest element
+// in [2^14, 2^15), so that bf16 values go into fp16 unrounded down to 2^-24 of
+// the largest.
+// P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand.  Here the sum
+// over thousands of tokens would cancel against its offset, so u - 8 is made
+// exactly, by one more fp16x2 add or fma.  P^T is 2^4 p in fp16 (the 2^4 also
+// in the sum it is divided by), p < 2^6, transposed in registers and multiplied
+// by the V scales of its two tokens in fp16: two roundings of 2^-12, a quarter
+// of what one to bf16 costs.  The scales are held relative to the largest so
+// far, at [2^4, 2^5): products reach 2^15, and a p down to 2^-18 and a scale
+// down to 2^-21 of the largest have no other rounding than those two.
 // Once per tile each lane turns the scales of its two tokens into such pairs.
 #include <cuda_fp16.h>
 
@@ -47,6 +51,12 @@ namespace aacc {
 
 constexpr int kAttWarps = 16;
 constexpr int kAttThreads = kAttWarps * 32;
+
+// A run of tiles [t0, t1) of item (b, h), whose row has n tiles; u is the unit number of t0.
+struct Kv4Seg {
+  uint32_t u;
+  int b, row, h, n, t0, t1, ctx;
+};
 
 template <int G>
 struct Kv4Smem {
@@ -61,6 +71,8 @@ struct Kv4Smem {
   uint32_t wsum[5][kAttWarps];
   uint64_t kfull[kAttWarps];
   uint64_t vfull[kAttWarps];
+  Kv4Seg ahead[kAttWarps];  // where each warp's loads are: segment, and
+  int ahead_t[kAttWarps];          // its next tile there that is not in the warp's list
   int last[kAttWarps];
   int abort;
 };
@@ -80,12 +92,6 @@ struct Kv4Args {
   int64_t max_blocks;
   int num_blocks, num_rows, batch, max_ctx, ctx_add, Hkv, tpb;  // tpb: tiles per block
   float scale;
-};
-
-// A run of tiles [t0, t1) of item (b, h), whose row has n tiles; u is the unit number of t0.
-struct Kv4Seg {
-  uint32_t u;
-  int b, row, h, n, t0, t1, ctx;
 };
 
 // Tokens of batch row b (0: padding, outside the tables, or empty).
@@ -150,13 +156,14 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   return y;
 }
 
-// d = a b, with no accumulator to clear.
-__device__ __forceinline__ void mma_f16_16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// d = a b + c, where c holds for both rows of a column pair.
+__device__ __forceinline__ void mma_f16_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                                   const float (&c)[2]) {
   asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%10,%10,%10,%10};"
+      "{%10,%11,%10,%11};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
 }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
@@ -182,10 +189,16 @@ __device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Bits 0-3 (HI: 4-7) of both halves of x, a code u each, as the fp16 pair (u - 8, u' - 8).
+// Bits 0-3 (HI: 4-7) of both halves of x, a code u each: as fp16 subnormals 2^-24 u (HI: 2^-20 u).
+template <bool HI>
+__device__ __forceinline__ uint32_t code_sub(uint32_t x) {
+  return x & (HI ? 0x00f000f0u : 0x000f000fu);
+}
+
+// The same as the fp16 pair (u - 8, u' - 8), through 1024 + u or 1024 + 16 u.
 template <bool HI>
 __device__ __forceinline__ uint32_t code(uint32_t x) {
-  const uint32_t y = and_or<HI ? 0x00f000f0u : 0x000f000fu>(x, 0x64006400u);  // 1024 + u, or 1024 + 16 u
+  const uint32_t y = and_or<HI ? 0x00f000f0u : 0x000f000fu>(x, 0x64006400u);
   const __half2 h = *reinterpret_cast<const __half2*>(&y);
   const __half2 r = HI ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f))
                        : __hadd2(h, __float2half2_rn(-1032.f));
@@ -327,23 +340,40 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       cs.t0 = (int)((u0 - u) - (uint32_t)cs.h * rounds) << tsh;
       cs.t1 = seg_end(cs.n, cs.t0, uend - u0, tsh);
     }
-    // The loads run one tile ahead of the arithmetic, across segments: tile lt of segment ls, which is
-    // tile lti of entry lbi of the row's block table.
-    Kv4Seg ls = cs;
-    int lt = ls.t0 + wt;
-    bool lhas = true;
-    while (lhas && lt >= ls.t1) {
-      lhas = kv4_next(a, sm, ls, uend, tsh);
-      lt = ls.t0 + wt;
-    }
-    int lbi = lt / a.tpb, lti = lt - lbi * a.tpb;
-    int32_t lid = lhas ? a.bt[ls.row * a.max_blocks + lbi] : 0;
-    auto record = [&]() -> int64_t {
-      if ((uint32_t)lid >= (uint32_t)a.num_blocks) {
-        if (lane == 0) report(a.err, ERR_BLOCK_OOB);
-        lid = 0;  // a valid address keeps the pipeline going; the result is flagged
+    // The loads run one tile ahead of the arithmetic, across segments.  The warp lists up to 32 of its tiles
+    // at a time, a tile per lane: block id `ids` and, within the block's records, `sub`; entry li of ln is next.
+    // The segment they come from rests in shared memory.
+    sm.ahead[warp] = cs;
+    sm.ahead_t[warp] = cs.t0 + wt;
+    __syncwarp();
+    int32_t ids = 0;
+    int sub = 0, li = 0, ln = 0;
+    auto list_tiles = [&]() {
+      Kv4Seg s = sm.ahead[warp];
+      int t = sm.ahead_t[warp];
+      li = 0;
+      ln = 0;
+      while (t >= s.t1) {
+        if (!kv4_next(a, sm, s, uend, tsh)) return;
+        t = s.t0 + wt;
       }
-      return kv4_record(lid, ls.h, lti, a.Hkv, a.tpb);
+      ln = min(32, (s.t1 - t + T - 1) >> tsh);
+      const int mine = min(t + (lane << tsh), s.t1 - 1), bi = mine / a.tpb;
+      ids = a.bt[s.row * a.max_blocks + bi];
+      sub = s.h * a.tpb + (mine - bi * a.tpb);
+      __syncwarp();
+      sm.ahead[warp] = s;
+      sm.ahead_t[warp] = t + (ln << tsh);
+      __syncwarp();
+    };
+    auto record = [&]() -> int64_t {
+      int32_t id = __shfl_sync(0xffffffffu, ids, li);
+      const int at = __shfl_sync(0xffffffffu, sub, li);
+      if ((uint32_t)id >= (uint32_t)a.num_blocks) {
+        if (lane == 0) report(a.err, ERR_BLOCK_OOB);
+        id = 0;  // a valid address keeps the pipeline going; the result is flagged
+      }
+      return ((int64_t)id * (a.Hkv * a.tpb) + at) * kKv4Record;
     };
     auto load_k = [&](int64_t rec) {
       if (lane == 0) {
@@ -357,6 +387,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         bulk_load(sm.v[warp], a.vc + rec, kKv4Record, &sm.vfull[warp]);
       }
     };
+    list_tiles();
+    bool lhas = ln > 0;  // there is a tile to load
     if (lhas) {
       const int64_t rec = record();
       load_k(rec);
@@ -370,7 +402,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       // ---- queries of the item: B operand, column g = query head (columns >= G are zero)
       const int64_t qh0 = ((int64_t)cs.b * a.Hkv + cs.h) * G;
       uint32_t qf[4][4];
-      float sl0, sl1;  // log2 softmax scale of the raw scores of heads 2c and 2c + 1
+      float sl0, sl1;     // log2 softmax scale of the raw scores of heads 2c and 2c + 1
+      float corr[4][2];  // -8 times 2^-24 times the sum of their q over group w
       {
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns q's sign
         uint32_t mx = 0;
@@ -390,16 +423,26 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         // 2^(14 - e) for a largest element in [2^e, 2^(e + 1)), as far as fp32 goes
         const int f = min(268 - (int)(mx >> 7), 254);
         const float up = __uint_as_float((uint32_t)f << 23);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float2 y = unpack_bf16(qf[w][r]);
-            qf[w][r] = pack_f16(y.x * up, y.y * up);
+            const float f16 = r & 1 ? 0.0625f * up : up;  // registers 1 and 3 meet the codes that weigh 16
+            qf[w][r] = pack_f16(y.x * f16, y.y * f16);
+            sum[w] += (y.x + y.y) * up;
           }
-        const float down = fabsf(a.scale) * kLog2e * (f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23));
+        const float down = fabsf(a.scale) * (0x1p24f * kLog2e) * (f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23));
         sl0 = __shfl_sync(0xffffffffu, down, 8 * c);
         sl1 = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 1);
+          sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 2);
+          corr[w][0] = -0x1p-21f * __shfl_sync(0xffffffffu, sum[w], 8 * c);
+          corr[w][1] = -0x1p-21f * __shfl_sync(0xffffffffu, sum[w], 8 * c + 4);
+        }
       }
       float o[8][4];
 #pragma unroll
@@ -408,24 +451,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       int ev = 4;  // biased exponent of the largest V scale so far (at least 4): O is kept times 2^(131 - ev)
 
       for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += T) {
-        // the next tile's block id, in flight during Q.K
-        if (lhas) {
-          lt += T;
-          lti += T;
-          if (lt >= ls.t1) {
-            do {
-              lhas = kv4_next(a, sm, ls, uend, tsh);
-              lt = ls.t0 + wt;
-            } while (lhas && lt >= ls.t1);
-            lbi = lt / a.tpb;
-            lti = lt - lbi * a.tpb;
-            if (lhas) lid = a.bt[ls.row * a.max_blocks + lbi];
-          } else if (lti >= a.tpb) {
-            const int d = lti / a.tpb;
-            lbi += d;
-            lti -= d * a.tpb;
-            lid = a.bt[ls.row * a.max_blocks + lbi];
-          }
+        if (lhas && ++li == ln) {  // the next block ids are in flight during Q.K
+          list_tiles();
+          lhas = ln > 0;
         }
         if (!warp_wait(&sm.kfull[warp], ph, a.err, abort)) {
           dead = true;
@@ -450,11 +478,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
             auto group = [&](auto W, uint32_t x, uint32_t y) {
               constexpr int w = decltype(W)::value;
               float acc[4];
-              const uint32_t a0[4] = {code<false>(x), code<false>(y), code<true>(x), code<true>(y)};
-              mma_f16_16816_first(acc, a0, qf[w][0], qf[w][1]);
+              const uint32_t a0[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
+              mma_f16_16816_from(acc, a0, qf[w][0], qf[w][1], corr[w]);
               x >>= 8;
               y >>= 8;
-              const uint32_t a1[4] = {code<false>(x), code<false>(y), code<true>(x), code<true>(y)};
+              const uint32_t a1[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
               mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
               const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
               s[sb][0] = w == 0 ? acc[0] * fx : fmaf(acc[0], fx, s[sb][0]);

@@ -73,18 +73,21 @@ def pool_from_rows(x: torch.Tensor, block_size: int, value: bool) -> torch.Tenso
 
 
 def attend(q, k, v, scale: float):
-    """q [Hq, 128], k/v float64 [n, Hkv, 128] -> (out, sum p|v|, logit reach) in float64.
+    """q [Hq, 128], k/v float64 [n, Hkv, 128] -> (out, sum p|v|, logit reach, sum p s) in float64.
 
-    The third is scale * max_t sum_groups s_g * sum|q_g| up to the factor
-    between |x| and s: an upper bound of what a logit is summed from."""
+    The third is scale * max_t sum_groups s_g * sum|q_g|, what a logit is summed from per unit of code; the
+    fourth has the V scale s of each dim's group.  s is taken as max|x| / 7: a group's largest code is 7."""
     G = q.shape[0] // k.shape[1]
     kk, vv = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
     x = torch.einsum("hd,nhd->hn", q.double(), kk) * scale
     p = torch.softmax(x, -1)
-    smax = kk.abs().reshape(kk.shape[0], kk.shape[1], 4, 32).amax(-1) / 7  # >= s * max code / 7
+
+    def group_scale(y):
+        return y.abs().reshape(y.shape[0], y.shape[1], 4, 32).amax(-1) / 7
     qa = q.double().abs().reshape(-1, 4, 32).sum(-1)
-    reach = abs(scale) * (smax * qa).sum(-1).amax(0)
-    return torch.einsum("hn,nhd->hd", p, vv), torch.einsum("hn,nhd->hd", p, vv.abs()), reach
+    reach = abs(scale) * (group_scale(kk) * qa).sum(-1).amax(0)
+    ps = torch.einsum("hn,nhg->hg", p, group_scale(vv)).repeat_interleave(32, -1)
+    return torch.einsum("hn,nhd->hd", p, vv), torch.einsum("hn,nhd->hd", p, vv.abs()), reach, ps
 
 
 def block_tables(lengths, block_size, max_blocks, free):

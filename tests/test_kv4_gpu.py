@@ -274,11 +274,15 @@ def call(c, cuda, *, rows=None, seqlens=None, ctx_add=1, scale=SCALE, max_contex
 def check(out, c, scale=SCALE, ctx=None):
     """Every output within its derived bound of the 64-bit result.
 
-    Rounding: the output once (2^-8 relative), and each probability times its V scale once to bf16 (2^-8
-    relative on every term, so 2^-8 sum p|v|).  A logit is summed in fp32 from codes offset by at most 31
-    (|code + offset| + offset <= 39), in at most 2^5 steps of 2^-23 relative to what it is summed from:
-    |error| <= 39 * 2^-18 * scale * sum s|q|, and exp turns that into a relative error of p, above and below
-    the fraction line; 2^-17 covers exp2 and the fp32 sums of up to 2^12 weighted terms of one lane."""
+    Rounding: the output once to bf16 (2^-8 relative); each probability once and its product with the V scale
+    once to fp16 (2^-11 relative each, so 2^-10 sum p|v|).
+    Scores: fp32 sums of q (u - 8), from terms of at most (15 + 8)|q| a code, in at most 2^5 steps that round
+    (or cut) to 2^-23 of the terms: |error| <= 23 * 2^-18 * scale * sum s|q|; exp makes it a relative error
+    of p, above and below the fraction line.  2^-17 covers exp2 and the fp32 sums of a lane's weights.
+    P V: fp32 sums of p s (u - 8) from terms of at most 23 p s a code.  Each of the two products for 16 tokens
+    rounds (or cuts) to 2^-22 of its terms and of what it adds to, which is sum p |v| and 8 p s of those
+    tokens: in all 2^-22 * 2 * 23 * sum p s, and 2^-22 * 2 * (tokens / 16 in one warp's run, below 2^8 here) *
+    sum p|v|."""
     k_all, v_all = O.pool_rows(c["kp"], False), O.pool_rows(c["vp"], True)
     out = out.cpu().double()
     for b, n in enumerate(c["ctx"] if ctx is None else ctx):
@@ -287,9 +291,10 @@ def check(out, c, scale=SCALE, ctx=None):
             continue
         pos = torch.arange(n)
         slot = c["bt"][b].long()[pos // c["bs"]] * c["bs"] + pos % c["bs"]
-        ref, mag, reach = O.attend(c["q"][b], k_all[slot], v_all[slot], scale)
-        rel = torch.expm1(2 * 39 * 2.0 ** -18 * reach)[:, None] + 2.0 ** -17
-        tol = 2.0 ** -8 * (ref.abs() + mag) * (1 + 2.0 ** -8) + rel * (mag + ref.abs())
+        ref, mag, reach, ps = O.attend(c["q"][b], k_all[slot], v_all[slot], scale)
+        rel = torch.expm1(2 * 23 * 2.0 ** -18 * reach)[:, None] + 2.0 ** -17
+        tol = (2.0 ** -8 * ref.abs() + 2.0 ** -10 * mag) * (1 + 2.0 ** -7) + rel * (mag + ref.abs())
+        tol += 2.0 ** -22 * 46 * ps + 2.0 ** -13 * mag
         bad = (out[b] - ref).abs() > tol
         assert not bad.any(), f"row {b} ctx {n}: {((out[b] - ref).abs() / tol).max().item():.2f} of the bound"
 
