@@ -9,10 +9,10 @@
 // Work: the kernel is persistent, one CTA of 16 warps per SM, grouped into
 // teams of T = 1, 2, 4, 8 or 16 warps.  An item is one (row, kv head), a unit
 // a round of T tiles of 64 tokens of an item, one for each warp of a team.
-// Every CTA counts the batch's units itself from seqlens and takes the T
-// that leaves the longest run shortest (the largest such T: fewer partials);
-// the units are cut into equal runs, one per team, whatever the rows' lengths
-// are.  A run that ends inside an item leaves an fp32 partial (max, sum, O);
+// Every CTA counts the batch's units itself from seqlens and takes the T of
+// the least estimated time (large T: few partials to merge; small T: no round
+// that is not full, no waiting); the units are cut into equal runs, one per
+// team, whatever the rows' lengths are.  A run that ends inside an item leaves an fp32 partial (max, sum, O);
 // the last team of the item to arrive merges the partials in order.
 //
 // Tiles: each warp streams its own tiles through one K and one V buffer with
@@ -68,7 +68,8 @@ struct Kv4Smem {
   uint32_t pre[kAttThreads];  // units before thread i's rows, per kv head
   int row[kAttThreads];       // of batches up to kAttThreads rows
   int ctx[kAttThreads];
-  uint32_t wsum[5][kAttWarps];
+  uint32_t wsum[6][kAttWarps];
+  uint32_t sum[6];
   uint64_t kfull[kAttWarps];
   uint64_t vfull[kAttWarps];
   Kv4Seg ahead[kAttWarps];  // where each warp's loads are: segment, and
@@ -255,16 +256,18 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   if (lane == 0) {
     mbar_init(&sm.kfull[warp], 1);
     mbar_init(&sm.vfull[warp], 1);
-    if (warp == 0) sm.abort = 0;
     fence_mbar_init();
   }
+  if (threadIdx.x < 6) sm.sum[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sm.abort = 0;
+  __syncthreads();
   griddep_wait();
   griddep_launch();
 
   // ---- count the batch's units for every team size: each thread sums a run of rows, then the CTA
   const int per = (a.batch + kAttThreads - 1) / kAttThreads;
   const int b_lo = min(a.batch, (int)threadIdx.x * per), b_hi = min(a.batch, b_lo + per);
-  uint32_t cnt[5] = {0, 0, 0, 0, 0};
+  uint32_t cnt[6] = {0, 0, 0, 0, 0, 0};  // [5]: rows with tokens
   for (int b = b_lo; b < b_hi; ++b) {
     int row;
     const int ctx = kv4_ctx(a, b, &row, blockIdx.x == 0 ? a.err : nullptr);
@@ -274,28 +277,40 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     }
 #pragma unroll
     for (int i = 0; i < 5; ++i) cnt[i] += (uint32_t)(tiles_of(ctx) + (1 << i) - 1) >> i;
+    cnt[5] += ctx > 0;
   }
+  {
+    uint32_t x = 0;  // lane i < 6: counter i over the warp
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const uint32_t x = __reduce_add_sync(0xffffffffu, cnt[i]);
-    if (lane == 0) sm.wsum[i][warp] = x;
-  }
-  __syncthreads();
-  int tsh = 0;
-  uint32_t N = 0, chunk = 0xffffffffu, before = 0;
-#pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const uint32_t mine = lane < kAttWarps ? sm.wsum[i][lane] : 0;
-    const uint32_t n = __reduce_add_sync(0xffffffffu, mine) * a.Hkv;
-    const uint32_t teams = gridDim.x * (kAttWarps >> i);
-    const uint32_t ch = (n + teams - 1) / teams;
-    if (ch <= chunk) {
-      tsh = i;
-      N = n;
-      chunk = ch;
-      before = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    for (int i = 0; i < 6; ++i) {
+      const uint32_t y = __reduce_add_sync(0xffffffffu, cnt[i]);
+      x = lane == i ? y : x;
+    }
+    if (lane < 6) {
+      sm.wsum[lane][warp] = x;
+      if (x) atomicAdd(&sm.sum[lane], x);
     }
   }
+  __syncthreads();
+  // Lane i weighs T = 2^i, in microseconds of a model fitted to runs of 17 shapes with each T (B200; within 2 %
+  // of the best T on average): a round of tiles takes 0.26 us per warp at work on the SM, but 2.5 us at least;
+  // a partial costs 0.1 us for each of the G / T heads that a warp merges; the end of a segment 0.2 us for each.
+  const int opt = min(lane, 4);
+  const uint32_t n_opt = sm.sum[opt] * a.Hkv, teams = gridDim.x * (kAttWarps >> opt);
+  const uint32_t c_opt = max((n_opt + teams - 1) / teams, 1u);
+  uint32_t key;
+  {
+    const float t = (float)(1 << opt), ch = (float)c_opt;
+    const float per_item = __fdividef((float)n_opt, (float)max(sm.sum[5] * a.Hkv, 1u));
+    const float busy = t * ceilf(__fdividef(ceilf(__fdividef((float)n_opt, ch)), (float)gridDim.x));
+    float cost = ch * fmaxf(2.5f, 0.26f * busy) +
+                 0.2f * (1.f + __fdividef(ch, fmaxf(per_item, 1.f))) * fmaxf(1.f, __fdividef(G, t));
+    if (per_item > 1.f) cost += 0.1f * G * __fdividef(per_item, ch * t);
+    key = (__float_as_uint(cost) & ~7u) | opt;
+  }
+  const int tsh = (int)(__reduce_min_sync(0xffffffffu, key) & 7u);
+  const uint32_t N = __shfl_sync(0xffffffffu, n_opt, tsh), chunk = __shfl_sync(0xffffffffu, c_opt, tsh);
+  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.wsum[tsh][lane & 15] : 0);
   uint32_t mine = cnt[0];
 #pragma unroll
   for (int i = 1; i < 5; ++i) mine = tsh == i ? cnt[i] : mine;
