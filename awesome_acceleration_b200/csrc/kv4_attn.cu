@@ -49,7 +49,9 @@
 
 namespace aacc {
 
-constexpr int kAttWarps = 16;
+constexpr int kAttWarps = 8;
+constexpr int kSizes = 4;   // team sizes: 1, 2, 4, 8 warps
+constexpr int kStages = 2;  // tiles of K and V that a warp has in hand or in flight
 constexpr int kAttThreads = kAttWarps * 32;
 
 // A run of tiles [t0, t1) of item (b, h), whose row has n tiles; u is the unit number of t0.
@@ -60,21 +62,22 @@ struct Kv4Seg {
 
 template <int G>
 struct Kv4Smem {
-  uint8_t k[kAttWarps][kKv4Record];
-  uint8_t v[kAttWarps][kKv4Record];
+  uint8_t kv[kAttWarps][kStages][2][kKv4Record];
   uint4 vpair[kAttWarps][32];  // V scales of tokens 2 i and 2 i + 1, fp16 pairs of groups 0..3
   float red_o[kAttWarps][G][128];
   float red_ml[kAttWarps][G][2];
-  uint32_t pre[kAttThreads];  // units before thread i's rows, per kv head
+  int first_b[kAttWarps];       // per team: the first row of the thread that holds its first unit,
+  uint32_t first_u[kAttWarps];  // and the unit that row starts at
   int row[kAttThreads];       // of batches up to kAttThreads rows
   int ctx[kAttThreads];
-  uint32_t wsum[6][kAttWarps];
-  uint32_t sum[6];
-  uint64_t kfull[kAttWarps];
-  uint64_t vfull[kAttWarps];
+  uint32_t wsum[kSizes + 1][kAttWarps];
+  uint32_t sum[kSizes + 1];
+  uint32_t plan[3];  // log2 T, units, units per run
+  uint64_t full[kAttWarps][kStages];
   Kv4Seg ahead[kAttWarps];  // where each warp's loads are: segment, and
   int ahead_t[kAttWarps];          // its next tile there that is not in the warp's list
-  int last[kAttWarps];
+  uint32_t merge_k[kAttWarps][2];  // per team and shared item: first run, and
+  int merge_n[kAttWarps][2];       // the number of runs if this one came last, else 0
   int abort;
 };
 
@@ -226,26 +229,107 @@ __device__ __forceinline__ void team_sync(int team, int tsh) {
     asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(32 << tsh) : "memory");
 }
 
-// Running (max, sum, O) of partial results that are weighted 2^max.
-struct Kv4Acc {
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  __device__ __forceinline__ void add(float pm, float pl, float4 po) {
-    const float n = fmaxf(m, pm);
-    const float u = n == -INFINITY ? 0.f : n;
-    const float f = ex2(m - u), g = ex2(pm - u);
-    m = n;
-    l = l * f + pl * g;
-    o.x = o.x * f + po.x * g;
-    o.y = o.y * f + po.y * g;
-    o.z = o.z * f + po.z * g;
-    o.w = o.w * f + po.w * g;
+// How a warp shares out sums of partial results: VW dims a lane, 4 or 1 at a time, so GS lanes to a head.
+// Several heads to a warp (VW 8, 16) have their loads in flight together; with VW 1 a warp takes 32 dims.
+template <int VW>
+struct Kv4Share {
+  static constexpr int GS = VW == 1 ? 32 : 128 / VW;
+  static constexpr int P = VW == 1 ? 1 : VW / 4;  // pieces
+  int hd, d;                                      // head; the first piece's first dim
+  __device__ __forceinline__ Kv4Share(int i, int lane) {
+    if constexpr (VW == 1) {
+      hd = i >> 2;
+      d = (i & 3) * 32 + lane;
+    } else {
+      hd = i * (32 / GS) + lane / GS;
+      d = lane % GS * 4;
+    }
   }
-  __device__ __forceinline__ uint2 result() const {
+  template <class Load>
+  __device__ __forceinline__ void read(const float* head, float (&y)[VW], Load load) const {
+    if constexpr (VW == 1) {
+      y[0] = load(head + d);
+    } else {
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const float4 v = load(reinterpret_cast<const float4*>(head + d + q * GS * 4));
+        y[4 * q] = v.x, y[4 * q + 1] = v.y, y[4 * q + 2] = v.z, y[4 * q + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void write(float* head, const float (&y)[VW]) const {
+    if constexpr (VW == 1) {
+      head[d] = y[0];
+    } else {
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+        *reinterpret_cast<float4*>(head + d + q * GS * 4) =
+            make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+    }
+  }
+  __device__ __forceinline__ void write(bf16* head, const float (&y)[VW], float l) const {
     const float inv = 1.f / l;
-    return make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    if constexpr (VW == 1) {
+      head[d] = tobf(y[0] * inv);
+    } else {
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+        *reinterpret_cast<uint2*>(head + d + q * GS * 4) =
+            make_uint2(pack_bf16(y[4 * q] * inv, y[4 * q + 1] * inv), pack_bf16(y[4 * q + 2] * inv, y[4 * q + 3] * inv));
+    }
   }
 };
+
+// Sum of `count` partial results (max, sum, O) of this lane's head, weighted 2^max: ml(p) gives (max, sum),
+// o(p, y) this lane's dims.  Each of the head's lanes weighs one part, so all loads are independent.
+template <int VW, class ML, class OF>
+__device__ __forceinline__ void kv4_combine(int count, int lane, ML ml, OF o, float& M, float& L, float (&O)[VW]) {
+  constexpr int GS = Kv4Share<VW>::GS;
+  const int gl = lane % GS, g0 = lane - gl;
+  M = -INFINITY;
+  L = 0.f;
+#pragma unroll
+  for (int i = 0; i < VW; ++i) O[i] = 0.f;
+  for (int p0 = 0; p0 < count; p0 += GS) {
+    const int n = min(GS, count - p0);
+    float2 x = make_float2(-INFINITY, 0.f);
+    if (gl < n) x = ml(p0 + gl);
+    float top = x.x;
+#pragma unroll
+    for (int d = 1; d < GS; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    top = fmaxf(M, top);
+    const float u = top == -INFINITY ? 0.f : top;
+    const float f = ex2(x.x - u), keep = ex2(M - u);
+    M = top;
+    float l = x.y * f;
+#pragma unroll
+    for (int d = 1; d < GS; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    L = L * keep + l;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) O[i] *= keep;
+#pragma unroll(VW == 1 ? 16 : 32 / VW)
+    for (int p = 0; p < n; ++p) {
+      const float w = __shfl_sync(0xffffffffu, f, g0 + p);
+      float y[VW];
+      o(p0 + p, y);
+#pragma unroll
+      for (int i = 0; i < VW; ++i) O[i] = fmaf(w, y[i], O[i]);
+    }
+  }
+}
+
+// f(VW) for a team of T warps and G heads.
+template <int G, class F>
+__device__ __forceinline__ void kv4_share(int T, F f) {
+  if (T > G)
+    f(std::integral_constant<int, 1>{});
+  else if (T == G || G == 1)
+    f(std::integral_constant<int, 4>{});
+  else if (2 * T == G || G == 2)
+    f(std::integral_constant<int, G >= 2 ? 8 : 4>{});
+  else
+    f(std::integral_constant<int, G >= 4 ? 16 : 4>{});
+}
 
 template <int G>
 __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Args a) {
@@ -254,11 +338,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   if (lane == 0) {
-    mbar_init(&sm.kfull[warp], 1);
-    mbar_init(&sm.vfull[warp], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&sm.full[warp][i], 1);
     fence_mbar_init();
   }
-  if (threadIdx.x < 6) sm.sum[threadIdx.x] = 0;
+  if (threadIdx.x <= kSizes) sm.sum[threadIdx.x] = 0;
   if (threadIdx.x == 0) sm.abort = 0;
   __syncthreads();
   griddep_wait();
@@ -267,7 +350,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   // ---- count the batch's units for every team size: each thread sums a run of rows, then the CTA
   const int per = (a.batch + kAttThreads - 1) / kAttThreads;
   const int b_lo = min(a.batch, (int)threadIdx.x * per), b_hi = min(a.batch, b_lo + per);
-  uint32_t cnt[6] = {0, 0, 0, 0, 0, 0};  // [5]: rows with tokens
+  uint32_t cnt[kSizes + 1] = {};  // [kSizes]: rows with tokens
   for (int b = b_lo; b < b_hi; ++b) {
     int row;
     const int ctx = kv4_ctx(a, b, &row, blockIdx.x == 0 ? a.err : nullptr);
@@ -276,17 +359,17 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       sm.row[b] = row;
     }
 #pragma unroll
-    for (int i = 0; i < 5; ++i) cnt[i] += (uint32_t)(tiles_of(ctx) + (1 << i) - 1) >> i;
-    cnt[5] += ctx > 0;
+    for (int i = 0; i < kSizes; ++i) cnt[i] += (uint32_t)(tiles_of(ctx) + (1 << i) - 1) >> i;
+    cnt[kSizes] += ctx > 0;
   }
-  {
-    uint32_t x = 0;  // lane i < 6: counter i over the warp
+  if (warp * 32 * per < a.batch) {
+    uint32_t x = 0;  // lane i: counter i over the warp
 #pragma unroll
-    for (int i = 0; i < 6; ++i) {
+    for (int i = 0; i <= kSizes; ++i) {
       const uint32_t y = __reduce_add_sync(0xffffffffu, cnt[i]);
       x = lane == i ? y : x;
     }
-    if (lane < 6) {
+    if (lane <= kSizes) {
       sm.wsum[lane][warp] = x;
       if (x) atomicAdd(&sm.sum[lane], x);
     }
@@ -294,54 +377,63 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   __syncthreads();
   // Lane i weighs T = 2^i, in microseconds of a model fitted to runs of 17 shapes with each T (B200; within 2 %
   // of the best T on average): a round of tiles takes 0.26 us per warp at work on the SM, but 2.5 us at least;
-  // a partial costs 0.1 us for each of the G / T heads that a warp merges; the end of a segment 0.2 us for each.
-  const int opt = min(lane, 4);
-  const uint32_t n_opt = sm.sum[opt] * a.Hkv, teams = gridDim.x * (kAttWarps >> opt);
-  const uint32_t c_opt = max((n_opt + teams - 1) / teams, 1u);
-  uint32_t key;
-  {
-    const float t = (float)(1 << opt), ch = (float)c_opt;
-    const float per_item = __fdividef((float)n_opt, (float)max(sm.sum[5] * a.Hkv, 1u));
-    const float busy = t * ceilf(__fdividef(ceilf(__fdividef((float)n_opt, ch)), (float)gridDim.x));
+  // merging costs 1 us, and 0.1 us for each of the G / T heads of a partial that a warp merges; the end of a
+  // segment 0.2 us for each.
+  if (warp == 0) {
+    const int opt = min(lane, kSizes - 1);
+    const uint32_t n = sm.sum[opt] * a.Hkv, teams = gridDim.x * (kAttWarps >> opt);
+    const uint32_t c = max((n + teams - 1) / teams, 1u);
+    const float t = (float)(1 << opt), ch = (float)c;
+    const float per_item = __fdividef((float)n, (float)max(sm.sum[kSizes] * a.Hkv, 1u));
+    const float busy = t * ceilf(__fdividef(ceilf(__fdividef((float)n, ch)), (float)gridDim.x));
     float cost = ch * fmaxf(2.5f, 0.26f * busy) +
                  0.2f * (1.f + __fdividef(ch, fmaxf(per_item, 1.f))) * fmaxf(1.f, __fdividef(G, t));
-    if (per_item > 1.f) cost += 0.1f * G * __fdividef(per_item, ch * t);
-    key = (__float_as_uint(cost) & ~7u) | opt;
+    if (per_item > ch) cost += 1.f + 0.1f * G * __fdividef(per_item, ch * t);
+    const uint32_t best = __reduce_min_sync(0xffffffffu, (__float_as_uint(cost) & ~7u) | opt) & 7u;
+    if (lane == best) {
+      sm.plan[0] = best;
+      sm.plan[1] = n;
+      sm.plan[2] = c;
+    }
   }
-  const int tsh = (int)(__reduce_min_sync(0xffffffffu, key) & 7u);
-  const uint32_t N = __shfl_sync(0xffffffffu, n_opt, tsh), chunk = __shfl_sync(0xffffffffu, c_opt, tsh);
-  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.wsum[tsh][lane & 15] : 0);
-  uint32_t mine = cnt[0];
+  __syncthreads();
+  const int tsh = (int)sm.plan[0];
+  const uint32_t N = sm.plan[1], chunk = sm.plan[2];
+  if (warp * 32 * per < a.batch) {
+    uint32_t mine = cnt[0];
 #pragma unroll
-  for (int i = 1; i < 5; ++i) mine = tsh == i ? cnt[i] : mine;
-  uint32_t inc = mine;
+    for (int i = 1; i < kSizes; ++i) mine = tsh == i ? cnt[i] : mine;
+    uint32_t inc = mine;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += y;
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += y;
+    }
+    // The thread whose rows hold a team's first unit tells it where they start.
+    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.wsum[tsh][lane % kAttWarps] : 0);  // of warps with rows
+    const uint32_t s0 = (before + inc - mine) * a.Hkv, s1 = s0 + mine * a.Hkv;
+    if (mine)
+      for (int i = 0; i < kAttWarps >> tsh; ++i) {
+        const uint32_t u = ((uint32_t)i * gridDim.x + blockIdx.x) * chunk;  // at most N + teams
+        if (u >= s0 && u < s1) {
+          sm.first_b[i] = b_lo;
+          sm.first_u[i] = s0;
+        }
+      }
   }
-  sm.pre[threadIdx.x] = before + inc - mine;
   __syncthreads();
 
   // ---- this team's run of units
   const int team = warp >> tsh, wt = warp & ((1 << tsh) - 1), T = 1 << tsh;
   const uint32_t k = (uint32_t)team * gridDim.x + blockIdx.x;  // runs go round the SMs: few runs use many of them
-  const uint32_t u0 = (uint32_t)min((uint64_t)k * chunk, (uint64_t)N), uend = min(u0 + chunk, N);
+  const uint32_t u0 = min(k * chunk, N), uend = min(u0 + chunk, N);
   volatile int* abort = &sm.abort;
 
   if (u0 < uend) {
     Kv4Seg cs;
     {
-      int lo = 0, hi = kAttThreads;  // the last thread whose rows start at or before u0
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (sm.pre[mid] * a.Hkv <= u0)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      uint32_t u = sm.pre[lo] * a.Hkv;
-      cs.b = lo * per;
+      uint32_t u = sm.first_u[team];
+      cs.b = sm.first_b[team];
       kv4_row(a, sm, cs);
       uint32_t rounds = (uint32_t)(cs.n + T - 1) >> tsh;
       while (u + rounds * a.Hkv <= u0) {
@@ -390,28 +482,36 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       }
       return ((int64_t)id * (a.Hkv * a.tpb) + at) * kKv4Record;
     };
-    auto load_k = [&](int64_t rec) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.kfull[warp], kKv4Record);
-        bulk_load(sm.k[warp], a.kc + rec, kKv4Record, &sm.kfull[warp]);
-      }
+    // Queries of a segment: raw, as loaded; head g's dims 32 w + 8 c .. + 7.
+    uint4 xq[4];
+    auto load_q = [&](const Kv4Seg& s) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        xq[w] = g < G ? *reinterpret_cast<const uint4*>(a.q + (((int64_t)s.b * a.Hkv + s.h) * G + g) * 128 + 32 * w + 8 * c)
+                      : make_uint4(0, 0, 0, 0);
     };
-    auto load_v = [&](int64_t rec) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.vfull[warp], kKv4Record);
-        bulk_load(sm.v[warp], a.vc + rec, kKv4Record, &sm.vfull[warp]);
-      }
-    };
+    load_q(cs);
     list_tiles();
-    bool lhas = ln > 0;  // there is a tile to load
-    if (lhas) {
+    uint32_t issued = 0, used = 0;  // tiles; tile i lies in stage i % kStages
+    bool dead = false;              // a copy did not come in time: no more loads, no more tiles
+    auto issue = [&]() {            // the list's next tile, if there is one, into the next stage
+      if (li == ln) return;
       const int64_t rec = record();
-      load_k(rec);
-      load_v(rec);
-    }
-    uint32_t ph = 0;    // parity of the tile in hand, for both buffers
-    bool dead = false;  // a copy did not come in time: no more loads, no more tiles
-    uint32_t kph = 0;   // then: the parity that the K buffer still waits for
+      const uint32_t st = issued++ % kStages;
+      if (lane == 0) {
+        uint64_t* bar = &sm.full[warp][st];
+        mbar_arrive_expect_tx(bar, 2 * kKv4Record);
+        bulk_load(sm.kv[warp][st][0], a.kc + rec, kKv4Record, bar);
+        bulk_load(sm.kv[warp][st][1], a.vc + rec, kKv4Record, bar);
+      }
+      if (++li == ln) list_tiles();  // the next block ids are on their way while a tile is worked on
+    };
+    for (int i = 0; i < kStages; ++i) issue();
+
+    // Items that this run holds a part of, not the whole: first query head, first and last unit.
+    int parts = 0;
+    int64_t part_q[2] = {0, 0};
+    uint32_t part_first[2] = {0, 0}, part_last[2] = {0, 0};
 
     while (true) {
       // ---- queries of the item: B operand, column g = query head (columns >= G are zero)
@@ -424,12 +524,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         uint32_t mx = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (g < G) x = *reinterpret_cast<const uint4*>(a.q + (qh0 + g) * 128 + 32 * w + 8 * c);
-          qf[w][0] = x.x ^ flip;
-          qf[w][1] = x.y ^ flip;
-          qf[w][2] = x.z ^ flip;
-          qf[w][3] = x.w ^ flip;
+          qf[w][0] = xq[w].x ^ flip;
+          qf[w][1] = xq[w].y ^ flip;
+          qf[w][2] = xq[w].z ^ flip;
+          qf[w][3] = xq[w].w ^ flip;
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = max(mx, max(qf[w][r] & 0x7fffu, (qf[w][r] >> 16) & 0x7fffu));
         }
@@ -466,187 +564,174 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       int ev = 4;  // biased exponent of the largest V scale so far (at least 4): O is kept times 2^(131 - ev)
 
       for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += T) {
-        if (lhas && ++li == ln) {  // the next block ids are in flight during Q.K
-          list_tiles();
-          lhas = ln > 0;
-        }
-        if (!warp_wait(&sm.kfull[warp], ph, a.err, abort)) {
+        const uint32_t st = used % kStages;
+        if (!warp_wait(&sm.full[warp][st], used / kStages & 1, a.err, abort)) {
           dead = true;
-          kph = ph;
-          lhas = false;
+          li = ln = 0;
           break;
         }
-        int64_t next_rec = 0;
-        int lim = cs.ctx - t * kKv4Tile;  // tokens from here to the end of the context
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half, lim -= 32) {
-          // ---- S = K Q^T for 32 tokens; lane (g, c): tokens 16 sb + g (+ 8), heads 2c and 2c + 1
-          const uint8_t* kb = sm.k[warp] + half * 2048;
-          const uint8_t* ksc = sm.k[warp] + kKv4Codes + half * 256;
-          float s[2][4];
-#pragma unroll
-          for (int sb = 0; sb < 2; ++sb) {
-            const uint4 x4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + lane * 16);        // token g
-            const uint4 y4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + 512 + lane * 16);  // token g + 8
-            const uint2 sx = *reinterpret_cast<const uint2*>(ksc + (16 * sb + g) * 8);
-            const uint2 sy = *reinterpret_cast<const uint2*>(ksc + (16 * sb + g + 8) * 8);
-            auto group = [&](auto W, uint32_t x, uint32_t y) {
-              constexpr int w = decltype(W)::value;
-              float acc[4];
-              const uint32_t a0[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
-              mma_f16_16816_from(acc, a0, qf[w][0], qf[w][1], corr[w]);
-              x >>= 8;
-              y >>= 8;
-              const uint32_t a1[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
-              mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
-              const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
-              s[sb][0] = w == 0 ? acc[0] * fx : fmaf(acc[0], fx, s[sb][0]);
-              s[sb][1] = w == 0 ? acc[1] * fx : fmaf(acc[1], fx, s[sb][1]);
-              s[sb][2] = w == 0 ? acc[2] * fy : fmaf(acc[2], fy, s[sb][2]);
-              s[sb][3] = w == 0 ? acc[3] * fy : fmaf(acc[3], fy, s[sb][3]);
-            };
-            group(std::integral_constant<int, 0>{}, x4.x, y4.x);
-            group(std::integral_constant<int, 1>{}, x4.y, y4.y);
-            group(std::integral_constant<int, 2>{}, x4.z, y4.z);
-            group(std::integral_constant<int, 3>{}, x4.w, y4.w);
-          }
-          const bool done = half == 1 || lim <= 32;  // no more tokens in this tile
-          if (done) {
-            __syncwarp();  // every lane has read the K buffer
-            if (lhas) {
-              next_rec = record();
-              load_k(next_rec);
-            }
-          }
+        ++used;
+        const uint8_t* kb = sm.kv[warp][st][0];
+        const uint8_t* vb = sm.kv[warp][st][1];
+        const int lim = cs.ctx - t * kKv4Tile;  // tokens from here to the end of the context
 
-          // ---- online softmax in the log2 domain
-          if (lim < 32) {
+        // ---- S = K Q^T; lane (g, c): tokens 16 sb + g (+ 8), heads 2c and 2c + 1
+        float s[4][4];
 #pragma unroll
-            for (int sb = 0; sb < 2; ++sb) {
-              if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = -INFINITY;
-              if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = -INFINITY;
-            }
-          }
-          // The reference of the exponentials follows the maximum only when a score passes it by 2^6: p stays
-          // below 2^6, and most halves need no shuffles and no rescaling.
-          const float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])) * sl0;
-          const float x1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3])) * sl1;
-          float a0 = 1.f, a1 = 1.f;
-          bool grow = __any_sync(0xffffffffu, x0 > m0 + 6.f || x1 > m1 + 6.f);
-          if (grow) {
-            float n0 = x0, n1 = x1;
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) {
-              n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
-              n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
-            }
-            n0 = fmaxf(m0, n0);
-            n1 = fmaxf(m1, n1);
-            a0 = ex2(m0 - n0);
-            a1 = ex2(m1 - n1);
-            m0 = n0;
-            m1 = n1;
-            l0 *= a0;
-            l1 *= a1;
-          }
-          const float r0 = 4.f - m0, r1 = 4.f - m1;  // 2^4 p
-#pragma unroll
-          for (int sb = 0; sb < 2; ++sb) {
-            s[sb][0] = ex2(fmaf(s[sb][0], sl0, r0));
-            s[sb][1] = ex2(fmaf(s[sb][1], sl1, r1));
-            s[sb][2] = ex2(fmaf(s[sb][2], sl0, r0));
-            s[sb][3] = ex2(fmaf(s[sb][3], sl1, r1));
-          }
-          if (lim < 32) {  // also where a scale of 0 makes -inf * 0 a NaN
-#pragma unroll
-            for (int sb = 0; sb < 2; ++sb) {
-              if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = 0.f;
-              if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = 0.f;
-            }
-          }
-          l0 += (s[0][0] + s[0][2]) + (s[1][0] + s[1][2]);
-          l1 += (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
-
-          if (half == 0) {
-            if (!warp_wait(&sm.vfull[warp], ph, a.err, abort)) {
-              dead = true;
-              kph = lhas && done ? ph ^ 1 : ph;
-              lhas = false;
-              break;
-            }
-            // The tile's largest V scale (they are not negative: their bits order as they do); lane: tokens
-            // 2 lane and 2 lane + 1.  Behind the context a scale may be anything: it becomes zero.
-            uint4 x = *(reinterpret_cast<const uint4*>(sm.v[warp] + kKv4Codes) + lane);
-            if (lim < kKv4Tile) {
-              if (2 * lane >= lim) x.x = x.y = 0;
-              if (2 * lane + 1 >= lim) x.z = x.w = 0;
-            }
-            const uint32_t big = max(max(max(x.x, x.y), max(x.z, x.w)),
-                                     max(max(x.x << 16, x.y << 16), max(x.z << 16, x.w << 16)));
-            const int e = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
-            if (e > ev) {
-              const float f = ex2((float)(ev - e));
-              a0 *= f;
-              a1 *= f;
-              ev = e;
-              grow = true;
-            }
-            const float cv = __uint_as_float((uint32_t)(258 - ev) << 23);
-            const uint2 ta = make_uint2(x.x, x.y), tb = make_uint2(x.z, x.w);
-            sm.vpair[warp][lane] = make_uint4(pack_f16(scale_of<0>(ta) * cv, scale_of<0>(tb) * cv),
-                                              pack_f16(scale_of<1>(ta) * cv, scale_of<1>(tb) * cv),
-                                              pack_f16(scale_of<2>(ta) * cv, scale_of<2>(tb) * cv),
-                                              pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
-            __syncwarp();
-          }
-          if (grow) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              o[j][0] *= a0;
-              o[j][1] *= a1;
-              o[j][2] *= a0;
-              o[j][3] *= a1;
-            }
-          }
-
-          // ---- O^T += V^T P^T
-          const uint8_t* vb = sm.v[warp] + half * 2048;
-#pragma unroll
-          for (int sb = 0; sb < 2; ++sb) {
-            const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
-            const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
-            const uint4 sx = sm.vpair[warp][(2 * half + sb) * 8 + c], sy = sm.vpair[warp][(2 * half + sb) * 8 + 4 + c];
-            const uint32_t px = movmatrix_trans(pack_f16(s[sb][0], s[sb][1]));  // head g, tokens 2c, 2c + 1
-            const uint32_t py = movmatrix_trans(pack_f16(s[sb][2], s[sb][3]));  // ... + 8
-            auto group = [&](auto W) {  // 32 dims: j = 2w and 2w + 1
-              constexpr int w = decltype(W)::value;
-              const uint32_t b0 = mul_f16(px, w == 0 ? sx.x : w == 1 ? sx.y : w == 2 ? sx.z : sx.w);
-              const uint32_t b1 = mul_f16(py, w == 0 ? sy.x : w == 1 ? sy.y : w == 2 ? sy.z : sy.w);
-              // 16 bits of tokens 2c | 2c + 1 each: four nibbles = dims 16 j + 2g, + 1 of j = 2w, 2w + 1
-              constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
-              uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
-              uint32_t y = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
-              const uint32_t a0[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
-              mma_f16_16816(o[2 * w], a0, b0, b1);
-              x >>= 8;
-              y >>= 8;
-              const uint32_t a1[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
-              mma_f16_16816(o[2 * w + 1], a1, b0, b1);
-            };
-            group(std::integral_constant<int, 0>{});
-            group(std::integral_constant<int, 1>{});
-            group(std::integral_constant<int, 2>{});
-            group(std::integral_constant<int, 3>{});
-          }
-          if (done) break;
+        for (int sb = 0; sb < 4; ++sb) {
+          const uint4 x4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + lane * 16);        // token g
+          const uint4 y4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + 512 + lane * 16);  // token g + 8
+          const uint2 sx = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + g) * 8);
+          const uint2 sy = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + g + 8) * 8);
+          auto group = [&](auto W, uint32_t x, uint32_t y) {
+            constexpr int w = decltype(W)::value;
+            float acc[4];
+            const uint32_t a0[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
+            mma_f16_16816_from(acc, a0, qf[w][0], qf[w][1], corr[w]);
+            x >>= 8;
+            y >>= 8;
+            const uint32_t a1[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
+            mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
+            const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
+            s[sb][0] = w == 0 ? acc[0] * fx : fmaf(acc[0], fx, s[sb][0]);
+            s[sb][1] = w == 0 ? acc[1] * fx : fmaf(acc[1], fx, s[sb][1]);
+            s[sb][2] = w == 0 ? acc[2] * fy : fmaf(acc[2], fy, s[sb][2]);
+            s[sb][3] = w == 0 ? acc[3] * fy : fmaf(acc[3], fy, s[sb][3]);
+          };
+          group(std::integral_constant<int, 0>{}, x4.x, y4.x);
+          group(std::integral_constant<int, 1>{}, x4.y, y4.y);
+          group(std::integral_constant<int, 2>{}, x4.z, y4.z);
+          group(std::integral_constant<int, 3>{}, x4.w, y4.w);
         }
-        if (dead) break;
-        ph ^= 1;
-        __syncwarp();  // every lane has read the V buffer
-        if (lhas) load_v(next_rec);
+
+        // ---- the tile's V scales as fp16 pairs; lane: tokens 2 lane and 2 lane + 1.  Behind the context a scale
+        // may be anything: it becomes zero.  They are not negative: their bits order as they do.
+        float a0 = 1.f, a1 = 1.f;
+        bool grow = false;
+        {
+          uint4 x = *(reinterpret_cast<const uint4*>(vb + kKv4Codes) + lane);
+          if (lim < kKv4Tile) {
+            if (2 * lane >= lim) x.x = x.y = 0;
+            if (2 * lane + 1 >= lim) x.z = x.w = 0;
+          }
+          const uint32_t big = max(max(max(x.x, x.y), max(x.z, x.w)),
+                                   max(max(x.x << 16, x.y << 16), max(x.z << 16, x.w << 16)));
+          const int e = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
+          if (e > ev) {
+            a0 = a1 = ex2((float)(ev - e));
+            ev = e;
+            grow = true;
+          }
+          const float cv = __uint_as_float((uint32_t)(258 - ev) << 23);
+          const uint2 ta = make_uint2(x.x, x.y), tb = make_uint2(x.z, x.w);
+          sm.vpair[warp][lane] = make_uint4(pack_f16(scale_of<0>(ta) * cv, scale_of<0>(tb) * cv),
+                                            pack_f16(scale_of<1>(ta) * cv, scale_of<1>(tb) * cv),
+                                            pack_f16(scale_of<2>(ta) * cv, scale_of<2>(tb) * cv),
+                                            pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
+        }
+
+        // ---- online softmax in the log2 domain
+        if (lim < kKv4Tile) {
+#pragma unroll
+          for (int sb = 0; sb < 4; ++sb) {
+            if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = -INFINITY;
+            if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = -INFINITY;
+          }
+        }
+        // The reference of the exponentials follows the maximum only when a score passes it by 2^6: p stays
+        // below 2^6, and most tiles need no shuffles and no rescaling.
+        float x0 = fmaxf(s[0][0], s[0][2]), x1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+        for (int sb = 1; sb < 4; ++sb) {
+          x0 = fmaxf(x0, fmaxf(s[sb][0], s[sb][2]));
+          x1 = fmaxf(x1, fmaxf(s[sb][1], s[sb][3]));
+        }
+        x0 *= sl0;
+        x1 *= sl1;
+        if (__any_sync(0xffffffffu, x0 > m0 + 6.f || x1 > m1 + 6.f)) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+          }
+          x0 = fmaxf(m0, x0);
+          x1 = fmaxf(m1, x1);
+          const float f0 = ex2(m0 - x0), f1 = ex2(m1 - x1);
+          m0 = x0;
+          m1 = x1;
+          l0 *= f0;
+          l1 *= f1;
+          a0 *= f0;
+          a1 *= f1;
+          grow = true;
+        }
+        const float r0 = 4.f - m0, r1 = 4.f - m1;  // 2^4 p
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb) {
+          s[sb][0] = ex2(fmaf(s[sb][0], sl0, r0));
+          s[sb][1] = ex2(fmaf(s[sb][1], sl1, r1));
+          s[sb][2] = ex2(fmaf(s[sb][2], sl0, r0));
+          s[sb][3] = ex2(fmaf(s[sb][3], sl1, r1));
+        }
+        if (lim < kKv4Tile) {  // also where a scale of 0 makes -inf * 0 a NaN
+#pragma unroll
+          for (int sb = 0; sb < 4; ++sb) {
+            if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = 0.f;
+            if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb) {
+          l0 += s[sb][0] + s[sb][2];
+          l1 += s[sb][1] + s[sb][3];
+        }
+        if (grow) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            o[j][0] *= a0;
+            o[j][1] *= a1;
+            o[j][2] *= a0;
+            o[j][3] *= a1;
+          }
+        }
+        __syncwarp();  // vpair is written
+
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int sb = 0; sb < 4; ++sb) {
+          const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
+          const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
+          const uint4 sx = sm.vpair[warp][sb * 8 + c], sy = sm.vpair[warp][sb * 8 + 4 + c];
+          const uint32_t px = movmatrix_trans(pack_f16(s[sb][0], s[sb][1]));  // head g, tokens 2c, 2c + 1
+          const uint32_t py = movmatrix_trans(pack_f16(s[sb][2], s[sb][3]));  // ... + 8
+          auto group = [&](auto W) {  // 32 dims: j = 2w and 2w + 1
+            constexpr int w = decltype(W)::value;
+            const uint32_t b0 = mul_f16(px, w == 0 ? sx.x : w == 1 ? sx.y : w == 2 ? sx.z : sx.w);
+            const uint32_t b1 = mul_f16(py, w == 0 ? sy.x : w == 1 ? sy.y : w == 2 ? sy.z : sy.w);
+            // 16 bits of tokens 2c | 2c + 1 each: four nibbles = dims 16 j + 2g, + 1 of j = 2w, 2w + 1
+            constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
+            uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
+            uint32_t y = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
+            const uint32_t a0[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
+            mma_f16_16816(o[2 * w], a0, b0, b1);
+            x >>= 8;
+            y >>= 8;
+            const uint32_t a1[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
+            mma_f16_16816(o[2 * w + 1], a1, b0, b1);
+          };
+          group(std::integral_constant<int, 0>{});
+          group(std::integral_constant<int, 1>{});
+          group(std::integral_constant<int, 2>{});
+          group(std::integral_constant<int, 3>{});
+        }
+        __syncwarp();  // every lane has read the stage
+        issue();
       }
 
       // ---- end of the segment: the team's warps meet in shared memory
+      Kv4Seg nx = cs;
+      const bool more = kv4_next(a, sm, nx, uend, tsh);
+      if (more) load_q(nx);
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
@@ -667,67 +752,76 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       team_sync(team, tsh);
       const bool whole = cs.t0 == 0 && cs.t1 == cs.n;
       const uint32_t slot = 2 * k + (cs.t0 == 0);
-      for (int hd = wt; hd < G; hd += T) {
-        Kv4Acc acc;
-        for (int w = team << tsh; w < (team + 1) << tsh; ++w)
-          acc.add(sm.red_ml[w][hd][0], sm.red_ml[w][hd][1], reinterpret_cast<const float4*>(sm.red_o[w][hd])[lane]);
-        if (whole) {
-          reinterpret_cast<uint2*>(a.out + (qh0 + hd) * 128)[lane] = acc.result();
-        } else {
-          reinterpret_cast<float4*>(a.ws_o)[((int64_t)slot * G + hd) * 32 + lane] = acc.o;
-          if (lane == 0) reinterpret_cast<float2*>(a.ws_ml)[(int64_t)slot * G + hd] = make_float2(acc.m, acc.l);
+      kv4_share<G>(T, [&](auto V) {
+        constexpr int VW = decltype(V)::value;
+        for (int i = wt; i < G * 4 / VW; i += T) {
+          const Kv4Share<VW> sh(i, lane);
+          float M, L, O[VW];
+          kv4_combine<VW>(
+              T, lane, [&](int w) { return *reinterpret_cast<const float2*>(sm.red_ml[(team << tsh) + w][sh.hd]); },
+              [&](int w, float(&y)[VW]) {
+                sh.read(sm.red_o[(team << tsh) + w][sh.hd], y, [](auto* p) { return *p; });
+              },
+              M, L, O);
+          if (whole) {
+            sh.write(a.out + (qh0 + sh.hd) * 128, O, L);
+          } else {
+            const int64_t at = (int64_t)slot * G + sh.hd;
+            sh.write(a.ws_o + at * 128, O);
+            if (sh.d == 0) reinterpret_cast<float2*>(a.ws_ml)[at] = make_float2(M, L);
+          }
         }
-      }
-      if (!whole) {
-        // The item's first unit lies in run k0, its last in run k0 + parts - 1; the last of them to get
-        // here merges: run k0's tail (slot 2 k0 + 1), then the heads of the others (2 k), in this order
-        // within each of `sl` slices that the team's warps share out.
+      });
+      if (!whole) {  // at most twice: where the run begins and where it ends
         const uint32_t first = cs.u - (cs.t0 >> tsh);
-        const uint32_t k0 = first / chunk;
-        const int parts = (int)((first + ((uint32_t)(cs.n + T - 1) >> tsh) - 1) / chunk - k0) + 1;
-        __threadfence();
-        team_sync(team, tsh);
-        if (wt == 0 && lane == 0) sm.last[team] = atomicInc(a.cnt + k0, parts - 1) == (unsigned)(parts - 1);
-        team_sync(team, tsh);
-        if (sm.last[team]) {
-          __threadfence();
-          const int sl = max(T / G, 1);  // a power of two, as T and G are
-          for (int hs = wt; hs < G * sl; hs += T) {
-            const int hd = hs % G;
-            Kv4Acc acc;
-#pragma unroll 4
-            for (int p = hs / G; p < parts; p += sl) {
-              const int64_t at = (int64_t)(2 * (k0 + p) + (p == 0)) * G + hd;
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + at);
-              acc.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(a.ws_o) + at * 32 + lane));
-            }
-            if (sl == 1) {
-              reinterpret_cast<uint2*>(a.out + (qh0 + hd) * 128)[lane] = acc.result();
-            } else {
-              reinterpret_cast<float4*>(sm.red_o[warp][0])[lane] = acc.o;
-              if (lane == 0) *reinterpret_cast<float2*>(sm.red_ml[warp][0]) = make_float2(acc.m, acc.l);
-            }
-          }
-          if (sl > 1) {
-            team_sync(team, tsh);
-            if (wt < G) {
-              Kv4Acc acc;
-              for (int i = 0; i < sl; ++i) {
-                const int w = warp + i * G;
-                acc.add(sm.red_ml[w][0][0], sm.red_ml[w][0][1], reinterpret_cast<const float4*>(sm.red_o[w][0])[lane]);
-              }
-              reinterpret_cast<uint2*>(a.out + (qh0 + wt) * 128)[lane] = acc.result();
-            }
-          }
+        const uint32_t end = first + ((uint32_t)(cs.n + T - 1) >> tsh) - 1;
+        if (parts == 0) {  // (no indexing: they stay in registers)
+          part_q[0] = qh0, part_first[0] = first, part_last[0] = end;
+        } else {
+          part_q[1] = qh0, part_first[1] = first, part_last[1] = end;
         }
+        ++parts;
       }
       team_sync(team, tsh);  // the team's shared buffers are read
-      if (!kv4_next(a, sm, cs, uend, tsh)) break;
+      if (!more) break;
+      cs = nx;
     }
-    if (dead) {  // copies in flight land (or run out of time once more) before the CTA ends
-      mbar_wait(&sm.kfull[warp], kph, a.err, nullptr);
-      mbar_wait(&sm.vfull[warp], ph, a.err, nullptr);
+    if (parts) {
+      // Of the runs k0 .. k0 + n - 1 that share an item, the last to get here sums their parts: run k0's tail
+      // (slot 2 k0 + 1), then the heads of the others (slots 2 k), in this order whichever run it is.
+      __threadfence();
+      team_sync(team, tsh);
+      if (wt == 0 && lane < parts) {
+        const uint32_t k0 = (lane ? part_first[1] : part_first[0]) / chunk;
+        const uint32_t n = (lane ? part_last[1] : part_last[0]) / chunk - k0 + 1;
+        sm.merge_k[team][lane] = k0;
+        sm.merge_n[team][lane] = atomicInc(a.cnt + k0, n - 1) == n - 1 ? (int)n : 0;
+      }
+      team_sync(team, tsh);
+#pragma unroll 1
+      for (int q = 0; q < parts; ++q) {
+        const int n = sm.merge_n[team][q];
+        if (n == 0) continue;
+        __threadfence();
+        const int64_t k0 = sm.merge_k[team][q];
+        bf16* out = a.out + (q ? part_q[1] : part_q[0]) * 128;
+        kv4_share<G>(T, [&](auto V) {
+          constexpr int VW = decltype(V)::value;
+          for (int i = wt; i < G * 4 / VW; i += T) {
+            const Kv4Share<VW> sh(i, lane);
+            auto at = [&](int p) { return (2 * (k0 + p) + (p == 0)) * G + sh.hd; };
+            float M, L, O[VW];
+            kv4_combine<VW>(
+                n, lane, [&](int p) { return __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + at(p)); },
+                [&](int p, float(&y)[VW]) { sh.read(a.ws_o + at(p) * 128, y, [](auto* x) { return __ldcg(x); }); }, M, L,
+                O);
+            sh.write(out + sh.hd * 128, O, L);
+          }
+        });
+      }
     }
+    if (dead)  // copies in flight land (or run out of time once more) before the CTA ends
+      for (; (int)(issued - used) > 0; ++used) mbar_wait(&sm.full[warp][used % kStages], used / kStages & 1, a.err, nullptr);
   }
 
   // ---- rows without tokens are zero

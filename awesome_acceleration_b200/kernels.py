@@ -99,26 +99,34 @@ def prefill_attention(q, k_cache, v_cache, block_tables, seq_rows, cu_q, ctx_sta
 
 
 # ---------------------------------------------------------------- request maps
-def _device_of(t: torch.Tensor, what: str, name: str) -> int:
-    """The index of the current CUDA device, which `t` must be on: the kernels launch on its current stream."""
-    dev = t.get_device()
-    if dev < 0 or dev != torch._C._cuda_getDevice():
-        raise ValueError(f"{what}: {name} is on {t.device}, expected the current CUDA device")
-    return dev
+# The wrappers below are called once per layer of a decode step, so their checks are one expression each; what
+# exactly is wrong is only looked for once something is.
+_I32, _I64, _U8 = torch.int32, torch.int64, torch.uint8
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream, without a Stream object around it
 
 
-def _here(t: torch.Tensor, dtype, ndim: int, dev: int, what: str, name: str) -> None:
-    """`t` must be a contiguous `ndim`-d `dtype` tensor on device `dev`."""
-    if t is None:
-        raise ValueError(f"{what}: {name} is missing")
-    if t.dtype is not dtype or t.dim() != ndim or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be a contiguous {ndim}-d {dtype} tensor on cuda:{dev}, got "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device}, contiguous={t.is_contiguous()}")
+def _refuse(what: str, *args) -> None:
+    """Raise for the first of (tensor, dtype, ndim, name) that is not a contiguous `ndim`-d `dtype` tensor on the
+    current CUDA device, on whose current stream the kernels launch."""
+    for t, dtype, ndim, name in args:
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: {name} is not a tensor")
+        if not t.is_cuda or t.get_device() != _current_device():
+            raise ValueError(f"{what}: {name} is on {t.device}, expected the current CUDA device")
+        if t.dtype is not dtype or t.dim() != ndim or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous {ndim}-d {dtype} tensor, got {tuple(t.shape)} "
+                             f"{t.dtype}, contiguous={t.is_contiguous()}")
+    raise ValueError(f"{what}: shapes do not fit: " +
+                     ", ".join(f"{name} {tuple(t.shape)}" for t, _, _, name in args))
 
 
-def _raw_stream(dev: int) -> int:
-    """The current stream of device `dev`, without a Stream object around it (a tenth of the cost)."""
-    return torch._C._cuda_getCurrentRawStream(dev)
+def _ok(t, dtype, ndim: int, dev: int) -> bool:
+    return (t is not None and t.dtype is dtype and t.dim() == ndim and t.get_device() == dev and t.is_contiguous())
+
+
+def _is_current(dev: int) -> bool:
+    return dev >= 0 and dev == _current_device()
 
 
 def build_block_tables(lengths, block_size: int, *, max_blocks: int | None = None, free_blocks=None, out=None,
@@ -128,27 +136,25 @@ def build_block_tables(lengths, block_size: int, *, max_blocks: int | None = Non
     `free_blocks` (int32; None: 0, 1, 2, ...) in request order, the rest of
     its row is -1.  `used` (int32 [1]) receives the number of blocks taken."""
     what = "build_block_tables"
-    dev = _device_of(lengths, what, "lengths")
-    _here(lengths, torch.int32, 1, dev, what, "lengths")
+    dev = lengths.get_device()
+    if not (_ok(lengths, _I32, 1, dev) and _is_current(dev)):
+        _refuse(what, (lengths, _I32, 1, "lengths"))
     S = lengths.shape[0]
     if out is None:
         if max_blocks is None:
             raise ValueError(f"{what}: give max_blocks or out")
-        out = torch.empty((S, max_blocks), dtype=torch.int32, device=lengths.device)
-    else:
-        _here(out, torch.int32, 2, dev, what, "out")
-        if out.shape[0] != S or (max_blocks is not None and out.shape[1] != max_blocks):
-            raise ValueError(f"{what}: out is {tuple(out.shape)} for {S} requests")
+        out = torch.empty((S, max_blocks), dtype=_I32, device=lengths.device)
+    elif not _ok(out, _I32, 2, dev) or out.shape[0] != S or (max_blocks is not None and out.shape[1] != max_blocks):
+        _refuse(what, (out, _I32, 2, "out"), (lengths, _I32, 1, "lengths"))
     num_free = 0x7fffffff
     if free_blocks is not None:
-        _here(free_blocks, torch.int32, 1, dev, what, "free_blocks")
+        if not _ok(free_blocks, _I32, 1, dev):
+            _refuse(what, (free_blocks, _I32, 1, "free_blocks"))
         num_free = free_blocks.shape[0]
-    if used is not None:
-        _here(used, torch.int32, 1, dev, what, "used")
-        if used.shape[0] != 1:
-            raise ValueError(f"{what}: used holds one value")
-    rc = _lib_().aacc_build_block_tables(lengths.data_ptr(), S, block_size, _p(free_blocks), num_free, out.data_ptr(),
-                                         out.shape[1], _p(used), _raw_stream(dev))
+    if used is not None and not (_ok(used, _I32, 1, dev) and used.shape[0] == 1):
+        _refuse(what, (used, _I32, 1, "used"))
+    rc = _lib.load().aacc_build_block_tables(lengths.data_ptr(), S, block_size, _p(free_blocks), num_free,
+                                             out.data_ptr(), out.shape[1], _p(used), _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
     return out
@@ -163,33 +169,30 @@ def build_slot_maps(lengths, block_tables, *, block_size: int, num_blocks: int, 
     negative: padding).  Entries behind the last request get position 0 and
     slot -1; `num_tokens` may exceed the sum of the lengths."""
     what = "build_slot_maps"
-    dev = _device_of(lengths, what, "lengths")
-    _here(lengths, torch.int32, 1, dev, what, "lengths")
-    _here(block_tables, torch.int32, 2, dev, what, "block_tables")
+    dev = lengths.get_device()
+    if not (_ok(lengths, _I32, 1, dev) and _ok(block_tables, _I32, 2, dev) and _is_current(dev)):
+        _refuse(what, (lengths, _I32, 1, "lengths"), (block_tables, _I32, 2, "block_tables"))
     S = lengths.shape[0]
-    if starts is not None:
-        _here(starts, torch.int32, 1, dev, what, "starts")
-        if starts.shape[0] != S:
-            raise ValueError(f"{what}: {starts.shape[0]} starts for {S} requests")
-    if rows is not None:
-        _here(rows, torch.int64, 1, dev, what, "rows")
-        if rows.shape[0] != S:
-            raise ValueError(f"{what}: {rows.shape[0]} rows for {S} requests")
-
-    def output(t, dtype, n, name):
-        if t is None:
-            return torch.empty(n, dtype=dtype, device=lengths.device)
-        _here(t, dtype, 1, dev, what, name)
-        if t.shape[0] != n:
-            raise ValueError(f"{what}: {name} has {t.shape[0]} entries, expected {n}")
-        return t
-    cu = output(cu, torch.int32, S + 1, "cu")
-    positions = output(positions, torch.int64, num_tokens, "positions")
-    slots = output(slots, torch.int64, num_tokens, "slots")
+    if starts is not None and not (_ok(starts, _I32, 1, dev) and starts.shape[0] == S):
+        _refuse(what, (starts, _I32, 1, "starts"), (lengths, _I32, 1, "lengths"))
+    if rows is not None and not (_ok(rows, _I64, 1, dev) and rows.shape[0] == S):
+        _refuse(what, (rows, _I64, 1, "rows"), (lengths, _I32, 1, "lengths"))
+    if cu is None:
+        cu = torch.empty(S + 1, dtype=_I32, device=lengths.device)
+    elif not (_ok(cu, _I32, 1, dev) and cu.shape[0] == S + 1):
+        _refuse(what, (cu, _I32, 1, "cu"), (lengths, _I32, 1, "lengths"))
+    if positions is None:
+        positions = torch.empty(num_tokens, dtype=_I64, device=lengths.device)
+    elif not (_ok(positions, _I64, 1, dev) and positions.shape[0] == num_tokens):
+        _refuse(f"{what} (num_tokens {num_tokens})", (positions, _I64, 1, "positions"))
+    if slots is None:
+        slots = torch.empty(num_tokens, dtype=_I64, device=lengths.device)
+    elif not (_ok(slots, _I64, 1, dev) and slots.shape[0] == num_tokens):
+        _refuse(f"{what} (num_tokens {num_tokens})", (slots, _I64, 1, "slots"))
     num_rows, max_blocks = block_tables.shape
-    rc = _lib_().aacc_build_slot_maps(lengths.data_ptr(), _p(starts), _p(rows), S, block_tables.data_ptr(), num_rows,
-                                      max_blocks, block_size, num_blocks, cu.data_ptr(), positions.data_ptr(),
-                                      slots.data_ptr(), num_tokens, _raw_stream(dev))
+    rc = _lib.load().aacc_build_slot_maps(
+        lengths.data_ptr(), _p(starts), _p(rows), S, block_tables.data_ptr(), num_rows, max_blocks, block_size,
+        num_blocks, cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), num_tokens, _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
     return cu, positions, slots
@@ -207,23 +210,23 @@ def kv4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int) -> tupl
     return num_blocks, num_kv_heads, block_size // KV4_TILE, KV4_RECORD_BYTES
 
 
-def _kv4_pools(k_cache, v_cache, what: str):
-    """(device, num_blocks, Hkv, block_size) of a layer's pools, checked."""
-    dev = _device_of(k_cache, what, "k_cache")
-    _here(k_cache, torch.uint8, 4, dev, what, "k_cache")
-    _here(v_cache, torch.uint8, 4, dev, what, "v_cache")
+def _kv4_pools(k_cache, v_cache, dev: int, what: str):
+    """(num_blocks, Hkv, block_size) of a layer's pools on device `dev`, checked."""
+    if not (_ok(k_cache, _U8, 4, dev) and _ok(v_cache, _U8, 4, dev) and _is_current(dev)):
+        _refuse(what, (k_cache, _U8, 4, "k_cache"), (v_cache, _U8, 4, "v_cache"))
     shape = k_cache.shape
-    if shape[3] != KV4_RECORD_BYTES or v_cache.shape != shape:
+    nb, hkv, tiles, rec = shape
+    if rec != KV4_RECORD_BYTES or v_cache.shape != shape:
         raise ValueError(f"{what}: pools are {tuple(shape)} and {tuple(v_cache.shape)}, expected two of "
                          f"[blocks, heads, block_size / {KV4_TILE}, {KV4_RECORD_BYTES}]")
-    return dev, shape[0], shape[1], shape[2] * KV4_TILE
+    return nb, hkv, tiles * KV4_TILE
 
 
 def _kv_rows(x, hkv: int, T: int, dev: int, what: str, name: str):
     """(row stride, head stride) in elements of bf16 rows [T, hkv, 128] or [T, hkv * 128]."""
     shape, strides = tuple(x.shape), x.stride()
     if (x.dtype is not BF16 or x.get_device() != dev or strides[-1] != 1
-            or shape not in ((T, hkv, 128), (T, hkv * 128))):
+            or (shape != (T, hkv, 128) and shape != (T, hkv * 128))):
         raise ValueError(f"{what}: {name} must be bf16 rows [{T}, {hkv}, 128] with contiguous dims on cuda:{dev}, got "
                          f"{shape} {x.dtype} strides {strides} on {x.device}")
     # a dimension of size 1 may carry any stride: it is never stepped over
@@ -236,13 +239,15 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     flat slots of the 4-bit pools (see kv4_cache_shape); negative slots skip,
     the others must be distinct."""
     what = "kv4_store"
-    dev, nb, hkv, bs = _kv4_pools(k_cache, v_cache, what)
-    _here(slot_mapping, torch.int64, 1, dev, what, "slot_mapping")
+    dev = k_cache.get_device()
+    nb, hkv, bs = _kv4_pools(k_cache, v_cache, dev, what)
+    if not _ok(slot_mapping, _I64, 1, dev):
+        _refuse(what, (slot_mapping, _I64, 1, "slot_mapping"))
     T = slot_mapping.shape[0]
     ks, kh = _kv_rows(k, hkv, T, dev, what, "k")
     vs, vh = _kv_rows(v, hkv, T, dev, what, "v")
-    rc = _lib_().aacc_kv4_store(k.data_ptr(), v.data_ptr(), T, ks, kh, vs, vh, slot_mapping.data_ptr(),
-                                k_cache.data_ptr(), v_cache.data_ptr(), nb, hkv, bs, _raw_stream(dev))
+    rc = _lib.load().aacc_kv4_store(k.data_ptr(), v.data_ptr(), T, ks, kh, vs, vh, slot_mapping.data_ptr(),
+                                    k_cache.data_ptr(), v_cache.data_ptr(), nb, hkv, bs, _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
 
@@ -250,30 +255,31 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
 def kv4_load(k_cache, v_cache, slots, k_out=None, v_out=None, *, out_slots=None):
     """Dequantise flat slots (int64 [T]) of the 4-bit pools into bf16: rows
     k_out/v_out [n, Hkv, 128], or paged caches [blocks, Hkv, bs, 128] of any
-    block size; token t goes to row / flat slot out_slots[t] (None: t).  A
-    negative slot on either side skips the token.  Returns (k_out, v_out);
-    outputs made here are zero where a token is skipped."""
+    block size; token t goes to row / flat slot out_slots[t] (None: t), and
+    these must be distinct.  A negative slot on either side skips the token.
+    Returns (k_out, v_out); outputs made here are zero where a token is
+    skipped."""
     what = "kv4_load"
-    dev, nb, hkv, bs = _kv4_pools(k_cache, v_cache, what)
-    _here(slots, torch.int64, 1, dev, what, "slots")
+    dev = k_cache.get_device()
+    nb, hkv, bs = _kv4_pools(k_cache, v_cache, dev, what)
+    if not _ok(slots, _I64, 1, dev):
+        _refuse(what, (slots, _I64, 1, "slots"))
     T = slots.shape[0]
-    if out_slots is not None:
-        _here(out_slots, torch.int64, 1, dev, what, "out_slots")
-        if out_slots.shape[0] != T:
-            raise ValueError(f"{what}: {out_slots.shape[0]} out_slots for {T} slots")
+    if out_slots is not None and not (_ok(out_slots, _I64, 1, dev) and out_slots.shape[0] == T):
+        _refuse(what, (out_slots, _I64, 1, "out_slots"), (slots, _I64, 1, "slots"))
     if k_out is None or v_out is None:
         if out_slots is not None or k_out is not None or v_out is not None:
             raise ValueError(f"{what}: give both k_out and v_out (or neither and no out_slots)")
         k_out, v_out = torch.zeros((2, T, hkv, 128), dtype=BF16, device=k_cache.device)
     shape = k_out.shape
-    _here(k_out, BF16, len(shape), dev, what, "k_out")
-    _here(v_out, BF16, len(shape), dev, what, "v_out")
-    if v_out.shape != shape or len(shape) not in (3, 4) or shape[1] != hkv or shape[-1] != 128:
-        raise ValueError(f"{what}: outputs are {tuple(shape)} and {tuple(v_out.shape)}, expected two of "
-                         f"[rows, {hkv}, 128] or [blocks, {hkv}, block_size, 128]")
-    rc = _lib_().aacc_kv4_load(k_cache.data_ptr(), v_cache.data_ptr(), nb, hkv, bs, slots.data_ptr(), _p(out_slots), T,
-                               k_out.data_ptr(), v_out.data_ptr(), shape[0], 1 if len(shape) == 3 else shape[2],
-                               _raw_stream(dev))
+    ndim = len(shape)
+    if not (_ok(k_out, BF16, ndim, dev) and _ok(v_out, BF16, ndim, dev) and v_out.shape == shape
+            and (ndim == 3 or ndim == 4) and shape[1] == hkv and shape[-1] == 128):
+        _refuse(f"{what} (outputs [rows, {hkv}, 128] or [blocks, {hkv}, block_size, 128])",
+                (k_out, BF16, ndim, "k_out"), (v_out, BF16, ndim, "v_out"))
+    rc = _lib.load().aacc_kv4_load(k_cache.data_ptr(), v_cache.data_ptr(), nb, hkv, bs, slots.data_ptr(),
+                                   _p(out_slots), T, k_out.data_ptr(), v_out.data_ptr(), shape[0],
+                                   1 if ndim == 3 else shape[2], _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
     return k_out, v_out
@@ -288,29 +294,24 @@ def kv4_decode_attention(q, k_cache, v_cache, block_tables, rows, seqlens, *, ct
                          max_context: int, workspace: torch.Tensor, out=None) -> torch.Tensor:
     """q [B, Hq, 128] -> out [B, Hq, 128] over seqlens[rows[b]] + ctx_add
     tokens of the 4-bit pools (paged_decode_attention over the bf16 cache).
-    Calls that share `workspace` must be ordered on one stream."""
+    Calls that share `workspace` (uint8) must be ordered on one stream."""
     what = "kv4_decode_attention"
-    dev, nb, hkv, bs = _kv4_pools(k_cache, v_cache, what)
-    _here(q, BF16, 3, dev, what, "q")
-    _here(block_tables, torch.int32, 2, dev, what, "block_tables")
-    _here(rows, torch.int64, 1, dev, what, "rows")
-    _here(seqlens, torch.int32, 1, dev, what, "seqlens")
-    _here(workspace, torch.uint8, 1, dev, what, "workspace")
-    B, hq, d = q.shape
-    num_rows, max_blocks = block_tables.shape
-    if d != 128 or rows.shape[0] != B or seqlens.shape[0] != num_rows:
-        raise ValueError(f"{what}: q {tuple(q.shape)} with {rows.shape[0]} rows; {seqlens.shape[0]} seqlens with "
-                         f"{num_rows} block table rows")
+    dev = k_cache.get_device()
+    nb, hkv, bs = _kv4_pools(k_cache, v_cache, dev, what)
     if out is None:
         out = torch.empty_like(q)
-    else:
-        _here(out, BF16, 3, dev, what, "out")
-        if out.shape != q.shape:
-            raise ValueError(f"{what}: out is {tuple(out.shape)}, expected {tuple(q.shape)}")
-    rc = _lib_().aacc_kv4_decode_attention(
+    if not (q.dtype is BF16 and _ok(block_tables, _I32, 2, dev) and _ok(rows, _I64, 1, dev)
+            and _ok(seqlens, _I32, 1, dev) and _ok(workspace, _U8, 1, dev) and q.is_contiguous()
+            and q.get_device() == dev and _ok(out, BF16, 3, dev) and out.shape == q.shape
+            and rows.shape[0] == q.shape[0] and q.shape[2] == 128 and seqlens.shape[0] == block_tables.shape[0]):
+        _refuse(what, (q, BF16, 3, "q"), (block_tables, _I32, 2, "block_tables"), (rows, _I64, 1, "rows"),
+                (seqlens, _I32, 1, "seqlens"), (workspace, _U8, 1, "workspace"), (out, BF16, 3, "out"))
+    B, hq, _ = q.shape
+    num_rows, max_blocks = block_tables.shape
+    rc = _lib.load().aacc_kv4_decode_attention(
         q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), nb, block_tables.data_ptr(), num_rows,
         max_blocks, rows.data_ptr(), seqlens.data_ptr(), ctx_add, B, hq, hkv, bs, scale, max_context,
-        workspace.data_ptr(), workspace.shape[0], _raw_stream(dev))
+        workspace.data_ptr(), workspace.numel(), _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
     return out
