@@ -375,20 +375,18 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     }
   }
   __syncthreads();
-  // Lane i weighs T = 2^i, in microseconds of a model fitted to runs of 17 shapes with each T (B200; within 2 %
-  // of the best T on average): a round of tiles takes 0.26 us per warp at work on the SM, but 2.5 us at least;
-  // merging costs 1 us, and 0.1 us for each of the G / T heads of a partial that a warp merges; the end of a
-  // segment 0.2 us for each.
+  // Lane i weighs T = 2^i, in microseconds of a model fitted to runs of 17 shapes with each T (B200; on average
+  // within 1 % of the best T, at most 5 %): 3 us for a round of tiles; for each segment of a run 0.15 us per warp
+  // that the first has to wait for; where items are shared, 2 us, and 0.06 us for each of the G / T heads of a
+  // part that a warp adds.
   if (warp == 0) {
     const int opt = min(lane, kSizes - 1);
     const uint32_t n = sm.sum[opt] * a.Hkv, teams = gridDim.x * (kAttWarps >> opt);
     const uint32_t c = max((n + teams - 1) / teams, 1u);
     const float t = (float)(1 << opt), ch = (float)c;
     const float per_item = __fdividef((float)n, (float)max(sm.sum[kSizes] * a.Hkv, 1u));
-    const float busy = t * ceilf(__fdividef(ceilf(__fdividef((float)n, ch)), (float)gridDim.x));
-    float cost = ch * fmaxf(2.5f, 0.26f * busy) +
-                 0.2f * (1.f + __fdividef(ch, fmaxf(per_item, 1.f))) * fmaxf(1.f, __fdividef(G, t));
-    if (per_item > ch) cost += 1.f + 0.1f * G * __fdividef(per_item, ch * t);
+    float cost = 3.f * ch + 0.15f * (t - 1.f) * (1.f + __fdividef(ch, fmaxf(per_item, 1.f)));
+    if (per_item > ch) cost += 2.f + 0.06f * G * __fdividef(per_item, ch * t);
     const uint32_t best = __reduce_min_sync(0xffffffffu, (__float_as_uint(cost) & ~7u) | opt) & 7u;
     if (lane == best) {
       sm.plan[0] = best;
