@@ -14,6 +14,9 @@ unit the attention kernels stream with TMA.
 Host bookkeeping (block free list, per-row lengths) lives here; the device
 copies (``block_tables`` int32 [rows][max_blocks], ``seqlens`` int32 [rows])
 are what the kernels read.
+
+``PagedKV4Cache`` is the same cache with K and V held in 4 bits (144 bytes per
+token and kv head instead of 512).
 """
 from __future__ import annotations
 
@@ -22,6 +25,8 @@ import torch
 
 
 class PagedKVCache:
+    bits = 16  # per stored value
+
     def __init__(self, num_layers: int, num_kv_heads: int, num_rows: int, max_seq_len: int, *,
                  block_size: int = 256, num_blocks: int | None = None, head_dim: int = 128,
                  device="cuda", dtype=torch.bfloat16):
@@ -36,7 +41,7 @@ class PagedKVCache:
         if num_blocks is None:
             num_blocks = num_rows * self.max_blocks
         self.num_blocks = num_blocks
-        shape = (num_layers, num_blocks, num_kv_heads, block_size, head_dim)
+        shape, dtype = self._pool(dtype)
         # Zero-filled: masked tail tokens of a tile are multiplied by p = 0,
         # so the pool must never hold non-finite values.
         self.k = torch.zeros(shape, dtype=dtype, device=device)
@@ -48,6 +53,15 @@ class PagedKVCache:
         self.lengths = np.zeros(num_rows, dtype=np.int64)  # host mirror of seqlens
         self._free = list(range(num_blocks - 1, -1, -1))  # pop() yields the lowest id
         self._dirty = False
+
+    def _pool(self, dtype):
+        """Shape and dtype of the K (and of the V) pool of all layers."""
+        return (self.num_layers, self.num_blocks, self.num_kv_heads, self.block_size, 128), dtype
+
+    @staticmethod
+    def bytes_per_token_head() -> int:
+        """Bytes of K and V of one token and kv head."""
+        return 2 * 128 * 2
 
     # ------------------------------------------------------------ blocks
     @property
@@ -120,3 +134,47 @@ class PagedKVCache:
         k = self.k[layer][blk, :, off]
         v = self.v[layer][blk, :, off]
         return k, v
+
+    def store(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Write K, V rows [T, Hkv, 128] (bf16, on the cache's device, the current one) to flat slots."""
+        from . import kernels as K
+        T = k.shape[0]
+        K.kv_store(k.view(T, -1), v.view(T, -1), slots, self.k[layer], self.v[layer])
+
+
+class PagedKV4Cache(PagedKVCache):
+    """K and V in 4-bit codes with a bf16 scale per 32 dims (``kernels.kv4_store``), uint8
+    ``[num_layers][num_blocks][num_kv_heads][block_size / 64][4608]``.  What is stored is rounded: a value is
+    within half a step of its group's scale, max|x| / 7, of the original."""
+
+    bits = 4
+
+    def _pool(self, dtype):
+        from . import kernels as K
+        if dtype != torch.bfloat16:
+            raise ValueError("the 4-bit cache quantises bf16 rows")
+        return (self.num_layers,) + K.kv4_cache_shape(self.num_blocks, self.num_kv_heads, self.block_size), torch.uint8
+
+    @staticmethod
+    def bytes_per_token_head() -> int:
+        from . import kernels as K
+        return 2 * K.KV4_RECORD_BYTES // K.KV4_TILE
+
+    def gather(self, layer: int, row: int, length: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The values that the cache holds for the first `length` tokens of `row`, bf16 [length, Hkv, 128]."""
+        from . import kernels as K
+        with torch.cuda.device(self.k.device):
+            slots = torch.from_numpy(self.slot_mapping(row, 0, length)).to(self.k.device)
+            return K.kv4_load(self.k[layer], self.v[layer], slots)
+
+    def store(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        from . import kernels as K
+        K.kv4_store(k, v, slots, self.k[layer], self.v[layer])
+
+
+def kv_cache_class(kv_bits: int) -> type[PagedKVCache]:
+    """The cache that holds a value in `kv_bits` bits (16: bf16; 4)."""
+    for cls in (PagedKVCache, PagedKV4Cache):
+        if cls.bits == kv_bits:
+            return cls
+    raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")

@@ -24,7 +24,9 @@ them back into its cache (``import_request_kv``, model/model.py:168-177,
                     side has acknowledged (through whatever channel carried
                     the ticket).
 
-Buffer layout: bf16 ``[2][layers][length][kv_heads][128]`` (K, then V).
+Buffer layout: bf16 ``[2][layers][length][kv_heads][128]`` (K, then V).  A
+4-bit cache exports the values it holds and quantises what it imports, so
+either side may hold its cache in 16 or in 4 bits.
 """
 from __future__ import annotations
 
@@ -123,12 +125,17 @@ def import_request_kv_ipc(model, slot_idx: int, ticket: KVTicket) -> None:
             stream = torch.cuda.current_stream().cuda_stream
             layer_bytes = n * kv.num_kv_heads * 128 * 2
             rs = kv.num_kv_heads * 128  # row stride of one token, elements
-            nb, hkv, bs, _ = kv.k[0].shape
+            pool = (kv.num_blocks, kv.num_kv_heads, kv.block_size)
             for i in range(kv.num_layers):
                 k_ptr = ptr + i * layer_bytes
                 v_ptr = ptr + (kv.num_layers + i) * layer_bytes
-                _lib.check(lib.aacc_kv_store(k_ptr, v_ptr, n, rs, rs, slots.data_ptr(), kv.k[i].data_ptr(),
-                                             kv.v[i].data_ptr(), nb, hkv, bs, stream), "kv_store (ipc import)")
+                caches = (slots.data_ptr(), kv.k[i].data_ptr(), kv.v[i].data_ptr())
+                if kv.bits == 4:
+                    _lib.check(lib.aacc_kv4_store(k_ptr, v_ptr, n, rs, 128, rs, 128, *caches, *pool, stream),
+                               "kv4_store (ipc import)")
+                else:
+                    _lib.check(lib.aacc_kv_store(k_ptr, v_ptr, n, rs, rs, *caches, *pool, stream),
+                               "kv_store (ipc import)")
             torch.cuda.current_stream().synchronize()  # done reading the peer buffer
         finally:
             K.peer_buffer_close(ptr)

@@ -25,6 +25,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from .kv_cache import kv_cache_class
 from .model.model import Qwen3Config, Qwen3ForCausalLM
 
 
@@ -63,7 +64,7 @@ def sampling_seed(base: int, serial: int, index: int) -> int:
 
 
 def kv_sized_max_seqs(config: Qwen3Config, max_num_seqs: int, max_seq_len: int, reserve_gb: float,
-                      device, tp_size: int = 1, prefill_chunk_tokens: int = 0) -> int:
+                      device, tp_size: int = 1, prefill_chunk_tokens: int = 0, kv_bits: int = 16) -> int:
     """The reference's batch sizing from GPU memory (llm.py:58-71, llm_tp.py:160-178):
     KV bytes per token (this rank's heads) against the memory left after a fixed
     reserve.  Called once the weights are on the device, it also keeps the
@@ -72,21 +73,28 @@ def kv_sized_max_seqs(config: Qwen3Config, max_num_seqs: int, max_seq_len: int, 
     torch.cuda.synchronize(device)
     torch.cuda.empty_cache()  # blocks the allocator caches (e.g. weight-init temporaries) are free for the KV pool
     free, total = torch.cuda.mem_get_info(device)
-    per_tok = 2 * config.num_key_value_heads * config.head_dim * 2 * config.num_hidden_layers // tp_size
+    per_tok = (kv_cache_class(kv_bits).bytes_per_token_head() * config.num_key_value_heads * config.num_hidden_layers
+               // tp_size)
     q_cols = config.num_attention_heads * config.head_dim // tp_size
     act = prefill_chunk_tokens * (3 * config.hidden_size + 2 * q_cols + config.intermediate_size // tp_size) * 2
+    if kv_bits == 4:  # a chunk's bf16 K/V rows, and the bf16 context of its sequences (one layer)
+        act += (2 * prefill_chunk_tokens + max_seq_len) * 2 * config.num_key_value_heads * config.head_dim * 2 // tp_size
     reserve = reserve_gb * (1024 ** 3)
     avail = min(total - reserve, free - reserve - act)
     return max(1, min(max_num_seqs, int(avail / per_tok) // max_seq_len))
 
 
 class LLM:
-    """High-throughput Qwen3 engine with continuous batching on one B200."""
+    """High-throughput Qwen3 engine with continuous batching on one B200.
+
+    ``kv_bits=4`` holds the KV cache in 4 bits instead of bf16: 3.6 times the
+    sequences in the same memory, and decode attention that reads 3.6 times
+    less, for K and V rounded to 15 steps of their groups of 32 dims."""
 
     def __init__(self, model_path: str | None = None, max_num_seqs: int = 32, max_seq_len: int = 4096,
                  dtype=torch.bfloat16, *, config: Qwen3Config | None = None, model: Qwen3ForCausalLM | None = None,
                  seed: int = 0, block_size: int = 256, use_cuda_graphs: bool = True,
-                 prefill_chunk_tokens: int = 32768, device=None, verbose: bool = False):
+                 prefill_chunk_tokens: int = 32768, device=None, verbose: bool = False, kv_bits: int = 16):
         self.device = torch.device(device or "cuda")
         if self.device.type == "cuda" and self.device.index is None:  # pin it: the loop runs in another thread
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -113,8 +121,9 @@ class LLM:
         self.model.prefill_chunk_tokens = prefill_chunk_tokens
         self.model.fuse_qkv()  # before sizing: the fused weights are what stays resident
         self.max_num_seqs = kv_sized_max_seqs(self.config, max_num_seqs, max_seq_len, 3.0, self.device,
-                                              prefill_chunk_tokens=prefill_chunk_tokens)
-        self.model.init_kv_cache(self.max_num_seqs, max_seq_len, self.device, dtype, block_size=block_size)
+                                              prefill_chunk_tokens=prefill_chunk_tokens, kv_bits=kv_bits)
+        self.model.init_kv_cache(self.max_num_seqs, max_seq_len, self.device, dtype, block_size=block_size,
+                                 kv_bits=kv_bits)
         self._request_queue: queue.Queue[_Request] = queue.Queue()
         self._base_seed = int(seed)  # sampling noise: one stream per (request, prompt)
         self._serials = itertools.count(1)

@@ -41,7 +41,7 @@ class LLMTP:
                  dtype=torch.bfloat16, enable_tp: bool = True, tp_size: int = 1, *,
                  config: Qwen3Config | None = None, state_dict: dict | None = None, seed: int = 0,
                  block_size: int = 256, use_cuda_graphs: bool = True, prefill_chunk_tokens: int = 32768,
-                 timeout_s: float = 300.0):
+                 timeout_s: float = 300.0, kv_bits: int = 16):
         if enable_tp:
             D.init_distributed(tp_size=tp_size, timeout_s=timeout_s)
         self.tp_size = D.get_tp_world_size()
@@ -85,12 +85,13 @@ class LLMTP:
         self.model.prefill_chunk_tokens = prefill_chunk_tokens
         self.model.fuse_qkv()  # before sizing: the fused weights are what stays resident
         self.max_num_seqs = kv_sized_max_seqs(self.config, max_num_seqs, max_seq_len, 15.0, self.device, self.tp_size,
-                                              prefill_chunk_tokens)
+                                              prefill_chunk_tokens, kv_bits)
         if self.tp_size > 1:  # free memory differs a little per GPU; the group must agree on slots and buckets
             n = torch.tensor([self.max_num_seqs], dtype=torch.int64)
             torch.distributed.all_reduce(n, op=torch.distributed.ReduceOp.MIN, group=D.get_tp_cpu_group())
             self.max_num_seqs = int(n.item())
-        self.model.init_kv_cache(self.max_num_seqs, max_seq_len, self.device, dtype, block_size=block_size)
+        self.model.init_kv_cache(self.max_num_seqs, max_seq_len, self.device, dtype, block_size=block_size,
+                                 kv_bits=kv_bits)
         self._bcast = torch.zeros(5 * self.model.max_batch, dtype=torch.int64, device=self.device)
         self._base_seed = int(seed)  # sampling noise: one stream per (request, prompt)
         self._serials = itertools.count(1)

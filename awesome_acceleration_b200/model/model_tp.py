@@ -20,8 +20,8 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from ..kv_cache import PagedKVCache
-from ..runtime import LayerWeights, Qwen3Runtime, TPComm, interleave_gate_up, rope_table
+from ..kv_cache import PagedKVCache, kv_cache_class
+from ..runtime import LayerWeights, Qwen3Runtime, TPComm, interleave_gate_up, rope_table, runtime_class
 from .distributed import (get_tp_cpu_group, get_tp_group, get_tp_rank, get_tp_world_size, split_tensor_along_dim,
                           tensor_model_parallel_all_gather)
 from .model import Qwen3Config, RMSNorm, RotaryEmbedding
@@ -140,13 +140,14 @@ class Qwen3ForCausalLMTP(nn.Module):
         self.runtime = None
 
     def init_kv_cache(self, num_slots: int, max_seq_len: int, device, dtype, *, block_size: int = 256,
-                      num_blocks: int | None = None, max_batch: int | None = None):
-        """Per-rank KV heads (model/model_tp.py:410-426), paged."""
+                      num_blocks: int | None = None, max_batch: int | None = None, kv_bits: int = 16):
+        """Per-rank KV heads (model/model_tp.py:410-426), paged; kv_bits=4 as on one GPU."""
         if dtype != torch.bfloat16:
             raise ValueError("the B200 hot path computes in bf16")
         cfg = self.config
-        self.kv = PagedKVCache(cfg.num_hidden_layers, cfg.num_key_value_heads // self.tp_size, num_slots,
-                               max_seq_len, block_size=block_size, num_blocks=num_blocks, device=device, dtype=dtype)
+        self.kv = kv_cache_class(kv_bits)(cfg.num_hidden_layers, cfg.num_key_value_heads // self.tp_size, num_slots,
+                                          max_seq_len, block_size=block_size, num_blocks=num_blocks, device=device,
+                                          dtype=dtype)
         self.max_batch = max_batch or num_slots or 1  # a decode step may hold every slot
         for i, layer in enumerate(self.model.layers):
             attn = layer.self_attn
@@ -168,7 +169,7 @@ class Qwen3ForCausalLMTP(nn.Module):
                                    l.self_attn.o_proj.weight.data, l.post_attention_layernorm.weight.data,
                                    l.mlp._gate_up, l.mlp.down_proj.weight.data) for l in self.model.layers]
             comm = TPComm(self.tp_rank, self.tp_size, get_tp_group(), get_tp_cpu_group())
-            self.runtime = Qwen3Runtime(
+            self.runtime = runtime_class(self.kv)(
                 hidden=cfg.hidden_size, intermediate=cfg.intermediate_size, num_q_heads=cfg.num_attention_heads,
                 num_kv_heads=cfg.num_key_value_heads, vocab=cfg.vocab_size, eps=cfg.rms_norm_eps, layers=layers,
                 embed=self.model.embed_tokens.weight.data, final_norm=self.model.norm.weight.data,

@@ -285,23 +285,24 @@ class Qwen3Runtime:
         sp = K.pick_skinny_splits(M, N, Kd, target=target, max_elems=part.numel())
         return sp, part[:sp * M * N].view(sp, M, N)
 
-    def _qkv(self, i, lw, x, positions, slot_map, q, part):
-        """Fused QKV projection + q/k-norm + RoPE + KV store (model/model.py:219-226)."""
-        kv = self.kv
+    def _qkv(self, i, lw, x, positions, slot_map, q, part, pools=None):
+        """Fused QKV projection + q/k-norm + RoPE + KV store (model/model.py:219-226),
+        into layer i's cache or the given (k, v) `pools`."""
+        k_pool, v_pool = (self.kv.k[i], self.kv.v[i]) if pools is None else pools
         M = x.shape[0]
         if self._skinny(M, part):
             sp, pv = self._skinny_part(M, lw.wqkv, part, K.SKINNY_TARGET_CTAS)
             if M <= self.skinny_fused_rows:
                 K.skinny_qkv_norm_rope_store(x, lw.wqkv, pv, sp, self.buf.sk_cnt, lw.q_norm, lw.k_norm, self.eps,
-                                             positions, self.rope, slot_map, kv.k[i], kv.v[i], self.Hq, q_out=q)
+                                             positions, self.rope, slot_map, k_pool, v_pool, self.Hq, q_out=q)
             else:
                 K.gemm_skinny_splitk(x, lw.wqkv, pv, sp)
                 K.splitk_qkv_norm_rope_store(pv, sp, lw.q_norm, lw.k_norm, self.eps, positions, self.rope, slot_map,
-                                             kv.k[i], kv.v[i], self.Hq, q_out=q)
+                                             k_pool, v_pool, self.Hq, q_out=q)
             return
         if self._cluster(M, part):
             K.qkv_norm_rope_store_cluster(x, lw.wqkv, lw.q_norm, lw.k_norm, self.eps, positions, self.rope, slot_map,
-                                          kv.k[i], kv.v[i], self.Hq, q_out=q)
+                                          k_pool, v_pool, self.Hq, q_out=q)
             return
         splits = self._splits(M, lw.wqkv, part)
         if splits > 1:
@@ -309,10 +310,10 @@ class Qwen3Runtime:
             pv = part[:splits * M * N].view(splits, M, N)
             K.gemm_splitk(x, lw.wqkv, pv, splits)
             K.splitk_qkv_norm_rope_store(pv, splits, lw.q_norm, lw.k_norm, self.eps, positions, self.rope, slot_map,
-                                         kv.k[i], kv.v[i], self.Hq, q_out=q)
+                                         k_pool, v_pool, self.Hq, q_out=q)
         else:
             K.qkv_norm_rope_store(x, lw.wqkv, lw.q_norm, lw.k_norm, self.eps, positions, self.rope, slot_map,
-                                  kv.k[i], kv.v[i], self.Hq, q_out=q)
+                                  k_pool, v_pool, self.Hq, q_out=q)
 
     def _gate_up(self, lw, x, act, part):
         """gate/up projection + SiLU-mul (model/model.py:189-190)."""
@@ -407,6 +408,12 @@ class Qwen3Runtime:
         K.argmax_merge_packed(gathered, M, tokens)
 
     # ------------------------------------------------------------------ decode
+    def _decode_attend(self, i, q, out, rows):
+        """Layer i's attention of one decode step."""
+        kv = self.kv
+        K.paged_decode_attention(q, kv.k[i], kv.v[i], kv.block_tables, rows, kv.seqlens, ctx_add=1, scale=self.scale,
+                                 max_context=self.max_context, workspace=self.buf.attn_ws, out=out)
+
     def _decode_body(self, B: int, logits=None):
         b = self.buf
         kv = self.kv
@@ -415,8 +422,7 @@ class Qwen3Runtime:
         K.embed_rmsnorm(ids, self.embed, self.layers[0].in_ln, self.eps, b.res[:B], b.x[:B])
 
         def attend(i, q, out):
-            K.paged_decode_attention(q, kv.k[i], kv.v[i], kv.block_tables, rows, kv.seqlens, ctx_add=1,
-                                     scale=self.scale, max_context=self.max_context, workspace=b.attn_ws, out=out)
+            self._decode_attend(i, q, out, rows)
 
         self._layer_chain(b.x[:B], b.res[:B], b.delta[:B], b.q[:B], b.attn[:B], b.act[:B], attend, pos,
                           b.slot_map[:B], part=b.part)
@@ -590,6 +596,21 @@ class Qwen3Runtime:
         return int(self._tok_err[handle])
 
     # ------------------------------------------------------------------ prefill
+    def _prefill_slots(self, rows, lens) -> list[np.ndarray]:
+        """Per-token int64 arrays that go to the device with a prefill's ids and positions (see _prefill_chunk)."""
+        return [np.concatenate([self.kv.slot_mapping(r, 0, L) for r, L in zip(rows, lens)])]
+
+    def _prefill_chunk(self, seq_rows, cu_q, ctx0, ends, max_q: int, maps):
+        """(slots of the chunk's tokens, attend(i, q, out) of layer i) for pieces of the rows `seq_rows` with query
+        offsets `cu_q` after `ctx0` cached tokens, up to the host list `ends`; `maps` has the chunk's columns of
+        the _prefill_slots arrays."""
+        kv = self.kv
+
+        def attend(i, q, out):
+            K.prefill_attention(q, kv.k[i], kv.v[i], kv.block_tables, seq_rows, cu_q, ctx0, max_q_len=max_q,
+                                scale=self.scale, out=out)
+        return maps[0], attend
+
     def prefill(self, sequences: list[list[int]], rows: list[int], *, positions: list[list[int]] | None = None,
                 store_lengths: list[int] | None = None, all_logits: bool = False, last_logits: bool = False,
                 temperatures: list[float] | None = None, seeds: list[int] | None = None):
@@ -614,11 +635,10 @@ class Qwen3Runtime:
             pos = np.concatenate([np.arange(L, dtype=np.int64) for L in lens])
         else:
             pos = np.concatenate([np.asarray(p, dtype=np.int64) for p in positions])
-        smap = np.concatenate([kv.slot_mapping(r, 0, L) for r, L in zip(rows, lens)])
-        host = torch.from_numpy(np.stack([flat, pos, smap])).pin_memory()
+        host = torch.from_numpy(np.stack([flat, pos, *self._prefill_slots(rows, lens)])).pin_memory()
         meta = host.to(dev, non_blocking=True)
         self.h2d_bytes += host.numel() * 8
-        ids_d, pos_d, smap_d = meta[0], meta[1], meta[2]
+        ids_d, pos_d = meta[0], meta[1]
         tokens = torch.empty(n, dtype=torch.int64, device=dev)
         samp = None
         if temperatures is not None and any(t > 0 for t in temperatures):
@@ -684,12 +704,9 @@ class Qwen3Runtime:
             xs, rs, ds = x[:Tc], res[:Tc], delta[:Tc]
             K.embed_rmsnorm(ids_d[t0:t0 + Tc], self.embed, self.layers[0].in_ln, self.eps, rs, xs)
 
-            def attend(i, qq, out, seq_rows=seq_rows, cu_q=cu_q, ctx0=ctx0, max_q=max_q):
-                K.prefill_attention(qq, kv.k[i], kv.v[i], kv.block_tables, seq_rows, cu_q, ctx0, max_q_len=max_q,
-                                    scale=self.scale, out=out)
-
-            self._layer_chain(xs, rs, ds, q[:Tc], attn[:Tc], act[:Tc], attend, pos_d[t0:t0 + Tc],
-                              smap_d[t0:t0 + Tc])
+            slots, attend = self._prefill_chunk(seq_rows, cu_q, ctx0, [e for _, _, e in ch], max_q,
+                                                meta[2:, t0:t0 + Tc])
+            self._layer_chain(xs, rs, ds, q[:Tc], attn[:Tc], act[:Tc], attend, pos_d[t0:t0 + Tc], slots)
             if all_logits:
                 tk = torch.empty(Tc, dtype=torch.int64, device=dev)
                 K.lm_head_argmax(xs, self.lm_head, tk, lm_ws, logits=out_logits[t0:t0 + Tc], best_val=best[:Tc],
@@ -711,3 +728,74 @@ class Qwen3Runtime:
             K.argmax_rows(K.gather_rows(out_logits, last), tokens)
         kv.set_lengths(rows, store_lengths if store_lengths is not None else lens)
         return (tokens, out_logits) if (all_logits or last_logits) else tokens
+
+
+class Qwen3RuntimeKV4(Qwen3Runtime):
+    """The same steps over a 4-bit cache (PagedKV4Cache).
+
+    The QKV epilogue writes the new tokens' bf16 K/V to staging rows, kv4_store quantises them into the cache.
+    Decode attends to the cache as it is.  Prefill loads the context of the chunk's sequences, the chunk's own
+    tokens among it, from the cache into a bf16 scratch pool of one layer, with block tables and slot maps built
+    on the device, and attends to that: what a token attends to is what the cache holds, however the prompt is
+    cut into chunks and whether a token comes from prefill or decode."""
+
+    SCRATCH_BLOCK = 256  # tokens per block of the prefill's scratch pool
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self._stage_decode = self._staging(self.max_batch)
+        self._stage = self._stage_decode  # prefill puts its own here while it runs
+        self.kv4_ws = torch.zeros(K.kv4_decode_workspace_bytes(self.Hq, self.Hkv), dtype=torch.uint8,
+                                  device=self.device)
+
+    def _staging(self, n: int):
+        """(k, v, slots): a bf16 pool of n one-token blocks, i.e. rows [n, Hkv, 128], and their slots 0 .. n - 1."""
+        kv = torch.zeros((2, n, self.Hkv, 1, 128), dtype=torch.bfloat16, device=self.device)
+        return kv[0], kv[1], torch.arange(n, dtype=torch.int64, device=self.device)
+
+    def _qkv(self, i, lw, x, positions, slot_map, q, part):
+        k, v, slots = self._stage
+        M = x.shape[0]
+        super()._qkv(i, lw, x, positions, slots[:M], q, part, pools=(k, v))
+        K.kv4_store(k[:M, :, 0], v[:M, :, 0], slot_map, self.kv.k[i], self.kv.v[i])
+
+    def _decode_attend(self, i, q, out, rows):
+        kv = self.kv
+        K.kv4_decode_attention(q, kv.k[i], kv.v[i], kv.block_tables, rows, kv.seqlens, ctx_add=1, scale=self.scale,
+                               max_context=self.max_context, workspace=self.kv4_ws, out=out)
+
+    def _prefill_slots(self, rows, lens):
+        return []  # built on the device, per chunk
+
+    def prefill(self, *args, **kw):
+        try:
+            return super().prefill(*args, **kw)
+        finally:
+            self._stage = self._stage_decode
+
+    def _prefill_chunk(self, seq_rows, cu_q, ctx0, ends, max_q: int, maps):
+        kv, bs = self.kv, self.SCRATCH_BLOCK
+        n_new, n_ctx, n_blk = maps.shape[1], sum(ends), sum((e + bs - 1) // bs for e in ends)
+        lens = cu_q[1:] - cu_q[:-1]
+        total = ctx0 + lens
+        ctx0 = ctx0.contiguous()
+        cache = dict(block_size=kv.block_size, num_blocks=kv.num_blocks, rows=seq_rows)
+        cu, _, new_slots = K.build_slot_maps(lens, kv.block_tables, num_tokens=n_new, starts=ctx0, **cache)
+        _, _, src = K.build_slot_maps(total, kv.block_tables, num_tokens=n_ctx, **cache)
+        tables = K.build_block_tables(total, bs, max_blocks=(max(ends) + bs - 1) // bs)
+        _, _, dst = K.build_slot_maps(total, tables, num_tokens=n_ctx, block_size=bs, num_blocks=n_blk)
+        rows = torch.arange(len(ends), dtype=torch.int64, device=self.device)
+        if self._stage is self._stage_decode or self._stage[0].shape[0] < n_new:
+            self._stage = self._staging(n_new)
+        # Zero-filled: the attention multiplies the tail of a sequence's last tile by p = 0.
+        k, v = torch.zeros((2, n_blk, self.Hkv, bs, 128), dtype=torch.bfloat16, device=self.device)
+
+        def attend(i, q, out):
+            K.kv4_load(kv.k[i], kv.v[i], src, k, v, out_slots=dst)
+            K.prefill_attention(q, k, v, tables, rows, cu, ctx0, max_q_len=max_q, scale=self.scale, out=out)
+        return new_slots, attend
+
+
+def runtime_class(kv: PagedKVCache) -> type[Qwen3Runtime]:
+    """The runtime that drives a cache of `kv`'s kind."""
+    return Qwen3RuntimeKV4 if kv.bits == 4 else Qwen3Runtime

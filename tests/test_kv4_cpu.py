@@ -88,3 +88,53 @@ def test_c_abi_checks_arguments_before_any_cuda_call():
         return lib.aacc_build_slot_maps(16, None, None, S, 16, nr, mb, bs, nb, 16, None, 16, T, None)
     for kw in (dict(S=-1), dict(nr=-1), dict(mb=0), dict(bs=0), dict(nb=0), dict(T=-1), dict(T=2 ** 31)):
         assert maps(**kw) == 1, kw
+
+
+def test_cache_of_either_width():
+    from awesome_acceleration_b200.kv_cache import PagedKV4Cache, PagedKVCache, kv_cache_class
+    assert kv_cache_class(16) is PagedKVCache and kv_cache_class(4) is PagedKV4Cache
+    for bits in (8, 0, 32):
+        with pytest.raises(ValueError, match="kv_bits"):
+            kv_cache_class(bits)
+    kv = PagedKV4Cache(3, 2, 4, 1000, block_size=128, device="cpu")
+    assert kv.k.shape == (3, kv.num_blocks, 2, 2, 4608) and kv.k.dtype == torch.uint8 and kv.bits == 4
+    assert PagedKVCache.bytes_per_token_head() == 512 and PagedKV4Cache.bytes_per_token_head() == 144
+    kv.reserve(1, 300)
+    kv.sync()
+    assert kv.block_tables[1, :4].tolist() == [0, 1, 2, -1]
+    assert kv.slot_mapping(1, 127, 130).tolist() == [127, 128, 129]
+    with pytest.raises(ValueError, match="bf16"):
+        PagedKV4Cache(1, 1, 1, 64, device="cpu", dtype=torch.float16)
+
+
+def test_runtime_of_either_width(monkeypatch):
+    """The 4-bit runtime projects into its staging rows and stores them, then attends to the 4-bit pools."""
+    import types
+
+    from awesome_acceleration_b200 import runtime as R
+    calls = []
+
+    class Rec:
+        CLUSTER_MAX_ROWS, SKINNY_MAX_ROWS = K.CLUSTER_MAX_ROWS, K.SKINNY_MAX_ROWS
+
+        def __getattr__(self, name):
+            return lambda *a, **kw: calls.append((name, a, kw))
+    monkeypatch.setattr(R, "K", Rec())
+    assert R.runtime_class(types.SimpleNamespace(bits=4)) is R.Qwen3RuntimeKV4
+    assert R.runtime_class(types.SimpleNamespace(bits=16)) is R.Qwen3Runtime
+    rt = R.Qwen3RuntimeKV4.__new__(R.Qwen3RuntimeKV4)
+    rt.eps, rt.rope, rt.Hq, rt.Hkv, rt.skinny_rows, rt.cluster_gemm = 1e-6, None, 4, 2, 0, False
+    rt.device, rt.scale, rt.max_context, rt.kv4_ws = torch.device("cpu"), 1.0, 256, None
+    rt.kv = types.SimpleNamespace(k=["k0"], v=["v0"], block_tables="bt", seqlens="sl")
+    rt._stage = rt._stage_decode = rt._staging(8)
+    lw = types.SimpleNamespace(wqkv=torch.empty((1024, 256)), q_norm=None, k_norm=None)
+    slot_map = torch.tensor([5, -1, 9])
+    rt._qkv(0, lw, torch.empty((3, 256)), None, slot_map, None, None)
+    assert [c[0] for c in calls] == ["qkv_norm_rope_store", "kv4_store"]
+    a = calls[0][1]
+    assert a[7].tolist() == [0, 1, 2] and a[8].shape == (8, 2, 1, 128)  # staging slots and pool
+    k, v, slots, kc, vc = calls[1][1]
+    assert k.shape == v.shape == (3, 2, 128) and slots is slot_map and (kc, vc) == ("k0", "v0")
+    assert k.data_ptr() == rt._stage[0].data_ptr() and k.stride() == (256, 128, 1)
+    rt._decode_attend(0, "q", "out", "rows")
+    assert calls[2][0] == "kv4_decode_attention" and calls[2][1][:3] == ("q", "k0", "v0")
