@@ -210,25 +210,13 @@ def kv4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int) -> tupl
     return num_blocks, num_kv_heads, block_size // KV4_TILE, KV4_RECORD_BYTES
 
 
-def _kv4_pools(k_cache, v_cache, dev: int, what: str):
-    """(num_blocks, Hkv, block_size) of a layer's pools on device `dev`, checked."""
-    if not (_ok(k_cache, _U8, 4, dev) and _ok(v_cache, _U8, 4, dev) and _is_current(dev)):
-        _refuse(what, (k_cache, _U8, 4, "k_cache"), (v_cache, _U8, 4, "v_cache"))
-    shape = k_cache.shape
-    nb, hkv, tiles, rec = shape
-    if rec != KV4_RECORD_BYTES or v_cache.shape != shape:
-        raise ValueError(f"{what}: pools are {tuple(shape)} and {tuple(v_cache.shape)}, expected two of "
-                         f"[blocks, heads, block_size / {KV4_TILE}, {KV4_RECORD_BYTES}]")
-    return nb, hkv, tiles * KV4_TILE
-
-
 def _kv_rows(x, hkv: int, T: int, dev: int, what: str, name: str):
     """(row stride, head stride) in elements of bf16 rows [T, hkv, 128] or [T, hkv * 128]."""
-    shape, strides = tuple(x.shape), x.stride()
-    if (x.dtype is not BF16 or x.get_device() != dev or strides[-1] != 1
-            or (shape != (T, hkv, 128) and shape != (T, hkv * 128))):
+    shape, strides = x.shape, x.stride()
+    if not (x.dtype is BF16 and x.get_device() == dev and strides[-1] == 1
+            and (shape == (T, hkv, 128) or shape == (T, hkv * 128))):
         raise ValueError(f"{what}: {name} must be bf16 rows [{T}, {hkv}, 128] with contiguous dims on cuda:{dev}, got "
-                         f"{shape} {x.dtype} strides {strides} on {x.device}")
+                         f"{tuple(shape)} {x.dtype} strides {strides} on {x.device}")
     # a dimension of size 1 may carry any stride: it is never stepped over
     return strides[0] if T > 1 else 0, (strides[1] if len(shape) == 3 else 128) if hkv > 1 else 0
 
@@ -239,11 +227,16 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     flat slots of the 4-bit pools (see kv4_cache_shape); negative slots skip,
     the others must be distinct."""
     what = "kv4_store"
-    dev = k_cache.get_device()
-    nb, hkv, bs = _kv4_pools(k_cache, v_cache, dev, what)
-    if not _ok(slot_mapping, _I64, 1, dev):
-        _refuse(what, (slot_mapping, _I64, 1, "slot_mapping"))
-    T = slot_mapping.shape[0]
+    dev, pool, n = k_cache.get_device(), k_cache.shape, slot_mapping.shape
+    if not (k_cache.dtype is _U8 and v_cache.dtype is _U8 and v_cache.shape == pool and len(pool) == 4
+            and pool[3] == KV4_RECORD_BYTES and slot_mapping.dtype is _I64 and len(n) == 1
+            and dev >= 0 and dev == _current_device() and v_cache.get_device() == dev
+            and slot_mapping.get_device() == dev and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and slot_mapping.is_contiguous()):
+        _refuse(what, (k_cache, _U8, 4, "k_cache"), (v_cache, _U8, 4, "v_cache"),
+                (slot_mapping, _I64, 1, "slot_mapping"))
+    nb, hkv, tiles, _ = pool
+    bs, T = tiles * KV4_TILE, n[0]
     ks, kh = _kv_rows(k, hkv, T, dev, what, "k")
     vs, vh = _kv_rows(v, hkv, T, dev, what, "v")
     rc = _lib.load().aacc_kv4_store(k.data_ptr(), v.data_ptr(), T, ks, kh, vs, vh, slot_mapping.data_ptr(),
@@ -260,21 +253,26 @@ def kv4_load(k_cache, v_cache, slots, k_out=None, v_out=None, *, out_slots=None)
     Returns (k_out, v_out); outputs made here are zero where a token is
     skipped."""
     what = "kv4_load"
-    dev = k_cache.get_device()
-    nb, hkv, bs = _kv4_pools(k_cache, v_cache, dev, what)
-    if not _ok(slots, _I64, 1, dev):
-        _refuse(what, (slots, _I64, 1, "slots"))
-    T = slots.shape[0]
-    if out_slots is not None and not (_ok(out_slots, _I64, 1, dev) and out_slots.shape[0] == T):
-        _refuse(what, (out_slots, _I64, 1, "out_slots"), (slots, _I64, 1, "slots"))
+    dev, pool, n = k_cache.get_device(), k_cache.shape, slots.shape
+    if not (k_cache.dtype is _U8 and v_cache.dtype is _U8 and v_cache.shape == pool and len(pool) == 4
+            and pool[3] == KV4_RECORD_BYTES and slots.dtype is _I64 and len(n) == 1
+            and dev >= 0 and dev == _current_device() and v_cache.get_device() == dev and slots.get_device() == dev
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and slots.is_contiguous()
+            and (out_slots is None or (out_slots.dtype is _I64 and out_slots.shape == n
+                                       and out_slots.get_device() == dev and out_slots.is_contiguous()))):
+        _refuse(what, (k_cache, _U8, 4, "k_cache"), (v_cache, _U8, 4, "v_cache"), (slots, _I64, 1, "slots"),
+                *(() if out_slots is None else ((out_slots, _I64, 1, "out_slots"),)))
+    nb, hkv, tiles, _ = pool
+    bs, T = tiles * KV4_TILE, n[0]
     if k_out is None or v_out is None:
         if out_slots is not None or k_out is not None or v_out is not None:
             raise ValueError(f"{what}: give both k_out and v_out (or neither and no out_slots)")
         k_out, v_out = torch.zeros((2, T, hkv, 128), dtype=BF16, device=k_cache.device)
     shape = k_out.shape
     ndim = len(shape)
-    if not (_ok(k_out, BF16, ndim, dev) and _ok(v_out, BF16, ndim, dev) and v_out.shape == shape
-            and (ndim == 3 or ndim == 4) and shape[1] == hkv and shape[-1] == 128):
+    if not (k_out.dtype is BF16 and v_out.dtype is BF16 and v_out.shape == shape and (ndim == 3 or ndim == 4)
+            and shape[1] == hkv and shape[-1] == 128 and k_out.get_device() == dev and v_out.get_device() == dev
+            and k_out.is_contiguous() and v_out.is_contiguous()):
         _refuse(f"{what} (outputs [rows, {hkv}, 128] or [blocks, {hkv}, block_size, 128])",
                 (k_out, BF16, ndim, "k_out"), (v_out, BF16, ndim, "v_out"))
     rc = _lib.load().aacc_kv4_load(k_cache.data_ptr(), v_cache.data_ptr(), nb, hkv, bs, slots.data_ptr(),
@@ -296,21 +294,28 @@ def kv4_decode_attention(q, k_cache, v_cache, block_tables, rows, seqlens, *, ct
     tokens of the 4-bit pools (paged_decode_attention over the bf16 cache).
     Calls that share `workspace` (uint8) must be ordered on one stream."""
     what = "kv4_decode_attention"
-    dev = k_cache.get_device()
-    nb, hkv, bs = _kv4_pools(k_cache, v_cache, dev, what)
     if out is None:
         out = torch.empty_like(q)
-    if not (q.dtype is BF16 and _ok(block_tables, _I32, 2, dev) and _ok(rows, _I64, 1, dev)
-            and _ok(seqlens, _I32, 1, dev) and _ok(workspace, _U8, 1, dev) and q.is_contiguous()
-            and q.get_device() == dev and _ok(out, BF16, 3, dev) and out.shape == q.shape
-            and rows.shape[0] == q.shape[0] and q.shape[2] == 128 and seqlens.shape[0] == block_tables.shape[0]):
-        _refuse(what, (q, BF16, 3, "q"), (block_tables, _I32, 2, "block_tables"), (rows, _I64, 1, "rows"),
-                (seqlens, _I32, 1, "seqlens"), (workspace, _U8, 1, "workspace"), (out, BF16, 3, "out"))
-    B, hq, _ = q.shape
-    num_rows, max_blocks = block_tables.shape
+    dev, shape, pool, bt = q.get_device(), q.shape, k_cache.shape, block_tables.shape
+    if not (q.dtype is BF16 and out.dtype is BF16 and out.shape == shape and len(shape) == 3 and shape[2] == 128
+            and k_cache.dtype is _U8 and v_cache.dtype is _U8 and v_cache.shape == pool and len(pool) == 4
+            and pool[3] == KV4_RECORD_BYTES and block_tables.dtype is _I32 and len(bt) == 2
+            and rows.dtype is _I64 and rows.shape == shape[:1] and seqlens.dtype is _I32 and seqlens.shape == bt[:1]
+            and workspace is not None and workspace.dtype is _U8 and dev >= 0 and dev == _current_device() and out.get_device() == dev
+            and k_cache.get_device() == dev and v_cache.get_device() == dev and block_tables.get_device() == dev
+            and rows.get_device() == dev and seqlens.get_device() == dev and workspace.get_device() == dev
+            and q.is_contiguous() and out.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and block_tables.is_contiguous() and rows.is_contiguous() and seqlens.is_contiguous()
+            and workspace.is_contiguous()):
+        _refuse(what, (q, BF16, 3, "q"), (k_cache, _U8, 4, "k_cache"), (v_cache, _U8, 4, "v_cache"),
+                (block_tables, _I32, 2, "block_tables"), (rows, _I64, 1, "rows"), (seqlens, _I32, 1, "seqlens"),
+                (workspace, _U8, 1, "workspace"), (out, BF16, 3, "out"))
+    B, hq, _ = shape
+    nb, hkv, tiles, _ = pool
+    num_rows, max_blocks = bt
     rc = _lib.load().aacc_kv4_decode_attention(
         q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), nb, block_tables.data_ptr(), num_rows,
-        max_blocks, rows.data_ptr(), seqlens.data_ptr(), ctx_add, B, hq, hkv, bs, scale, max_context,
+        max_blocks, rows.data_ptr(), seqlens.data_ptr(), ctx_add, B, hq, hkv, tiles * KV4_TILE, scale, max_context,
         workspace.data_ptr(), workspace.numel(), _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
