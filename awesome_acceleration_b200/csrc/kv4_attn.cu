@@ -52,7 +52,8 @@ namespace aacc {
 constexpr int kAttWarps = 8;
 constexpr int kSizes = 4;   // team sizes: 1, 2, 4, 8 warps
 constexpr int kStages = 2;  // tiles of K and V that a warp has in hand or in flight
-constexpr int kAttThreads = kAttWarps * 32;
+constexpr int kAttThreads = 2 * kAttWarps * 32;  // as many warps again load
+constexpr int kPlanWarps = kAttThreads / 32;
 
 // A run of tiles [t0, t1) of item (b, h), whose row has n tiles; u is the unit number of t0.
 struct Kv4Seg {
@@ -70,12 +71,11 @@ struct Kv4Smem {
   uint32_t first_u[kAttWarps];  // and the unit that row starts at
   int row[kAttThreads];       // of batches up to kAttThreads rows
   int ctx[kAttThreads];
-  uint32_t wsum[kSizes + 1][kAttWarps];
+  uint32_t wsum[kSizes + 1][kPlanWarps];
   uint32_t sum[kSizes + 1];
   uint32_t plan[3];  // log2 T, units, units per run
   uint64_t full[kAttWarps][kStages];
-  Kv4Seg ahead[kAttWarps];  // where each warp's loads are: segment, and
-  int ahead_t[kAttWarps];          // its next tile there that is not in the warp's list
+  uint64_t empty[kAttWarps][kStages];
   uint32_t merge_k[kAttWarps][2];  // per team and shared item: first run, and
   int merge_n[kAttWarps][2];       // the number of runs if this one came last, else 0
   int abort;
@@ -337,8 +337,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   Kv4Smem<G>& sm = *reinterpret_cast<Kv4Smem<G>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&sm.full[warp][i], 1);
+  if (lane == 0 && warp < kAttWarps) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[warp][i], 1);
+      mbar_init(&sm.empty[warp][i], 1);
+    }
     fence_mbar_init();
   }
   if (threadIdx.x <= kSizes) sm.sum[threadIdx.x] = 0;
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       if (lane >= d) inc += y;
     }
     // The thread whose rows hold a team's first unit tells it where they start.
-    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.wsum[tsh][lane % kAttWarps] : 0);  // of warps with rows
+    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.wsum[tsh][lane % kPlanWarps] : 0);  // of warps with rows
     const uint32_t s0 = (before + inc - mine) * a.Hkv, s1 = s0 + mine * a.Hkv;
     if (mine)
       for (int i = 0; i < kAttWarps >> tsh; ++i) {
@@ -422,64 +425,75 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   __syncthreads();
 
   // ---- this team's run of units
-  const int team = warp >> tsh, wt = warp & ((1 << tsh) - 1), T = 1 << tsh;
+  const int wc = warp % kAttWarps;  // the consumer warp that this one is, or loads for
+  const int team = wc >> tsh, wt = wc & ((1 << tsh) - 1), T = 1 << tsh;
   const uint32_t k = (uint32_t)team * gridDim.x + blockIdx.x;  // runs go round the SMs: few runs use many of them
   const uint32_t u0 = min(k * chunk, N), uend = min(u0 + chunk, N);
   volatile int* abort = &sm.abort;
+  Kv4Seg cs;
+  if (u0 < uend) {
+    uint32_t u = sm.first_u[team];
+    cs.b = sm.first_b[team];
+    kv4_row(a, sm, cs);
+    uint32_t rounds = (uint32_t)(cs.n + T - 1) >> tsh;
+    while (u + rounds * a.Hkv <= u0) {
+      u += rounds * a.Hkv;
+      ++cs.b;
+      kv4_row(a, sm, cs);
+      rounds = (uint32_t)(cs.n + T - 1) >> tsh;
+    }
+    cs.u = u0;
+    cs.h = (int)((u0 - u) / rounds);
+    cs.t0 = (int)((u0 - u) - (uint32_t)cs.h * rounds) << tsh;
+    cs.t1 = seg_end(cs.n, cs.t0, uend - u0, tsh);
+  }
+
+  if (warp >= kAttWarps) {
+    // ---- a loading warp: the tiles of its consumer, in order, up to kStages ahead.  It lists up to 32 of them at
+    // a time, a tile per lane: the block ids arrive together.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (u0 >= uend) return;
+    uint32_t issued = 0;
+    bool ok = true, more = true;
+    int t = cs.t0 + wt;
+    while (ok && more) {
+      const int n = min(32, (cs.t1 - t + T - 1) >> tsh);  // <= 0: no tile of this segment for this warp
+      if (n > 0) {
+        const int my = min(t + (lane << tsh), cs.t1 - 1), bi = my / a.tpb;
+        uint32_t rec = (uint32_t)a.bt[cs.row * a.max_blocks + bi];
+        if (rec >= (uint32_t)a.num_blocks) {
+          report(a.err, ERR_BLOCK_OOB);
+          rec = 0;  // a valid address keeps the pipeline going; the result is flagged
+        }
+        rec = (rec * (uint32_t)a.Hkv + (uint32_t)cs.h) * (uint32_t)a.tpb + (uint32_t)(my - bi * a.tpb);
+        for (int i = 0; ok && i < n; ++i, ++issued) {
+          const uint32_t st = issued % kStages;
+          const int64_t at = (int64_t)__shfl_sync(0xffffffffu, rec, i) * kKv4Record;
+          if (issued >= kStages) ok = warp_wait(&sm.empty[wc][st], (issued / kStages - 1) & 1, a.err, abort);
+          if (!ok) break;
+          if (lane == 0) {
+            uint64_t* bar = &sm.full[wc][st];
+            mbar_arrive_expect_tx(bar, 2 * kKv4Record);
+            bulk_load(sm.kv[wc][st][0], a.kc + at, kKv4Record, bar);
+            bulk_load(sm.kv[wc][st][1], a.vc + at, kKv4Record, bar);
+          }
+          __syncwarp();
+        }
+        t += n << tsh;
+      }
+      if (ok && t >= cs.t1) {
+        more = kv4_next(a, sm, cs, uend, tsh);
+        t = cs.t0 + wt;
+      }
+    }
+    // Every copy has landed (or has run out of time) before the warp, and with it the CTA, may end.
+    for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+      mbar_wait(&sm.full[wc][i % kStages], i / kStages & 1, a.err, nullptr);
+    return;
+  }
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
 
   if (u0 < uend) {
-    Kv4Seg cs;
-    {
-      uint32_t u = sm.first_u[team];
-      cs.b = sm.first_b[team];
-      kv4_row(a, sm, cs);
-      uint32_t rounds = (uint32_t)(cs.n + T - 1) >> tsh;
-      while (u + rounds * a.Hkv <= u0) {
-        u += rounds * a.Hkv;
-        ++cs.b;
-        kv4_row(a, sm, cs);
-        rounds = (uint32_t)(cs.n + T - 1) >> tsh;
-      }
-      cs.u = u0;
-      cs.h = (int)((u0 - u) / rounds);
-      cs.t0 = (int)((u0 - u) - (uint32_t)cs.h * rounds) << tsh;
-      cs.t1 = seg_end(cs.n, cs.t0, uend - u0, tsh);
-    }
-    // The loads run one tile ahead of the arithmetic, across segments.  The warp lists up to 32 of its tiles
-    // at a time, a tile per lane: block id `ids` and, within the block's records, `sub`; entry li of ln is next.
-    // The segment they come from rests in shared memory.
-    sm.ahead[warp] = cs;
-    sm.ahead_t[warp] = cs.t0 + wt;
-    __syncwarp();
-    int32_t ids = 0;
-    int sub = 0, li = 0, ln = 0;
-    auto list_tiles = [&]() {
-      Kv4Seg s = sm.ahead[warp];
-      int t = sm.ahead_t[warp];
-      li = 0;
-      ln = 0;
-      while (t >= s.t1) {
-        if (!kv4_next(a, sm, s, uend, tsh)) return;
-        t = s.t0 + wt;
-      }
-      ln = min(32, (s.t1 - t + T - 1) >> tsh);
-      const int mine = min(t + (lane << tsh), s.t1 - 1), bi = mine / a.tpb;
-      ids = a.bt[s.row * a.max_blocks + bi];
-      sub = s.h * a.tpb + (mine - bi * a.tpb);
-      __syncwarp();
-      sm.ahead[warp] = s;
-      sm.ahead_t[warp] = t + (ln << tsh);
-      __syncwarp();
-    };
-    auto record = [&]() -> int64_t {
-      int32_t id = __shfl_sync(0xffffffffu, ids, li);
-      const int at = __shfl_sync(0xffffffffu, sub, li);
-      if ((uint32_t)id >= (uint32_t)a.num_blocks) {
-        if (lane == 0) report(a.err, ERR_BLOCK_OOB);
-        id = 0;  // a valid address keeps the pipeline going; the result is flagged
-      }
-      return ((int64_t)id * (a.Hkv * a.tpb) + at) * kKv4Record;
-    };
     // Queries of a segment: raw, as loaded; head g's dims 32 w + 8 c .. + 7.
     uint4 xq[4];
     auto load_q = [&](const Kv4Seg& s) {
@@ -489,22 +503,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
                       : make_uint4(0, 0, 0, 0);
     };
     load_q(cs);
-    list_tiles();
-    uint32_t issued = 0, used = 0;  // tiles; tile i lies in stage i % kStages
-    bool dead = false;              // a copy did not come in time: no more loads, no more tiles
-    auto issue = [&]() {            // the list's next tile, if there is one, into the next stage
-      if (li == ln) return;
-      const int64_t rec = record();
-      const uint32_t st = issued++ % kStages;
-      if (lane == 0) {
-        uint64_t* bar = &sm.full[warp][st];
-        mbar_arrive_expect_tx(bar, 2 * kKv4Record);
-        bulk_load(sm.kv[warp][st][0], a.kc + rec, kKv4Record, bar);
-        bulk_load(sm.kv[warp][st][1], a.vc + rec, kKv4Record, bar);
-      }
-      if (++li == ln) list_tiles();  // the next block ids are on their way while a tile is worked on
-    };
-    for (int i = 0; i < kStages; ++i) issue();
+    uint32_t used = 0;  // tiles; tile i lies in stage i % kStages
+    bool dead = false;  // a copy did not come in time: no more tiles
 
     // Items that this run holds a part of, not the whole: first query head, first and last unit.
     int parts = 0;
@@ -565,7 +565,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         const uint32_t st = used % kStages;
         if (!warp_wait(&sm.full[warp][st], used / kStages & 1, a.err, abort)) {
           dead = true;
-          li = ln = 0;
           break;
         }
         ++used;
@@ -723,7 +722,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
           group(std::integral_constant<int, 3>{});
         }
         __syncwarp();  // every lane has read the stage
-        issue();
+        if (lane == 0) mbar_arrive(&sm.empty[warp][st]);
       }
 
       // ---- end of the segment: the team's warps meet in shared memory
@@ -818,8 +817,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         });
       }
     }
-    if (dead)  // copies in flight land (or run out of time once more) before the CTA ends
-      for (; (int)(issued - used) > 0; ++used) mbar_wait(&sm.full[warp][used % kStages], used / kStages & 1, a.err, nullptr);
   }
 
   // ---- rows without tokens are zero
