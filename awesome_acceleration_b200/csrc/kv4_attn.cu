@@ -294,6 +294,12 @@ __device__ __forceinline__ void kv4_combine(int count, int lane, ML ml, OF o, fl
     const int n = min(GS, count - p0);
     float2 x = make_float2(-INFINITY, 0.f);
     if (gl < n) x = ml(p0 + gl);
+    constexpr int kAhead = VW == 1 ? 0 : 2;  // parts whose O sets out with the weights
+    float y0[2][VW];
+    if (kAhead) {
+      o(p0, y0[0]);
+      o(p0 + min(1, n - 1), y0[1]);
+    }
     float top = x.x;
 #pragma unroll
     for (int d = 1; d < GS; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -307,8 +313,13 @@ __device__ __forceinline__ void kv4_combine(int count, int lane, ML ml, OF o, fl
     L = L * keep + l;
 #pragma unroll
     for (int i = 0; i < VW; ++i) O[i] *= keep;
+    if (kAhead) {
+      const float w0 = __shfl_sync(0xffffffffu, f, g0), w1 = __shfl_sync(0xffffffffu, f, g0 + 1);
+#pragma unroll
+      for (int i = 0; i < VW; ++i) O[i] = fmaf(w0, y0[0][i], n > 1 ? fmaf(w1, y0[1][i], O[i]) : O[i]);
+    }
 #pragma unroll(VW == 1 ? 16 : 32 / VW)
-    for (int p = 0; p < n; ++p) {
+    for (int p = kAhead; p < n; ++p) {
       const float w = __shfl_sync(0xffffffffu, f, g0 + p);
       float y[VW];
       o(p0 + p, y);
@@ -863,12 +874,6 @@ int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, con
   if (G != 1 && G != 2 && G != 4 && G != 8)
     return set_error(AACC_ERR_UNSUPPORTED, "kv4_decode_attention: q/kv head ratio %d not in {1,2,4,8}", G);
   if (batch == 0) return AACC_OK;
-  if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
-    return set_error(AACC_ERR_INVALID, "kv4_decode_attention: pointers must be 16-byte aligned");
-  const int64_t need = aacc_kv4_decode_workspace_bytes(num_q_heads, num_kv_heads);
-  if (!workspace || workspace_bytes < need)
-    return set_error(AACC_ERR_INVALID, "kv4_decode_attention: workspace %lld < %lld bytes", (long long)workspace_bytes,
-                     (long long)need);
   if (max_context > max_blocks * block_size) max_context = max_blocks * block_size;
   if (max_context > 0x7fffffc0) max_context = 0x7fffffc0;
   // Units are counted in 32 bits.
@@ -876,6 +881,14 @@ int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, con
       (double)batch * num_kv_heads * (double)((max_context + kKv4Tile - 1) / kKv4Tile) > 2147483647.0)
     return set_error(AACC_ERR_UNSUPPORTED, "kv4_decode_attention: %lld rows of up to %lld tokens are too many",
                      (long long)batch, (long long)max_context);
+  if (!q || !out || !k_cache || !v_cache || !block_tables || !slot_indices || !seqlens)
+    return set_error(AACC_ERR_INVALID, "kv4_decode_attention: null pointer");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
+    return set_error(AACC_ERR_INVALID, "kv4_decode_attention: pointers must be 16-byte aligned");
+  const int64_t need = aacc_kv4_decode_workspace_bytes(num_q_heads, num_kv_heads);
+  if (!workspace || workspace_bytes < need)
+    return set_error(AACC_ERR_INVALID, "kv4_decode_attention: workspace %lld < %lld bytes", (long long)workspace_bytes,
+                     (long long)need);
   Kv4Args a;
   a.q = (const bf16*)q;
   a.out = (bf16*)out;

@@ -251,6 +251,7 @@ int aacc_kv4_store(const void* k, const void* v, int64_t num_tokens, int64_t k_r
   if (num_blocks > 0x7fffffff / block_size || num_tokens > 0x7fffffff / num_kv_heads)
     return set_error(AACC_ERR_UNSUPPORTED, "kv4_store: pool or token count too large");
   if (num_tokens == 0) return AACC_OK;
+  if (!k || !v || !slot_mapping || !k_cache || !v_cache) return set_error(AACC_ERR_INVALID, "kv4_store: null pointer");
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache) ||
       (k_row_stride | k_head_stride | v_row_stride | v_head_stride) % 8)
     return set_error(AACC_ERR_INVALID, "kv4_store: pointers/strides must be 16-byte aligned");
@@ -274,6 +275,8 @@ int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, 
       num_tokens > 0x7fffffff / num_kv_heads)
     return set_error(AACC_ERR_UNSUPPORTED, "kv4_load: pool or token count too large");
   if (num_tokens == 0) return AACC_OK;
+  if (!k_cache || !v_cache || !slots || !k_out || !v_out)
+    return set_error(AACC_ERR_INVALID, "kv4_load: null pointer");
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_out) || !aligned16(v_out))
     return set_error(AACC_ERR_INVALID, "kv4_load: pointers must be 16-byte aligned");
   const int hpw = kv4_heads_per_warp(num_tokens, num_kv_heads);

@@ -185,6 +185,7 @@ int aacc_build_block_tables(const int32_t* lengths, int64_t num_requests, int bl
   if (num_requests < 0 || num_requests > 0x7fffffff || block_size <= 0 || max_blocks <= 0 || num_free < 0)
     return set_error(AACC_ERR_INVALID, "build_block_tables: bad sizes");
   if (num_requests == 0) return AACC_OK;
+  if (!lengths || !block_tables) return set_error(AACC_ERR_INVALID, "build_block_tables: null pointer");
   // A CTA per SM at most twice over: each reads all the lengths before its own.
   const int64_t per = (num_requests + 2 * sm_count() - 1) / (2 * sm_count());
   return check_launch("build_block_tables",
@@ -200,6 +201,8 @@ int aacc_build_slot_maps(const int32_t* lengths, const int32_t* starts, const in
   if (num_requests < 0 || num_rows < 0 || max_blocks <= 0 || block_size <= 0 || num_blocks <= 0 || num_tokens < 0 ||
       num_tokens > 0x7fffffff)
     return set_error(AACC_ERR_INVALID, "build_slot_maps: bad sizes");
+  if (!cu_seqlens || (num_tokens > 0 && !slots) || (num_requests > 0 && (!lengths || !block_tables)))
+    return set_error(AACC_ERR_INVALID, "build_slot_maps: null pointer");
   const int64_t ctas = num_tokens > 0 ? (num_tokens + kMapTokens - 1) / kMapTokens : 1;
   return check_launch("build_slot_maps",
                       launch_k(build_slot_maps_kernel, dim3((unsigned)ctas), dim3(kMapThreads), 0, stream, lengths,

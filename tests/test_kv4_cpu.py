@@ -51,9 +51,10 @@ def test_c_abi_checks_arguments_before_any_cuda_call():
     lib = _lib.load()
     st = lib.aacc_kv4_store
 
-    def store(T=3, ks=256, kh=128, nb=2, hkv=2, bs=64, k=16):
-        return st(k, 16, T, ks, kh, 256, 128, 16, 16, 16, nb, hkv, bs, None)
-    for kw in (dict(T=-1), dict(nb=0), dict(hkv=0), dict(bs=0), dict(bs=96), dict(ks=100), dict(kh=127), dict(k=8)):
+    def store(T=3, ks=256, kh=128, nb=2, hkv=2, bs=64, k=16, slots=16):
+        return st(k, 16, T, ks, kh, 256, 128, slots, 16, 16, nb, hkv, bs, None)
+    for kw in (dict(T=-1), dict(nb=0), dict(hkv=0), dict(bs=0), dict(bs=96), dict(ks=100), dict(kh=127), dict(k=8),
+               dict(k=None), dict(slots=None)):
         assert store(**kw) == 1, kw
         assert b"kv4_store" in lib.aacc_last_error()
     assert store(T=2 ** 30, hkv=2) == 3 and store(nb=2 ** 25) == 3
@@ -61,7 +62,8 @@ def test_c_abi_checks_arguments_before_any_cuda_call():
 
     def load(T=3, nb=2, hkv=2, bs=64, ob=3, obs=1, k=16):
         return lib.aacc_kv4_load(k, 16, nb, hkv, bs, 16, None, T, 16, 16, ob, obs, None)
-    for kw in (dict(T=-1), dict(nb=0), dict(hkv=0), dict(bs=100), dict(ob=-1), dict(obs=0), dict(k=8)):
+    for kw in (dict(T=-1), dict(nb=0), dict(hkv=0), dict(bs=100), dict(ob=-1), dict(obs=0), dict(k=8),
+               dict(k=None)):
         assert load(**kw) == 1, kw
         assert b"kv4_load" in lib.aacc_last_error()
     assert load(T=2 ** 30, hkv=2) == 3 and load(nb=2 ** 25) == 3 and load(ob=2 ** 31) == 3
@@ -71,22 +73,24 @@ def test_c_abi_checks_arguments_before_any_cuda_call():
         return lib.aacc_kv4_decode_attention(q, 16, 16, 16, nb, 16, rows, mb, 16, 16, 1, B, hq, hkv, bs, 0.1, ctx, None,
                                              0, None)
     for kw in (dict(B=-1), dict(hkv=0), dict(hq=0), dict(hq=5), dict(bs=96), dict(bs=0), dict(nb=0), dict(mb=0),
-               dict(rows=-1), dict(ctx=0), dict(q=8)):
+               dict(rows=-1), dict(ctx=0), dict(q=8), dict(q=None)):
         assert attend(**kw) == 1, kw
         assert b"kv4_decode_attention" in lib.aacc_last_error()
     for hq in (6, 32):
         assert attend(hq=hq) == 3, hq  # 3 and 16 query heads per kv head
+    # units of work are counted in 32 bits
+    assert attend(B=2 ** 31) == 3 and attend(B=2 ** 26, mb=2 ** 10, ctx=2 ** 16) == 3
     assert attend(B=0) == 0
 
-    def tables(S=2, bs=64, nf=4, mb=2):
-        return lib.aacc_build_block_tables(16, S, bs, None, nf, 16, mb, None, None)
-    for kw in (dict(S=-1), dict(S=2 ** 31), dict(bs=0), dict(nf=-1), dict(mb=0)):
+    def tables(S=2, bs=64, nf=4, mb=2, lens=16):
+        return lib.aacc_build_block_tables(lens, S, bs, None, nf, 16, mb, None, None)
+    for kw in (dict(lens=None), dict(S=-1), dict(S=2 ** 31), dict(bs=0), dict(nf=-1), dict(mb=0)):
         assert tables(**kw) == 1, kw
     assert tables(S=0) == 0
 
-    def maps(S=2, nr=2, mb=2, bs=64, nb=2, T=4):
-        return lib.aacc_build_slot_maps(16, None, None, S, 16, nr, mb, bs, nb, 16, None, 16, T, None)
-    for kw in (dict(S=-1), dict(nr=-1), dict(mb=0), dict(bs=0), dict(nb=0), dict(T=-1), dict(T=2 ** 31)):
+    def maps(S=2, nr=2, mb=2, bs=64, nb=2, T=4, cu=16, slots=16):
+        return lib.aacc_build_slot_maps(16, None, None, S, 16, nr, mb, bs, nb, cu, None, slots, T, None)
+    for kw in (dict(cu=None), dict(slots=None), dict(S=-1), dict(nr=-1), dict(mb=0), dict(bs=0), dict(nb=0), dict(T=-1), dict(T=2 ** 31)):
         assert maps(**kw) == 1, kw
 
 

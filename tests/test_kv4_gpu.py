@@ -317,6 +317,21 @@ def test_decode_attention_few_and_many_rows(cuda, G, hkv, ctx):
     assert dev_err() == 0
 
 
+@pytest.mark.parametrize("B", [513, 1300])
+def test_decode_attention_batches_past_the_row_table(cuda, B):
+    """More rows than the kernel keeps in shared memory, padding and empty rows among them."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(1, 150, (B,), generator=g)
+    lens[::7] = 0
+    lens[1] = 1000
+    c = make_case([max(int(n), 1) for n in lens], 2, 1, 64, B)
+    rows = torch.arange(B)
+    rows[5::11] = -1
+    out = call(c, cuda, rows=rows, seqlens=lens.to(torch.int32), ctx_add=0)
+    check(out, c, ctx=[int(n) if r >= 0 else 0 for n, r in zip(lens, rows)])
+    assert dev_err() == 0
+
+
 def test_decode_attention_rows_padding_and_empty_contexts(cuda):
     c = make_case([5, 100, 64, 300, 1], 2, 2, 64, 4)
     order = torch.tensor([3, -1, 0, 2, -7, 1])          # rows permuted, two padding rows
