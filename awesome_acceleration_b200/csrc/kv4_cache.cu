@@ -32,12 +32,20 @@ struct Divide {
 };
 
 // Work of both kernels: a warp takes two tokens, lanes 0-15 the first and
-// 16-31 the second, and `hpw` heads of them, 8 dims a lane; the loads of
-// several heads are in flight together.  Two tokens that follow one another
-// share the 16-byte pieces of V's layout, so each store instruction fills
-// them whole.
-constexpr int kStoreHeads = 2;  // heads whose loads are issued together (registers: 8 a head)
-constexpr int kLoadHeads = 4;   // (4 a head)
+// 16-31 the second, and `hpw` heads of them, 8 dims a lane.  Two tokens that
+// follow one another share the 16-byte pieces of V's layout, so each store
+// instruction fills them whole.
+//
+// Measured, 32768 tokens of 8 heads (172 MB: 26.6 us at a copy's rate): store
+// 34 us (5.1 TB/s), load 30 us (5.8 TB/s).  The load is bound by memory.  The
+// store issues about 100 instructions per 8 values, in 70 % of all cycles,
+// and needs warps behind them: 48 of 40 registers, one head at a time, beat
+// 32 that load two heads together (37 us).  The load needs loads in flight:
+// four heads together (one: 33 us).  CTAs of 4 warps leave finer holes than 8
+// (35 and 30.5 us).
+constexpr int kLoadHeads = 4;
+constexpr int kMoveWarps = 4;
+constexpr int kMoveThreads = kMoveWarps * 32;
 
 struct Kv4Pair {
   int64_t t, rec0;  // token of this half warp; byte offset of its record for head 0
@@ -99,10 +107,12 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint4 x4, uint32_t (&code)[8]) 
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));  // 2^-126 <= s < 2^126: within 1 ulp
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = __uint_as_float((e & 1) ? x2[e >> 1] & 0xffff0000u : x2[e >> 1] << 16);
-      const float y = __fadd_rn(__fmaf_rn(x, r, 0x1.8p11f), -0x1.8p11f);
-      code[e] = __float_as_uint(__fadd_rn(y, 12582920.f));  // 1.5 * 2^23 + 8
+    for (int e = 0; e < 8; e += 2) {
+      const float2 y = __ffma2_rn(unpack_bf16(x2[e >> 1]), make_float2(r, r), make_float2(0x1.8p11f, 0x1.8p11f));
+      constexpr float kTo = 0x1.8p23f - 0x1.8p11f + 8.f;  // exact; the sum is rounded once, to an integer
+      const float2 z = __fadd2_rn(y, make_float2(kTo, kTo));
+      code[e] = __float_as_uint(z.x);
+      code[e + 1] = __float_as_uint(z.y);
     }
   } else {
 #pragma unroll
@@ -115,7 +125,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint4 x4, uint32_t (&code)[8]) 
   return sbits;
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kMoveThreads, 12)
     kv4_store_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t T, int64_t ks, int64_t kh,
                      int64_t vs, int64_t vh, const int64_t* __restrict__ slots, uint8_t* __restrict__ kc,
                      uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv, int hpw, Divide groups, Divide bs,
@@ -130,39 +140,38 @@ __global__ void __launch_bounds__(256)
   vc += p.rec0;
   k += p.t * ks + 8 * i;
   v += p.t * vs + 8 * i;
-  for (int h0 = p.h0; h0 < p.h1; h0 += kStoreHeads) {
-    uint4 xk[kStoreHeads], xv[kStoreHeads];
+  k += p.h0 * kh;
+  v += p.h0 * vh;
+  uint8_t* kw = kc + p.h0 * head_bytes + kv4_k_word(p.tt, i);
+  uint8_t* vw = vc + p.h0 * head_bytes + kv4_v_word(p.tt, i);
+  uint8_t* kq = kc + p.h0 * head_bytes + scale_at;
+  uint8_t* vq = vc + p.h0 * head_bytes + scale_at;
+#pragma unroll 1
+  for (int h = p.h0; h < p.h1; ++h, k += kh, v += vh) {
+    const uint4 xk = p.on ? *reinterpret_cast<const uint4*>(k) : make_uint4(0, 0, 0, 0);
+    const uint4 xv = p.on ? *reinterpret_cast<const uint4*>(v) : make_uint4(0, 0, 0, 0);
+    uint32_t code[8];
+    // sum_e code[e] 16^place(e) carries 0x4b400000 16^0..7 along: take it off at the end
+    constexpr uint32_t carried = 0x4b400000u * 0x11111111u;
+    const uint32_t sk = kv4_quantise(xk, code);
+    uint32_t w = 0;  // nibble n holds dim 8 i + 2 (n % 4) + n / 4
 #pragma unroll
-    for (int q = 0; q < kStoreHeads; ++q) {
-      const bool on = p.on && h0 + q < p.h1;
-      xk[q] = on ? *reinterpret_cast<const uint4*>(k + (h0 + q) * kh) : make_uint4(0, 0, 0, 0);
-      xv[q] = on ? *reinterpret_cast<const uint4*>(v + (h0 + q) * vh) : make_uint4(0, 0, 0, 0);
-    }
+    for (int n = 7; n >= 0; --n) w = w * 16 + code[2 * (n & 3) + (n >> 2)];
+    const uint32_t wk = w - carried;
+    const uint32_t sv = kv4_quantise(xv, code);
+    w = 0;  // byte b holds dims 8 i + 2 b and + 1
 #pragma unroll
-    for (int q = 0; q < kStoreHeads; ++q) {
-      const bool on = p.on && h0 + q < p.h1;
-      const int64_t rec = (h0 + q) * head_bytes;
-      uint32_t code[8];
-      // sum_e code[e] 16^place(e) carries 0x4b400000 16^0..7 along: take it off at the end
-      constexpr uint32_t carried = 0x4b400000u * 0x11111111u;
-      const uint32_t sk = kv4_quantise(xk[q], code);
-      uint32_t w = 0;  // nibble n holds dim 8 i + 2 (n % 4) + n / 4
-#pragma unroll
-      for (int n = 7; n >= 0; --n) w = w * 16 + code[2 * (n & 3) + (n >> 2)];
-      if (on) {
-        *reinterpret_cast<uint32_t*>(kc + rec + kv4_k_word(p.tt, i)) = w - carried;
-        if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(kc + rec + scale_at) = (uint16_t)sk;
-      }
-      const uint32_t sv = kv4_quantise(xv[q], code);
-      w = 0;  // byte b holds dims 8 i + 2 b and + 1
-#pragma unroll
-      for (int e = 7; e >= 0; --e) w = w * 16 + code[e];
-      w = transpose4(w - carried, lane);
-      if (on) {
-        *reinterpret_cast<uint32_t*>(vc + rec + kv4_v_word(p.tt, i)) = w;
-        if ((i & 3) == 0) *reinterpret_cast<uint16_t*>(vc + rec + scale_at) = (uint16_t)sv;
+    for (int e = 7; e >= 0; --e) w = w * 16 + code[e];
+    w = transpose4(w - carried, lane);
+    if (p.on) {
+      *reinterpret_cast<uint32_t*>(kw) = wk;
+      *reinterpret_cast<uint32_t*>(vw) = w;
+      if ((i & 3) == 0) {
+        *reinterpret_cast<uint16_t*>(kq) = (uint16_t)sk;
+        *reinterpret_cast<uint16_t*>(vq) = (uint16_t)sv;
       }
     }
+    kw += head_bytes, vw += head_bytes, kq += head_bytes, vq += head_bytes;
   }
 }
 
@@ -175,7 +184,7 @@ __device__ __forceinline__ uint32_t kv4_value(uint32_t x, uint32_t s) {
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kMoveThreads, 10)
     kv4_load_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, uint32_t num_slots, int Hkv,
                     int hpw, Divide groups, Divide bs, const int64_t* __restrict__ slots,
                     const int64_t* __restrict__ out_slots, int64_t T, bf16* __restrict__ ko, bf16* __restrict__ vo,
@@ -231,7 +240,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Heads a warp walks: as many as leave every SM its fill of warps (64).
+// Heads a warp walks, the slots looked up once for all: as many as leave every SM its fill of warps (64), up to 4.
+// At 32768 tokens and 8 heads, store and load: 1 head 47 and 54 us, 2 heads 39 and 36, 4 heads 35 and 30, 8 heads 36
+// and 30; at 32 tokens 4 heads a warp would leave most SMs without work.
 static int kv4_heads_per_warp(int64_t T, int Hkv) {
   const int64_t rows = (T + 1) / 2 * Hkv, want = (int64_t)sm_count() * 64;
   return (int)(rows <= want ? 1 : rows / want < 4 ? rows / want : 4);
@@ -258,7 +269,7 @@ int aacc_kv4_store(const void* k, const void* v, int64_t num_tokens, int64_t k_r
   const int hpw = kv4_heads_per_warp(num_tokens, num_kv_heads);
   const int64_t warps = (num_tokens + 1) / 2 * ((num_kv_heads + hpw - 1) / hpw);
   return check_launch("kv4_store",
-                      launch_k(kv4_store_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream,
+                      launch_k(kv4_store_kernel, dim3((unsigned)((warps + kMoveWarps - 1) / kMoveWarps)), dim3(kMoveThreads), 0, stream,
                                (const bf16*)k, (const bf16*)v, num_tokens, k_row_stride, k_head_stride, v_row_stride,
                                v_head_stride, slot_mapping, (uint8_t*)k_cache, (uint8_t*)v_cache,
                                (uint32_t)(num_blocks * block_size), num_kv_heads, hpw,
@@ -282,7 +293,7 @@ int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, 
   const int hpw = kv4_heads_per_warp(num_tokens, num_kv_heads);
   const int64_t warps = (num_tokens + 1) / 2 * ((num_kv_heads + hpw - 1) / hpw);
   return check_launch(
-      "kv4_load", launch_k(kv4_load_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream,
+      "kv4_load", launch_k(kv4_load_kernel, dim3((unsigned)((warps + kMoveWarps - 1) / kMoveWarps)), dim3(kMoveThreads), 0, stream,
                            (const uint8_t*)k_cache, (const uint8_t*)v_cache, (uint32_t)(num_blocks * block_size),
                            num_kv_heads, hpw, Divide((num_kv_heads + hpw - 1) / hpw), Divide(block_size), slots,
                            out_slots, num_tokens, (bf16*)k_out, (bf16*)v_out, (uint32_t)(out_blocks * out_block_size),
