@@ -27,6 +27,7 @@ import torch
 
 from .kv_cache import kv_cache_class
 from .model.model import Qwen3Config, Qwen3ForCausalLM
+from .runtime import Qwen3RuntimeKV4
 
 
 @dataclass
@@ -77,8 +78,10 @@ def kv_sized_max_seqs(config: Qwen3Config, max_num_seqs: int, max_seq_len: int, 
                // tp_size)
     q_cols = config.num_attention_heads * config.head_dim // tp_size
     act = prefill_chunk_tokens * (3 * config.hidden_size + 2 * q_cols + config.intermediate_size // tp_size) * 2
-    if kv_bits == 4:  # a chunk's bf16 K/V rows, and the bf16 context of its sequences (one layer)
-        act += (2 * prefill_chunk_tokens + max_seq_len) * 2 * config.num_key_value_heads * config.head_dim * 2 // tp_size
+    if kv_bits == 4:  # a chunk's bf16 K/V rows, and the bf16 context of its sequences in whole blocks (one layer)
+        blocks = min(max_num_seqs, prefill_chunk_tokens) * Qwen3RuntimeKV4.SCRATCH_BLOCK
+        act += ((2 * prefill_chunk_tokens + max_seq_len + blocks) * 2 * config.num_key_value_heads * config.head_dim * 2
+                // tp_size)
     reserve = reserve_gb * (1024 ** 3)
     avail = min(total - reserve, free - reserve - act)
     return max(1, min(max_num_seqs, int(avail / per_tok) // max_seq_len))

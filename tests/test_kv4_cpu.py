@@ -142,3 +142,22 @@ def test_runtime_of_either_width(monkeypatch):
     assert k.data_ptr() == rt._stage[0].data_ptr() and k.stride() == (256, 128, 1)
     rt._decode_attend(0, "q", "out", "rows")
     assert calls[2][0] == "kv4_decode_attention" and calls[2][1][:3] == ("q", "k0", "v0")
+
+
+def test_sizing_leaves_room_for_a_chunk_of_many_short_prompts(monkeypatch):
+    """A prefill chunk's scratch pool has a whole block for each sequence, however short."""
+    from awesome_acceleration_b200.llm import kv_sized_max_seqs
+    from awesome_acceleration_b200.model.model import Qwen3Config
+    from awesome_acceleration_b200.runtime import Qwen3RuntimeKV4
+    cfg = Qwen3Config(hidden_size=512, num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=4, head_dim=128,
+                      intermediate_size=1024, vocab_size=256)
+    free = 4 << 30
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    monkeypatch.setattr(torch.cuda, "empty_cache", lambda: None)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (free, 180 << 30))
+    chunk, seq, want = 4096, 1024, 4000
+    n = kv_sized_max_seqs(cfg, want, seq, 1.0, "cuda", 1, chunk, 4)
+    pool = n * seq * 4 * 144
+    scratch = n * Qwen3RuntimeKV4.SCRATCH_BLOCK * 4 * 128 * 2 * 2  # n prompts of one token in one chunk
+    rows = chunk * 4 * 128 * 2 * 2
+    assert 1 < n < want and pool + scratch + rows <= free - (1 << 30)
