@@ -494,7 +494,34 @@ def test_decode_attention_in_a_graph_and_on_another_stream(cuda):
     assert dev_err() == 0
 
 
+def test_decode_attention_on_two_streams_at_once(cuda):
+    """Calls in flight together, each with its own workspace, and one pool stored to by neither."""
+    cases = [make_case([4000, 3, 700] * 5, 2, 8, 64, 60), make_case([9000, 130], 8, 8, 64, 61)]
+    dev = [{x: c[x].to(cuda) for x in ("q", "kp", "vp", "bt")} for c in cases]
+    lens = [torch.tensor(c["ctx"], dtype=torch.int32, device=cuda) for c in cases]
+    rows = [torch.arange(len(c["ctx"]), device=cuda) for c in cases]
+    ws, outs = [workspace(c, cuda) for c in cases], [torch.empty_like(d["q"]) for d in dev]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                K().kv4_decode_attention(dev[i]["q"], dev[i]["kp"], dev[i]["vp"], dev[i]["bt"], rows[i], lens[i],
+                                         ctx_add=0, scale=SCALE, max_context=c["bt"].shape[1] * 64, workspace=ws[i],
+                                         out=outs[i])
+    torch.cuda.synchronize()
+    for c, out in zip(cases, outs):
+        check(out, c)
+    assert dev_err() == 0
+
+
 # --------------------------------------------------------------------------- request maps
+def test_block_tables_of_no_request_take_no_block(cuda):
+    used = torch.full((1,), 9, dtype=torch.int32, device=cuda)
+    K().build_block_tables(torch.empty(0, dtype=torch.int32, device=cuda), 64, max_blocks=3, used=used)
+    assert used.item() == 0 and dev_err() == 0
+
+
 @pytest.mark.parametrize("lens,bs", [([0], 64), ([1], 64), ([64, 65, 0, 1, 128, 700], 64), ([256] * 300, 256),
                                      (list(range(0, 2600, 2)), 128)])
 def test_block_tables(cuda, lens, bs):
