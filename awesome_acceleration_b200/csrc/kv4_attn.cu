@@ -3,24 +3,35 @@
 //   out[b][h] = sum_t softmax_t(scale q.k_t) v_t,  k_t = s n (4 groups of 32 dims)
 //
 // The floor is 144 bytes per (token, kv head) from HBM.  At that rate an SM
-// has about 400 cycles per 64 tokens, so the expansion of the codes has to
-// stay near one instruction a value, and there is no time for barriers.
+// has about 400 cycles per 64 tokens, in which it expands 16384 codes: that,
+// not the memory, is what bounds the kernel (with the arithmetic taken out
+// 256 rows take 110 us instead of 130).
 //
-// Work: the kernel is persistent, one CTA of 16 warps per SM, grouped into
-// teams of T = 1, 2, 4, 8 or 16 warps.  An item is one (row, kv head), a unit
-// a round of T tiles of 64 tokens of an item, one for each warp of a team.
-// Every CTA counts the batch's units itself from seqlens and takes the T of
-// the least estimated time (large T: few partials to merge; small T: no round
-// that is not full, no waiting); the units are cut into equal runs, one per
-// team, whatever the rows' lengths are.  A run that ends inside an item leaves an fp32 partial (max, sum, O);
-// the last team of the item to arrive merges the partials in order.
+// Measured (B200, bf16 q, floor at a copy's 6.45 TB/s): 256 rows of 512..4096
+// tokens at 16/8 heads 130 us (5.2 TB/s, floor 106); 256 of 1024..2047 at 64/8
+// heads 95 us (floor 71); 1 row of 40960 at 32/8 heads 21 us (floor 7.3), of
+// 333 6.5 us: a launch, the plan and the merge are about 6 us of each.
 //
-// Tiles: each warp streams its own tiles through one K and one V buffer with
-// bulk copies (lane 0 issues; the next K is fetched during softmax and P.V,
-// the next V during the next Q.K), so warps never wait for one another but at
-// the end of a team's item.  A tile is worked on in halves of 32 tokens, in a
-// rolled loop: straight-line code for whole tiles spent a fifth of a small
-// call on instruction fetches.
+// Work: the kernel is persistent, one CTA per SM of 8 warps that compute and 8
+// that load, grouped into teams of T = 1, 2, 4 or 8.  An item is one (row, kv
+// head), a unit a round of T tiles of 64 tokens of an item, one for each warp
+// of a team.  Every CTA counts the batch's units itself from seqlens and takes
+// the T of the least estimated time (large T: few partials to merge; small T:
+// no round that is not full, no waiting); the units are cut into equal runs,
+// one per team, whatever the rows' lengths are.  A run that ends inside an
+// item leaves an fp32 partial (max, sum, O); the last team of the item to
+// arrive merges the partials in order.
+//
+// Tiles: each computing warp has a loading warp and two stages of a K and a V
+// record, filled by bulk copies: warps never wait for one another but at the
+// end of a team's item.  The tiles' block ids are fetched by the loading
+// warps, 32 at a time; with their registers handed over (216 and 40 of the 128
+// at launch) the whole tile is straight-line code without spills.  Instead of
+// this: 16 warps that load for themselves and work on halves of a tile in a
+// rolled loop, 141 us; 8 that load for themselves 138; 12 that compute and 4
+// that load, one buffer each for K and V, 160; a third stage changes nothing;
+// Q.K of the next tile between P.V of this one 156.  Cycles of a warp per
+// tile: Q.K 1170, P.V 1135, softmax 490, scales 210, waiting for copies 180.
 //
 // Q.K: the tokens are the rows of m16n8k16's A operand, the G <= 8 query heads
 // its 8 columns.  With all else masked off, four bits at the foot of an fp16
@@ -422,7 +433,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       if (lane >= d) inc += y;
     }
     // The thread whose rows hold a team's first unit tells it where they start.
-    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.wsum[tsh][lane % kPlanWarps] : 0);  // of warps with rows
+    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.wsum[tsh][lane % kPlanWarps] : 0);
     const uint32_t s0 = (before + inc - mine) * a.Hkv, s1 = s0 + mine * a.Hkv;
     if (mine)
       for (int i = 0; i < kAttWarps >> tsh; ++i) {
@@ -510,7 +521,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     auto load_q = [&](const Kv4Seg& s) {
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        xq[w] = g < G ? *reinterpret_cast<const uint4*>(a.q + (((int64_t)s.b * a.Hkv + s.h) * G + g) * 128 + 32 * w + 8 * c)
+        xq[w] = g < G ? *reinterpret_cast<const uint4*>(a.q + (((int64_t)s.b * a.Hkv + s.h) * G + g) * 128 +
+                                                        32 * w + 8 * c)
                       : make_uint4(0, 0, 0, 0);
     };
     load_q(cs);
@@ -555,7 +567,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
             qf[w][r] = pack_f16(y.x * f16, y.y * f16);
             sum[w] += (y.x + y.y) * up;
           }
-        const float down = fabsf(a.scale) * (0x1p24f * kLog2e) * (f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23));
+        const float down = fabsf(a.scale) * (0x1p24f * kLog2e) *
+                           (f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23));
         sl0 = __shfl_sync(0xffffffffu, down, 8 * c);
         sl1 = __shfl_sync(0xffffffffu, down, 8 * c + 4);
 #pragma unroll

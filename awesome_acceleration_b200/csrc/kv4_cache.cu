@@ -268,8 +268,9 @@ int aacc_kv4_store(const void* k, const void* v, int64_t num_tokens, int64_t k_r
     return set_error(AACC_ERR_INVALID, "kv4_store: pointers/strides must be 16-byte aligned");
   const int hpw = kv4_heads_per_warp(num_tokens, num_kv_heads);
   const int64_t warps = (num_tokens + 1) / 2 * ((num_kv_heads + hpw - 1) / hpw);
+  const dim3 grid((unsigned)((warps + kMoveWarps - 1) / kMoveWarps));
   return check_launch("kv4_store",
-                      launch_k(kv4_store_kernel, dim3((unsigned)((warps + kMoveWarps - 1) / kMoveWarps)), dim3(kMoveThreads), 0, stream,
+                      launch_k(kv4_store_kernel, grid, dim3(kMoveThreads), 0, stream,
                                (const bf16*)k, (const bf16*)v, num_tokens, k_row_stride, k_head_stride, v_row_stride,
                                v_head_stride, slot_mapping, (uint8_t*)k_cache, (uint8_t*)v_cache,
                                (uint32_t)(num_blocks * block_size), num_kv_heads, hpw,
@@ -292,8 +293,9 @@ int aacc_kv4_load(const void* k_cache, const void* v_cache, int64_t num_blocks, 
     return set_error(AACC_ERR_INVALID, "kv4_load: pointers must be 16-byte aligned");
   const int hpw = kv4_heads_per_warp(num_tokens, num_kv_heads);
   const int64_t warps = (num_tokens + 1) / 2 * ((num_kv_heads + hpw - 1) / hpw);
+  const dim3 grid((unsigned)((warps + kMoveWarps - 1) / kMoveWarps));
   return check_launch(
-      "kv4_load", launch_k(kv4_load_kernel, dim3((unsigned)((warps + kMoveWarps - 1) / kMoveWarps)), dim3(kMoveThreads), 0, stream,
+      "kv4_load", launch_k(kv4_load_kernel, grid, dim3(kMoveThreads), 0, stream,
                            (const uint8_t*)k_cache, (const uint8_t*)v_cache, (uint32_t)(num_blocks * block_size),
                            num_kv_heads, hpw, Divide((num_kv_heads + hpw - 1) / hpw), Divide(block_size), slots,
                            out_slots, num_tokens, (bf16*)k_out, (bf16*)v_out, (uint32_t)(out_blocks * out_block_size),

@@ -301,8 +301,8 @@ def kv4_decode_attention(q, k_cache, v_cache, block_tables, rows, seqlens, *, ct
             and k_cache.dtype is _U8 and v_cache.dtype is _U8 and v_cache.shape == pool and len(pool) == 4
             and pool[3] == KV4_RECORD_BYTES and block_tables.dtype is _I32 and len(bt) == 2
             and rows.dtype is _I64 and rows.shape == shape[:1] and seqlens.dtype is _I32 and seqlens.shape == bt[:1]
-            and workspace is not None and workspace.dtype is _U8 and dev >= 0 and dev == _current_device() and out.get_device() == dev
-            and k_cache.get_device() == dev and v_cache.get_device() == dev and block_tables.get_device() == dev
+            and workspace is not None and workspace.dtype is _U8 and dev >= 0 and dev == _current_device()
+            and out.get_device() == dev and k_cache.get_device() == dev and v_cache.get_device() == dev and block_tables.get_device() == dev
             and rows.get_device() == dev and seqlens.get_device() == dev and workspace.get_device() == dev
             and q.is_contiguous() and out.is_contiguous() and k_cache.is_contiguous() and v_cache.is_contiguous()
             and block_tables.is_contiguous() and rows.is_contiguous() and seqlens.is_contiguous()
