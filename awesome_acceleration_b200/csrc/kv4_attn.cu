@@ -173,12 +173,12 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 
 // d = a b + c, where c holds for both rows of a column pair.
 __device__ __forceinline__ void mma_f16_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
-                                                   const float (&c)[2]) {
+                                                   float c0, float c1) {
   asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%11,%10,%11};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
@@ -516,14 +516,23 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
   asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
 
   if (u0 < uend) {
-    // Queries of a segment: raw, as loaded; head g's dims 32 w + 8 c .. + 7.
+    // The 8 columns of an MMA are kCols to a head.  A lane (g, c) looks at columns 2 c and 2 c + 1: with kCols = 1 it
+    // holds the scores of two heads for tokens g and g + 8 of 16, with 2 those of one head, and with 4 those of one
+    // head for one of the tokens (columns 4 h and 4 h + 2 are the same, so one lane takes g, its neighbour g + 8).
+    constexpr int kCols = G == 8 ? 1 : G == 4 ? 2 : 4;
+    constexpr int HV = kCols == 1 ? 2 : 1;  // heads per lane
+    constexpr int NV = 4 / kCols;           // scores per lane of 16 tokens: [token][head]
+    constexpr int kLow = kCols == 4 ? 1 : 4;  // a head's lanes: all g, and with kCols = 4 both of c / 2's
+    const int tok = kCols == 4 ? g + 8 * (c & 1) : g;  // the first's token; the second's is 8 further
+    // Queries of a segment: raw, as loaded; the dims 32 w + 8 c .. + 7 of the head of column g.
+    const int qh = g / kCols;
     uint4 xq[4];
     auto load_q = [&](const Kv4Seg& s) {
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        xq[w] = g < G ? *reinterpret_cast<const uint4*>(a.q + (((int64_t)s.b * a.Hkv + s.h) * G + g) * 128 +
-                                                        32 * w + 8 * c)
-                      : make_uint4(0, 0, 0, 0);
+        xq[w] = qh < G ? *reinterpret_cast<const uint4*>(a.q + (((int64_t)s.b * a.Hkv + s.h) * G + qh) * 128 +
+                                                         32 * w + 8 * c)
+                       : make_uint4(0, 0, 0, 0);
     };
     load_q(cs);
     uint32_t used = 0;  // tiles; tile i lies in stage i % kStages
@@ -535,11 +544,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     uint32_t part_first[2] = {0, 0}, part_last[2] = {0, 0};
 
     while (true) {
-      // ---- queries of the item: B operand, column g = query head (columns >= G are zero)
+      // ---- queries of the item: B operand (columns without a head are zero)
       const int64_t qh0 = ((int64_t)cs.b * a.Hkv + cs.h) * G;
       uint32_t qf[4][4];
-      float sl0, sl1;     // log2 softmax scale of the raw scores of heads 2c and 2c + 1
-      float corr[4][2];  // -8 times 2^-24 times the sum of their q over group w
+      float sl[HV];       // log2 softmax scale of the raw scores of this lane's heads
+      float corr[4][HV];  // -8 times 2^-24 times the sum of their q over group w
       {
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns q's sign
         uint32_t mx = 0;
@@ -569,20 +578,22 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
           }
         const float down = fabsf(a.scale) * (0x1p24f * kLog2e) *
                            (f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23));
-        sl0 = __shfl_sync(0xffffffffu, down, 8 * c);
-        sl1 = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+#pragma unroll
+        for (int e = 0; e < HV; ++e) sl[e] = __shfl_sync(0xffffffffu, down, 8 * c + 4 * e);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 1);
           sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], 2);
-          corr[w][0] = -0x1p-21f * __shfl_sync(0xffffffffu, sum[w], 8 * c);
-          corr[w][1] = -0x1p-21f * __shfl_sync(0xffffffffu, sum[w], 8 * c + 4);
+#pragma unroll
+          for (int e = 0; e < HV; ++e) corr[w][e] = -0x1p-21f * __shfl_sync(0xffffffffu, sum[w], 8 * c + 4 * e);
         }
       }
       float o[8][4];
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      float m[HV], l[HV];
+#pragma unroll
+      for (int e = 0; e < HV; ++e) m[e] = -INFINITY, l[e] = 0.f;
       int ev = 4;  // biased exponent of the largest V scale so far (at least 4): O is kept times 2^(131 - ev)
 
       for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += T) {
@@ -596,28 +607,30 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         const uint8_t* vb = sm.kv[warp][st][1];
         const int lim = cs.ctx - t * kKv4Tile;  // tokens from here to the end of the context
 
-        // ---- S = K Q^T; lane (g, c): tokens 16 sb + g (+ 8), heads 2c and 2c + 1
-        float s[4][4];
+        // ---- S = K Q^T
+        float s[4][NV];
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb) {
           const uint4 x4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + lane * 16);        // token g
           const uint4 y4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + 512 + lane * 16);  // token g + 8
-          const uint2 sx = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + g) * 8);
-          const uint2 sy = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + g + 8) * 8);
+          const uint2 sx = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + tok) * 8);
+          const uint2 sy = kCols == 4 ? sx : *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + tok + 8) * 8);
           auto group = [&](auto W, uint32_t x, uint32_t y) {
             constexpr int w = decltype(W)::value;
             float acc[4];
             const uint32_t a0[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
-            mma_f16_16816_from(acc, a0, qf[w][0], qf[w][1], corr[w]);
+            mma_f16_16816_from(acc, a0, qf[w][0], qf[w][1], corr[w][0], corr[w][HV - 1]);
             x >>= 8;
             y >>= 8;
             const uint32_t a1[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
             mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
             const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
-            s[sb][0] = w == 0 ? acc[0] * fx : fmaf(acc[0], fx, s[sb][0]);
-            s[sb][1] = w == 0 ? acc[1] * fx : fmaf(acc[1], fx, s[sb][1]);
-            s[sb][2] = w == 0 ? acc[2] * fy : fmaf(acc[2], fy, s[sb][2]);
-            s[sb][3] = w == 0 ? acc[3] * fy : fmaf(acc[3], fy, s[sb][3]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              const float v = kCols == 1 ? acc[i] : kCols == 2 ? acc[2 * i] : c & 1 ? acc[2] : acc[0];
+              const float f = i < HV ? fx : fy;
+              s[sb][i] = w == 0 ? v * f : fmaf(v, f, s[sb][i]);
+            }
           };
           group(std::integral_constant<int, 0>{}, x4.x, y4.x);
           group(std::integral_constant<int, 1>{}, x4.y, y4.y);
@@ -627,7 +640,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
 
         // ---- the tile's V scales as fp16 pairs; lane: tokens 2 lane and 2 lane + 1.  Behind the context a scale
         // may be anything: it becomes zero.  They are not negative: their bits order as they do.
-        float a0 = 1.f, a1 = 1.f;
+        float al[HV];
+#pragma unroll
+        for (int e = 0; e < HV; ++e) al[e] = 1.f;
         bool grow = false;
         {
           uint4 x = *(reinterpret_cast<const uint4*>(vb + kKv4Codes) + lane);
@@ -639,7 +654,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
                                    max(max(x.x << 16, x.y << 16), max(x.z << 16, x.w << 16)));
           const int e = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
           if (e > ev) {
-            a0 = a1 = ex2((float)(ev - e));
+#pragma unroll
+            for (int i = 0; i < HV; ++i) al[i] = ex2((float)(ev - e));
             ev = e;
             grow = true;
           }
@@ -654,77 +670,81 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         // ---- online softmax in the log2 domain
         if (lim < kKv4Tile) {
 #pragma unroll
-          for (int sb = 0; sb < 4; ++sb) {
-            if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = -INFINITY;
-            if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = -INFINITY;
-          }
+          for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+              if (16 * sb + tok + i / HV * 8 >= lim) s[sb][i] = -INFINITY;
         }
         // The reference of the exponentials follows the maximum only when a score passes it by 2^6: p stays
         // below 2^6, and most tiles need no shuffles and no rescaling.
-        float x0 = fmaxf(s[0][0], s[0][2]), x1 = fmaxf(s[0][1], s[0][3]);
+        float x[HV];
+        bool above = false;
 #pragma unroll
-        for (int sb = 1; sb < 4; ++sb) {
-          x0 = fmaxf(x0, fmaxf(s[sb][0], s[sb][2]));
-          x1 = fmaxf(x1, fmaxf(s[sb][1], s[sb][3]));
+        for (int e = 0; e < HV; ++e) {
+          x[e] = s[0][e];
+#pragma unroll
+          for (int i = 1; i < 4 * NV / HV; ++i) x[e] = fmaxf(x[e], s[i % 4][i / 4 * HV + e]);
+          x[e] *= sl[e];
+          above |= x[e] > m[e] + 6.f;
         }
-        x0 *= sl0;
-        x1 *= sl1;
-        if (__any_sync(0xffffffffu, x0 > m0 + 6.f || x1 > m1 + 6.f)) {
+        if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+          for (int e = 0; e < HV; ++e) {
+#pragma unroll
+            for (int d = kLow; d < 32; d += d == 1 ? 3 : d) x[e] = fmaxf(x[e], __shfl_xor_sync(0xffffffffu, x[e], d));
+            x[e] = fmaxf(m[e], x[e]);
+            const float f = ex2(m[e] - x[e]);
+            m[e] = x[e];
+            l[e] *= f;
+            al[e] *= f;
           }
-          x0 = fmaxf(m0, x0);
-          x1 = fmaxf(m1, x1);
-          const float f0 = ex2(m0 - x0), f1 = ex2(m1 - x1);
-          m0 = x0;
-          m1 = x1;
-          l0 *= f0;
-          l1 *= f1;
-          a0 *= f0;
-          a1 *= f1;
           grow = true;
         }
-        const float r0 = 4.f - m0, r1 = 4.f - m1;  // 2^4 p
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          s[sb][0] = ex2(fmaf(s[sb][0], sl0, r0));
-          s[sb][1] = ex2(fmaf(s[sb][1], sl1, r1));
-          s[sb][2] = ex2(fmaf(s[sb][2], sl0, r0));
-          s[sb][3] = ex2(fmaf(s[sb][3], sl1, r1));
-        }
+        for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+          for (int i = 0; i < NV; ++i) s[sb][i] = ex2(fmaf(s[sb][i], sl[i % HV], 4.f - m[i % HV]));  // 2^4 p
         if (lim < kKv4Tile) {  // also where a scale of 0 makes -inf * 0 a NaN
 #pragma unroll
-          for (int sb = 0; sb < 4; ++sb) {
-            if (16 * sb + g >= lim) s[sb][0] = s[sb][1] = 0.f;
-            if (16 * sb + g + 8 >= lim) s[sb][2] = s[sb][3] = 0.f;
-          }
+          for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+              if (16 * sb + tok + i / HV * 8 >= lim) s[sb][i] = 0.f;
         }
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          l0 += s[sb][0] + s[sb][2];
-          l1 += s[sb][1] + s[sb][3];
-        }
+        for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+          for (int i = 0; i < NV; ++i) l[i % HV] += s[sb][i];
         if (grow) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            o[j][0] *= a0;
-            o[j][1] *= a1;
-            o[j][2] *= a0;
-            o[j][3] *= a1;
-          }
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][i] *= al[i % HV];
         }
         __syncwarp();  // vpair is written
 
         // ---- O^T += V^T P^T
+        uint32_t pt = 0;
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb) {
           const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
           const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
           const uint4 sx = sm.vpair[warp][sb * 8 + c], sy = sm.vpair[warp][sb * 8 + 4 + c];
-          const uint32_t px = movmatrix_trans(pack_f16(s[sb][0], s[sb][1]));  // head g, tokens 2c, 2c + 1
-          const uint32_t py = movmatrix_trans(pack_f16(s[sb][2], s[sb][3]));  // ... + 8
+          uint32_t px, py;  // column g: its head's tokens 2c, 2c + 1 and ... + 8
+          if constexpr (kCols == 1) {
+            px = movmatrix_trans(pack_f16(s[sb][0], s[sb][1]));
+            py = movmatrix_trans(pack_f16(s[sb][NV - 2], s[sb][NV - 1]));
+          } else if constexpr (kCols == 2) {
+            // A head's even column takes tokens 0 .. 7, its odd one 8 .. 15: one transpose for both.
+            const uint32_t y = movmatrix_trans(pack_f16(s[sb][0], s[sb][NV - 1]));
+            px = g & 1 ? 0u : y;
+            py = g & 1 ? y : 0u;
+          } else {
+            // Columns 4 h and 4 h + 1 take tokens 0 .. 7 of even and of odd sb, + 2 and + 3 tokens 8 .. 15.
+            if (sb % 2 == 0) pt = movmatrix_trans(pack_f16(s[sb][0], s[(sb + 1) % 4][0]));
+            px = (g & 3) == sb % 2 ? pt : 0u;
+            py = (g & 3) == sb % 2 + 2 ? pt : 0u;
+          }
           auto group = [&](auto W) {  // 32 dims: j = 2w and 2w + 1
             constexpr int w = decltype(W)::value;
             const uint32_t b0 = mul_f16(px, w == 0 ? sx.x : w == 1 ? sx.y : w == 2 ? sx.z : sx.w);
@@ -753,22 +773,25 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       Kv4Seg nx = cs;
       const bool more = kv4_next(a, sm, nx, uend, tsh);
       if (more) load_q(nx);
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-      }
       const float down = __uint_as_float((uint32_t)(ev - 4) << 23) + (ev == 4 ? 0x1p-127f : 0.f);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // o[j][e], o[j][2 + e]: dims 16 j + 2g and + 1 of head 2c + e
-        const int hd = 2 * c + e;
-        if (hd < G) {
+      for (int e = 0; e < HV; ++e) {  // dims 16 j + 2g and + 1: o[j][e], o[j][2 + e], summed over a head's columns
+        const int hd = (2 * c + e) / kCols;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float2*>(&sm.red_o[warp][hd][16 * j + 2 * g]) =
-                make_float2(o[j][e] * down, o[j][2 + e] * down);
-          if (g == 0) *reinterpret_cast<float2*>(sm.red_ml[warp][hd]) = make_float2(e ? m1 : m0, e ? l1 : l0);
+        for (int d = kLow; d < 32; d += d == 1 ? 3 : d) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float y0 = o[j][e], y1 = o[j][2 + e];
+          if constexpr (kCols > 1) y0 += o[j][1], y1 += o[j][3];
+          if constexpr (kCols > 2) {
+            y0 += __shfl_xor_sync(0xffffffffu, y0, 1);
+            y1 += __shfl_xor_sync(0xffffffffu, y1, 1);
+          }
+          if (hd < G && (kCols < 4 || (c & 1) == (j & 1)))
+            *reinterpret_cast<float2*>(&sm.red_o[warp][hd][16 * j + 2 * g]) = make_float2(y0 * down, y1 * down);
         }
+        if (hd < G && g == 0 && (kCols < 4 || (c & 1) == 0))
+          *reinterpret_cast<float2*>(sm.red_ml[warp][hd]) = make_float2(m[e], l[e]);
       }
       team_sync(team, tsh);
       const bool whole = cs.t0 == 0 && cs.t1 == cs.n;
