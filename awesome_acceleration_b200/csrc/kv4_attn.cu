@@ -5,12 +5,13 @@
 // The floor is 144 bytes per (token, kv head) from HBM.  At that rate an SM
 // has about 400 cycles per 64 tokens, in which it expands 16384 codes: that,
 // not the memory, is what bounds the kernel (with the arithmetic taken out
-// 256 rows take 110 us instead of 130).
+// 256 rows take 110 us).
 //
 // Measured (B200, bf16 q, floor at a copy's 6.45 TB/s): 256 rows of 512..4096
-// tokens at 16/8 heads 130 us (5.2 TB/s, floor 106); 256 of 1024..2047 at 64/8
-// heads 95 us (floor 71); 1 row of 40960 at 32/8 heads 21 us (floor 7.3), of
-// 333 6.5 us: a launch, the plan and the merge are about 6 us of each.
+// tokens at 16/8 heads 120 to 130 us (up to 5.6 TB/s, floor 106); 256 of
+// 1024..2047 at 64/8 heads 95 us (floor 71); 40 of 1..3001 at 64/8 heads 27.5
+// us (floor 10); 1 row of 40960 at 32/8 heads 20 us (floor 7.3), of 333 at 16/8
+// 6.2 us: a launch, the plan and the merge are about 6 us of each.
 //
 // Work: the kernel is persistent, one CTA per SM of 8 warps that compute and 8
 // that load, grouped into teams of T = 1, 2, 4 or 8.  An item is one (row, kv
@@ -26,15 +27,18 @@
 // record, filled by bulk copies: warps never wait for one another but at the
 // end of a team's item.  The tiles' block ids are fetched by the loading
 // warps, 32 at a time; with their registers handed over (216 and 40 of the 128
-// at launch) the whole tile is straight-line code without spills.  Instead of
-// this: 16 warps that load for themselves and work on halves of a tile in a
-// rolled loop, 141 us; 8 that load for themselves 138; 12 that compute and 4
-// that load, one buffer each for K and V, 160; a third stage changes nothing;
-// Q.K of the next tile between P.V of this one 156.  Cycles of a warp per
-// tile: Q.K 1170, P.V 1135, softmax 490, scales 210, waiting for copies 180.
+// at launch) the whole tile is straight-line code without spills.  Where this
+// took 131 us for 256 rows, others took: 16 warps that load for themselves and
+// work on halves of a tile in a rolled loop 141; 8 that load for themselves
+// 138; 12 that compute and 4 that load, one buffer each for K and V, 160; a
+// third stage 131; Q.K of the next tile between P.V of this one 156.
 //
 // Q.K: the tokens are the rows of m16n8k16's A operand, the G <= 8 query heads
-// its 8 columns.  With all else masked off, four bits at the foot of an fp16
+// its 8 columns.  Fewer heads share the columns out: with a column each, a lane
+// would take the exponentials of two columns, empty or not, for all tokens
+// (256 rows at two heads 130 us, against 124 with four columns a head).  m16n8k32
+// on e4m3, where codes are operands as they are, is no way: it takes four times
+// as long as this one.  With all else masked off, four bits at the foot of an fp16
 // are the subnormal 2^-24 u, or 2^-20 u one nibble higher, and the tensor
 // cores take subnormals as they are: an AND makes two operands.  The 2^24 is
 // put right in the softmax scale, the 16 in q, and the offset of 8 through the
@@ -46,7 +50,7 @@
 // over thousands of tokens would cancel against its offset, so u - 8 is made
 // exactly, by one more fp16x2 add or fma.  P^T is 2^4 p in fp16 (the 2^4 also
 // in the sum it is divided by), p < 2^6, transposed in registers and multiplied
-// by the V scales of its two tokens in fp16: two roundings of 2^-12, a quarter
+// by the V scales of its two tokens in fp16: two roundings of 2^-11, a quarter
 // of what one to bf16 costs.  The scales are held relative to the largest so
 // far, at [2^4, 2^5): products reach 2^15, and a p down to 2^-18 and a scale
 // down to 2^-21 of the largest have no other rounding than those two.
@@ -240,54 +244,34 @@ __device__ __forceinline__ void team_sync(int team, int tsh) {
     asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(32 << tsh) : "memory");
 }
 
-// How a warp shares out sums of partial results: VW dims a lane, 4 or 1 at a time, so GS lanes to a head.
-// Several heads to a warp (VW 8, 16) have their loads in flight together; with VW 1 a warp takes 32 dims.
+// How a warp shares out sums of partial results: VW dims a lane, 4 at a time, so GS lanes to a head.
+// Several heads to a warp (VW 8, 16) have their loads in flight together.
 template <int VW>
 struct Kv4Share {
-  static constexpr int GS = VW == 1 ? 32 : 128 / VW;
-  static constexpr int P = VW == 1 ? 1 : VW / 4;  // pieces
-  int hd, d;                                      // head; the first piece's first dim
-  __device__ __forceinline__ Kv4Share(int i, int lane) {
-    if constexpr (VW == 1) {
-      hd = i >> 2;
-      d = (i & 3) * 32 + lane;
-    } else {
-      hd = i * (32 / GS) + lane / GS;
-      d = lane % GS * 4;
-    }
-  }
+  static constexpr int GS = 128 / VW;
+  static constexpr int P = VW / 4;  // pieces
+  int hd, d;                        // head; the first piece's first dim
+  __device__ __forceinline__ Kv4Share(int i, int lane) : hd(i * (32 / GS) + lane / GS), d(lane % GS * 4) {}
   template <class Load>
   __device__ __forceinline__ void read(const float* head, float (&y)[VW], Load load) const {
-    if constexpr (VW == 1) {
-      y[0] = load(head + d);
-    } else {
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const float4 v = load(reinterpret_cast<const float4*>(head + d + q * GS * 4));
-        y[4 * q] = v.x, y[4 * q + 1] = v.y, y[4 * q + 2] = v.z, y[4 * q + 3] = v.w;
-      }
+    for (int q = 0; q < P; ++q) {
+      const float4 v = load(reinterpret_cast<const float4*>(head + d + q * GS * 4));
+      y[4 * q] = v.x, y[4 * q + 1] = v.y, y[4 * q + 2] = v.z, y[4 * q + 3] = v.w;
     }
   }
   __device__ __forceinline__ void write(float* head, const float (&y)[VW]) const {
-    if constexpr (VW == 1) {
-      head[d] = y[0];
-    } else {
 #pragma unroll
-      for (int q = 0; q < P; ++q)
-        *reinterpret_cast<float4*>(head + d + q * GS * 4) =
-            make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
-    }
+    for (int q = 0; q < P; ++q)
+      *reinterpret_cast<float4*>(head + d + q * GS * 4) =
+          make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
   }
   __device__ __forceinline__ void write(bf16* head, const float (&y)[VW], float l) const {
     const float inv = 1.f / l;
-    if constexpr (VW == 1) {
-      head[d] = tobf(y[0] * inv);
-    } else {
 #pragma unroll
-      for (int q = 0; q < P; ++q)
-        *reinterpret_cast<uint2*>(head + d + q * GS * 4) =
-            make_uint2(pack_bf16(y[4 * q] * inv, y[4 * q + 1] * inv), pack_bf16(y[4 * q + 2] * inv, y[4 * q + 3] * inv));
-    }
+    for (int q = 0; q < P; ++q)
+      *reinterpret_cast<uint2*>(head + d + q * GS * 4) =
+          make_uint2(pack_bf16(y[4 * q] * inv, y[4 * q + 1] * inv), pack_bf16(y[4 * q + 2] * inv, y[4 * q + 3] * inv));
   }
 };
 
@@ -305,12 +289,9 @@ __device__ __forceinline__ void kv4_combine(int count, int lane, ML ml, OF o, fl
     const int n = min(GS, count - p0);
     float2 x = make_float2(-INFINITY, 0.f);
     if (gl < n) x = ml(p0 + gl);
-    constexpr int kAhead = VW == 1 ? 0 : 2;  // parts whose O sets out with the weights
-    float y0[2][VW];
-    if (kAhead) {
-      o(p0, y0[0]);
-      o(p0 + min(1, n - 1), y0[1]);
-    }
+    float y0[2][VW];  // the first two parts' O set out with the weights
+    o(p0, y0[0]);
+    o(p0 + min(1, n - 1), y0[1]);
     float top = x.x;
 #pragma unroll
     for (int d = 1; d < GS; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -324,13 +305,11 @@ __device__ __forceinline__ void kv4_combine(int count, int lane, ML ml, OF o, fl
     L = L * keep + l;
 #pragma unroll
     for (int i = 0; i < VW; ++i) O[i] *= keep;
-    if (kAhead) {
-      const float w0 = __shfl_sync(0xffffffffu, f, g0), w1 = __shfl_sync(0xffffffffu, f, g0 + 1);
+    const float w0 = __shfl_sync(0xffffffffu, f, g0), w1 = __shfl_sync(0xffffffffu, f, g0 + 1);
 #pragma unroll
-      for (int i = 0; i < VW; ++i) O[i] = fmaf(w0, y0[0][i], n > 1 ? fmaf(w1, y0[1][i], O[i]) : O[i]);
-    }
-#pragma unroll(VW == 1 ? 16 : 32 / VW)
-    for (int p = kAhead; p < n; ++p) {
+    for (int i = 0; i < VW; ++i) O[i] = fmaf(w0, y0[0][i], n > 1 ? fmaf(w1, y0[1][i], O[i]) : O[i]);
+#pragma unroll(32 / VW)
+    for (int p = 2; p < n; ++p) {
       const float w = __shfl_sync(0xffffffffu, f, g0 + p);
       float y[VW];
       o(p0 + p, y);
@@ -340,12 +319,11 @@ __device__ __forceinline__ void kv4_combine(int count, int lane, ML ml, OF o, fl
   }
 }
 
-// f(VW) for a team of T warps and G heads.
+// f(VW) for a team of T warps and G heads: a head to a warp, or as many as it takes.  (A head cut over several
+// warps was slower: every warp has to fetch all the parts' weights, 16 rows of 40960 at 8/8 heads 131 -> 124 us.)
 template <int G, class F>
 __device__ __forceinline__ void kv4_share(int T, F f) {
-  if (T > G)
-    f(std::integral_constant<int, 1>{});
-  else if (T == G || G == 1)
+  if (T >= G)
     f(std::integral_constant<int, 4>{});
   else if (2 * T == G || G == 2)
     f(std::integral_constant<int, G >= 2 ? 8 : 4>{});
@@ -400,18 +378,18 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     }
   }
   __syncthreads();
-  // Lane i weighs T = 2^i, in microseconds of a model fitted to runs of 17 shapes with each T (B200; on average
-  // within 1 % of the best T, at most 5 %): 3 us for a round of tiles; for each segment of a run 0.15 us per warp
-  // that the first has to wait for; where items are shared, 2 us, and 0.06 us for each of the G / T heads of a
-  // part that a warp adds.
+  // Lane i weighs T = 2^i, in units of a model fitted to runs of 24 shapes with each T (B200; on average within 1 %
+  // of the best T, at most 6 %; T = 1, 2, 4 or 8 for all would cost 95, 22, 19 or 23 % on average): 3 for a round of
+  // tiles; for each segment of a run 0.14 per head and warp that meets the first; where items are shared, 1.2, and
+  // for each part of an item 0.93 and 0.25 for each of the heads that a warp adds.
   if (warp == 0) {
     const int opt = min(lane, kSizes - 1);
     const uint32_t n = sm.sum[opt] * a.Hkv, teams = gridDim.x * (kAttWarps >> opt);
     const uint32_t c = max((n + teams - 1) / teams, 1u);
     const float t = (float)(1 << opt), ch = (float)c;
     const float per_item = __fdividef((float)n, (float)max(sm.sum[kSizes] * a.Hkv, 1u));
-    float cost = 3.f * ch + 0.15f * (t - 1.f) * (1.f + __fdividef(ch, fmaxf(per_item, 1.f)));
-    if (per_item > ch) cost += 2.f + 0.06f * G * __fdividef(per_item, ch * t);
+    float cost = 3.f * ch + 0.14f * G * (t - 1.f) * (1.f + __fdividef(ch, fmaxf(per_item, 1.f)));
+    if (per_item > ch) cost += 1.2f + __fdividef(per_item, ch) * (0.93f + __fdividef(0.25f * G, fminf(t, (float)G)));
     const uint32_t best = __reduce_min_sync(0xffffffffu, (__float_as_uint(cost) & ~7u) | opt) & 7u;
     if (lane == best) {
       sm.plan[0] = best;
@@ -857,8 +835,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
             float M, L, O[VW];
             kv4_combine<VW>(
                 n, lane, [&](int p) { return __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + at(p)); },
-                [&](int p, float(&y)[VW]) { sh.read(a.ws_o + at(p) * 128, y, [](auto* x) { return __ldcg(x); }); }, M, L,
-                O);
+                [&](int p, float(&y)[VW]) { sh.read(a.ws_o + at(p) * 128, y, [](auto* x) { return __ldcg(x); }); },
+                M, L, O);
             sh.write(out + sh.hd * 128, O, L);
           }
         });
