@@ -122,7 +122,7 @@ def _refuse(what: str, *args) -> None:
 
 
 def _ok(t, dtype, ndim: int, dev: int) -> bool:
-    return (t is not None and t.dtype is dtype and t.dim() == ndim and t.get_device() == dev and t.is_contiguous())
+    return (t is not None and t.dtype is dtype and t.ndim == ndim and t.get_device() == dev and t.is_contiguous())
 
 
 def _is_current(dev: int) -> bool:
@@ -139,7 +139,7 @@ def build_block_tables(lengths, block_size: int, *, max_blocks: int | None = Non
     dev = lengths.get_device()
     if not (_ok(lengths, _I32, 1, dev) and _is_current(dev)):
         _refuse(what, (lengths, _I32, 1, "lengths"))
-    S = lengths.shape[0]
+    S = lengths.numel()
     if out is None:
         if max_blocks is None:
             raise ValueError(f"{what}: give max_blocks or out")
@@ -150,8 +150,8 @@ def build_block_tables(lengths, block_size: int, *, max_blocks: int | None = Non
     if free_blocks is not None:
         if not _ok(free_blocks, _I32, 1, dev):
             _refuse(what, (free_blocks, _I32, 1, "free_blocks"))
-        num_free = free_blocks.shape[0]
-    if used is not None and not (_ok(used, _I32, 1, dev) and used.shape[0] == 1):
+        num_free = free_blocks.numel()
+    if used is not None and not (_ok(used, _I32, 1, dev) and used.numel() == 1):
         _refuse(what, (used, _I32, 1, "used"))
     rc = _lib.load().aacc_build_block_tables(lengths.data_ptr(), S, block_size, _p(free_blocks), num_free,
                                              out.data_ptr(), out.shape[1], _p(used), _raw_stream(dev))
@@ -172,22 +172,22 @@ def build_slot_maps(lengths, block_tables, *, block_size: int, num_blocks: int, 
     dev = lengths.get_device()
     if not (_ok(lengths, _I32, 1, dev) and _ok(block_tables, _I32, 2, dev) and _is_current(dev)):
         _refuse(what, (lengths, _I32, 1, "lengths"), (block_tables, _I32, 2, "block_tables"))
-    S = lengths.shape[0]
-    if starts is not None and not (_ok(starts, _I32, 1, dev) and starts.shape[0] == S):
+    S = lengths.numel()
+    if starts is not None and not (_ok(starts, _I32, 1, dev) and starts.numel() == S):
         _refuse(what, (starts, _I32, 1, "starts"), (lengths, _I32, 1, "lengths"))
-    if rows is not None and not (_ok(rows, _I64, 1, dev) and rows.shape[0] == S):
+    if rows is not None and not (_ok(rows, _I64, 1, dev) and rows.numel() == S):
         _refuse(what, (rows, _I64, 1, "rows"), (lengths, _I32, 1, "lengths"))
     if cu is None:
         cu = torch.empty(S + 1, dtype=_I32, device=lengths.device)
-    elif not (_ok(cu, _I32, 1, dev) and cu.shape[0] == S + 1):
+    elif not (_ok(cu, _I32, 1, dev) and cu.numel() == S + 1):
         _refuse(what, (cu, _I32, 1, "cu"), (lengths, _I32, 1, "lengths"))
     if positions is None:
         positions = torch.empty(num_tokens, dtype=_I64, device=lengths.device)
-    elif not (_ok(positions, _I64, 1, dev) and positions.shape[0] == num_tokens):
+    elif not (_ok(positions, _I64, 1, dev) and positions.numel() == num_tokens):
         _refuse(f"{what} (num_tokens {num_tokens})", (positions, _I64, 1, "positions"))
     if slots is None:
         slots = torch.empty(num_tokens, dtype=_I64, device=lengths.device)
-    elif not (_ok(slots, _I64, 1, dev) and slots.shape[0] == num_tokens):
+    elif not (_ok(slots, _I64, 1, dev) and slots.numel() == num_tokens):
         _refuse(f"{what} (num_tokens {num_tokens})", (slots, _I64, 1, "slots"))
     num_rows, max_blocks = block_tables.shape
     rc = _lib.load().aacc_build_slot_maps(
@@ -227,16 +227,16 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     flat slots of the 4-bit pools (see kv4_cache_shape); negative slots skip,
     the others must be distinct."""
     what = "kv4_store"
-    dev, pool, n = k_cache.get_device(), k_cache.shape, slot_mapping.shape
+    dev, pool, T = k_cache.get_device(), k_cache.shape, slot_mapping.numel()
     if not (k_cache.dtype is _U8 and v_cache.dtype is _U8 and v_cache.shape == pool and len(pool) == 4
-            and pool[3] == KV4_RECORD_BYTES and slot_mapping.dtype is _I64 and len(n) == 1
+            and pool[3] == KV4_RECORD_BYTES and slot_mapping.dtype is _I64 and slot_mapping.ndim == 1
             and dev >= 0 and dev == _current_device() and v_cache.get_device() == dev
             and slot_mapping.get_device() == dev and k_cache.is_contiguous() and v_cache.is_contiguous()
             and slot_mapping.is_contiguous()):
         _refuse(what, (k_cache, _U8, 4, "k_cache"), (v_cache, _U8, 4, "v_cache"),
                 (slot_mapping, _I64, 1, "slot_mapping"))
     nb, hkv, tiles, _ = pool
-    bs, T = tiles * KV4_TILE, n[0]
+    bs = tiles * KV4_TILE
     ks, kh = _kv_rows(k, hkv, T, dev, what, "k")
     vs, vh = _kv_rows(v, hkv, T, dev, what, "v")
     rc = _lib.load().aacc_kv4_store(k.data_ptr(), v.data_ptr(), T, ks, kh, vs, vh, slot_mapping.data_ptr(),
@@ -253,17 +253,17 @@ def kv4_load(k_cache, v_cache, slots, k_out=None, v_out=None, *, out_slots=None)
     Returns (k_out, v_out); outputs made here are zero where a token is
     skipped."""
     what = "kv4_load"
-    dev, pool, n = k_cache.get_device(), k_cache.shape, slots.shape
+    dev, pool, T = k_cache.get_device(), k_cache.shape, slots.numel()
     if not (k_cache.dtype is _U8 and v_cache.dtype is _U8 and v_cache.shape == pool and len(pool) == 4
-            and pool[3] == KV4_RECORD_BYTES and slots.dtype is _I64 and len(n) == 1
+            and pool[3] == KV4_RECORD_BYTES and slots.dtype is _I64 and slots.ndim == 1
             and dev >= 0 and dev == _current_device() and v_cache.get_device() == dev and slots.get_device() == dev
             and k_cache.is_contiguous() and v_cache.is_contiguous() and slots.is_contiguous()
-            and (out_slots is None or (out_slots.dtype is _I64 and out_slots.shape == n
+            and (out_slots is None or (out_slots.dtype is _I64 and out_slots.ndim == 1 and out_slots.numel() == T
                                        and out_slots.get_device() == dev and out_slots.is_contiguous()))):
         _refuse(what, (k_cache, _U8, 4, "k_cache"), (v_cache, _U8, 4, "v_cache"), (slots, _I64, 1, "slots"),
                 *(() if out_slots is None else ((out_slots, _I64, 1, "out_slots"),)))
     nb, hkv, tiles, _ = pool
-    bs, T = tiles * KV4_TILE, n[0]
+    bs = tiles * KV4_TILE
     if k_out is None or v_out is None:
         if out_slots is not None or k_out is not None or v_out is not None:
             raise ValueError(f"{what}: give both k_out and v_out (or neither and no out_slots)")
@@ -300,7 +300,8 @@ def kv4_decode_attention(q, k_cache, v_cache, block_tables, rows, seqlens, *, ct
     if not (q.dtype is BF16 and out.dtype is BF16 and out.shape == shape and len(shape) == 3 and shape[2] == 128
             and k_cache.dtype is _U8 and v_cache.dtype is _U8 and v_cache.shape == pool and len(pool) == 4
             and pool[3] == KV4_RECORD_BYTES and block_tables.dtype is _I32 and len(bt) == 2
-            and rows.dtype is _I64 and rows.shape == shape[:1] and seqlens.dtype is _I32 and seqlens.shape == bt[:1]
+            and rows.dtype is _I64 and rows.ndim == 1 and rows.numel() == shape[0]
+            and seqlens.dtype is _I32 and seqlens.ndim == 1 and seqlens.numel() == bt[0]
             and workspace is not None and workspace.dtype is _U8 and dev >= 0 and dev == _current_device()
             and out.get_device() == dev and k_cache.get_device() == dev and v_cache.get_device() == dev and block_tables.get_device() == dev
             and rows.get_device() == dev and seqlens.get_device() == dev and workspace.get_device() == dev
