@@ -30,8 +30,9 @@
 // at launch) the whole tile is straight-line code without spills.  Where this
 // took 131 us for 256 rows, others took: 16 warps that load for themselves and
 // work on halves of a tile in a rolled loop 141; 8 that load for themselves
-// 138; 12 that compute and 4 that load, one buffer each for K and V, 160; a
-// third stage 131; Q.K of the next tile between P.V of this one 156.
+// 138; 12 that compute and 4 that load 157, with three records each and 152
+// registers; a third stage 131; Q.K of the next tile between P.V of this one
+// 156.
 //
 // Q.K: the tokens are the rows of m16n8k16's A operand, the G <= 8 query heads
 // its 8 columns.  Fewer heads share the columns out: with a column each, a lane
