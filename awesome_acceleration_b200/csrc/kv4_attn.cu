@@ -631,7 +631,14 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
           }
           const uint32_t big = max(max(max(x.x, x.y), max(x.z, x.w)),
                                    max(max(x.x << 16, x.y << 16), max(x.z << 16, x.w << 16)));
-          const int e = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
+          int e = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
+          if (e >= 255) {  // a NaN: it reaches its own dims through vpair, the reference follows finite scales
+            auto finite = [](uint32_t bits) { return (~bits & 0x7f800000u) ? bits & 0x7fffffffu : 0u; };
+            const uint32_t f = max(max(max(finite(x.x), finite(x.y)), max(finite(x.z), finite(x.w))),
+                                   max(max(finite(x.x << 16), finite(x.y << 16)),
+                                       max(finite(x.z << 16), finite(x.w << 16))));
+            e = (int)(__reduce_max_sync(0xffffffffu, f) >> 23);
+          }
           if (e > ev) {
 #pragma unroll
             for (int i = 0; i < HV; ++i) al[i] = ex2((float)(ev - e));
