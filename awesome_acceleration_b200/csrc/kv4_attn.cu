@@ -49,13 +49,26 @@
 // the largest.
 // P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand.  Here the sum
 // over thousands of tokens would cancel against its offset, so u - 8 is made
-// exactly, by one more fp16x2 add or fma.  P^T is 2^4 p in fp16 (the 2^4 also
-// in the sum it is divided by), p < 2^6, transposed in registers and multiplied
-// by the V scales of its two tokens in fp16: two roundings of 2^-11, a quarter
-// of what one to bf16 costs.  The scales are held relative to the largest so
-// far, at [2^4, 2^5): products reach 2^15, and a p down to 2^-18 and a scale
-// down to 2^-21 of the largest have no other rounding than those two.
-// Once per tile each lane turns the scales of its two tokens into such pairs.
+// exactly, by one more fp16x2 add or fma.  P^T is 2^kUp p in fp16, p <= 2^kLag,
+// transposed in registers and multiplied by the V scales of its two tokens in
+// fp16: two roundings of 2^-11, a quarter of what one to bf16 costs.  The
+// scales are held relative to 2^(e + 1), the largest so far being in
+// [2^e, 2^(e + 1)), and are exact down to 2^-kSpan of that.  Once per tile each
+// lane turns the scales of its two tokens into such pairs.
+//
+// fp16 ends 2^-40 below its largest number: in P, and in the product with a
+// scale, up to 2^-25 is lost, 2^-(24 + kUp) 2^(e + 1) of a token's p s.  That
+// matters where the tokens of most of the probability have the small scales.
+// When the softmax reference was set, its token had p = 1 and a scale of at
+// least 2^low, the smallest in that tile, so that D = sum p s >= 2^low from then
+// on, and n tiles of 64 tokens lose at most 2^-16 D while
+// n <= 2^(kUp + 1 + low - e): 2^7 tiles, 8192 tokens of one warp, for scales
+// within 2^6 of one another.  Later tiles, and tiles with a scale below
+// 2^-kSpan of the largest (zero among them) or a NaN, take a second path: p s
+// in fp32, cut into two bf16 that two MMAs on bf16 codes add up.  O is held
+// relative to the largest scale, so that what lies 2^-100 below it still counts in
+// full.  A tile takes 2.5 times as long on it (256 rows with one token in 16 at
+// 2^-20 of the others: 287 us, without 119).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -70,6 +83,12 @@ constexpr int kSizes = 4;   // team sizes: 1, 2, 4, 8 warps
 constexpr int kStages = 2;  // tiles of K and V that a warp has in hand or in flight
 constexpr int kAttThreads = 2 * kAttWarps * 32;  // as many warps again load
 constexpr int kPlanWarps = kAttThreads / 32;
+constexpr int kLag = 3;           // the softmax reference follows a score that passes it by more than 2^kLag
+constexpr int kUp = 15 - kLag;    // P is held times 2^kUp: at most 2^15 in fp16
+constexpr int kSpan = 16;         // powers of two that V scales in fp16 may lie below the largest
+constexpr int kRoom = kUp + 1;    // see kv4_room
+// less `from` and a scale: bits 15 and 31 where the scale is below 2^(ev + 1)
+constexpr uint32_t kUpTo = (0x807fu + 0x8000u + (kSpan << 7)) * 0x10001u;
 
 // A run of tiles [t0, t1) of item (b, h), whose row has n tiles; u is the unit number of t0.
 struct Kv4Seg {
@@ -223,6 +242,20 @@ __device__ __forceinline__ uint32_t code(uint32_t x) {
   const __half2 r = HI ? __hfma2(h, __float2half2_rn(0.0625f), __float2half2_rn(-72.f))
                        : __hadd2(h, __float2half2_rn(-1032.f));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Bits 0-3 of both halves of x as the bf16 pair (u - 8, u' - 8), through 128 + u.
+__device__ __forceinline__ uint32_t code_bf16(uint32_t x) {
+  const uint32_t y = and_or<0x000f000fu>(x, 0x43004300u);
+  const __nv_bfloat162 r = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&y), __float2bfloat162_rn(-136.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Tiles that may hold p s in fp16 (see the head of the file) for the largest V scale in [2^ev, 2^(ev + 1)) and none
+// below 2^low where the softmax reference was set.
+__device__ __forceinline__ int kv4_room(int ev, int low) {
+  const int d = ev - low;
+  return d > kRoom ? 0 : 1 << (kRoom - max(d, 0));
 }
 
 // bf16 pair W / 2 of `p`, member W % 2, as fp32.
@@ -573,7 +606,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       float m[HV], l[HV];
 #pragma unroll
       for (int e = 0; e < HV; ++e) m[e] = -INFINITY, l[e] = 0.f;
-      int ev = 4;  // biased exponent of the largest V scale so far (at least 4): O is kept times 2^(131 - ev)
+      // Biased exponents of the largest V scale so far (at least this) and of the smallest in the tiles that set the
+      // softmax reference; tiles from `room` on are left to the second path.  O is kept times 2^(kUp + 126 - ev).
+      int ev = kSpan + 1, low = 255, room = 0;
+      uint32_t from = 0;  // and a scale: bits 15 and 31 where the scale is at least 2^(ev - kSpan); 0: not set
 
       for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += T) {
         const uint32_t st = used % kStages;
@@ -617,79 +653,153 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
           group(std::integral_constant<int, 3>{}, x4.w, y4.w);
         }
 
-        // ---- the tile's V scales as fp16 pairs; lane: tokens 2 lane and 2 lane + 1.  Behind the context a scale
-        // may be anything: it becomes zero.  They are not negative: their bits order as they do.
-        float al[HV];
-#pragma unroll
-        for (int e = 0; e < HV; ++e) al[e] = 1.f;
-        bool grow = false;
-        {
-          uint4 x = *(reinterpret_cast<const uint4*>(vb + kKv4Codes) + lane);
-          if (lim < kKv4Tile) {
-            if (2 * lane >= lim) x.x = x.y = 0;
-            if (2 * lane + 1 >= lim) x.z = x.w = 0;
-          }
-          const uint32_t big = max(max(max(x.x, x.y), max(x.z, x.w)),
-                                   max(max(x.x << 16, x.y << 16), max(x.z << 16, x.w << 16)));
-          int e = (int)(__reduce_max_sync(0xffffffffu, big) >> 23);
-          if (e >= 255) {  // a NaN: it reaches its own dims through vpair, the reference follows finite scales
-            auto finite = [](uint32_t bits) { return (~bits & 0x7f800000u) ? bits & 0x7fffffffu : 0u; };
-            const uint32_t f = max(max(max(finite(x.x), finite(x.y)), max(finite(x.z), finite(x.w))),
-                                   max(max(finite(x.x << 16), finite(x.y << 16)),
-                                       max(finite(x.z << 16), finite(x.w << 16))));
-            e = (int)(__reduce_max_sync(0xffffffffu, f) >> 23);
-          }
-          if (e > ev) {
-#pragma unroll
-            for (int i = 0; i < HV; ++i) al[i] = ex2((float)(ev - e));
-            ev = e;
-            grow = true;
-          }
-          const float cv = __uint_as_float((uint32_t)(258 - ev) << 23);
-          const uint2 ta = make_uint2(x.x, x.y), tb = make_uint2(x.z, x.w);
-          sm.vpair[warp][lane] = make_uint4(pack_f16(scale_of<0>(ta) * cv, scale_of<0>(tb) * cv),
-                                            pack_f16(scale_of<1>(ta) * cv, scale_of<1>(tb) * cv),
-                                            pack_f16(scale_of<2>(ta) * cv, scale_of<2>(tb) * cv),
-                                            pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
-        }
-
-        // ---- online softmax in the log2 domain
+        // ---- the tile's V scales; lane: tokens 2 lane and 2 lane + 1.  Behind the context a scale may be anything:
+        // it becomes that of the tile's first token, and p zero.
+        uint4 vs = *(reinterpret_cast<const uint4*>(vb + kKv4Codes) + lane);
         if (lim < kKv4Tile) {
+          const uint2 first = *reinterpret_cast<const uint2*>(vb + kKv4Codes);
+          if (2 * lane >= lim) vs.x = first.x, vs.y = first.y;
+          if (2 * lane + 1 >= lim) vs.z = first.x, vs.w = first.y;
 #pragma unroll
           for (int sb = 0; sb < 4; ++sb)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
               if (16 * sb + tok + i / HV * 8 >= lim) s[sb][i] = -INFINITY;
         }
-        // The reference of the exponentials follows the maximum only when a score passes it by 2^6: p stays
-        // below 2^6, and most tiles need no shuffles and no rescaling.
+        // Scales are not negative, so their bits order as they do: bits 15 and 31 stay where all are in range.
+        const uint32_t hi = __vmaxu2(__vimax3_u16x2(vs.x, vs.y, vs.z), vs.w);
+        const uint32_t lo = __vminu2(__vimin3_u16x2(vs.x, vs.y, vs.z), vs.w);
+        const bool odd = ~((lo + from) & (kUpTo - from - hi)) & 0x80008000u;
+
+        // ---- online softmax in the log2 domain.  The reference of the exponentials follows the maximum only when a
+        // score passes it by 2^kLag: p stays below that, and most tiles need no shuffles and no rescaling.
         float x[HV];
-        bool above = false;
+        bool above = false, wide = false;
 #pragma unroll
         for (int e = 0; e < HV; ++e) {
           x[e] = s[0][e];
 #pragma unroll
           for (int i = 1; i < 4 * NV / HV; ++i) x[e] = fmaxf(x[e], s[i % 4][i / 4 * HV + e]);
           x[e] *= sl[e];
-          above |= x[e] > m[e] + 6.f;
+          above |= x[e] > m[e] + (float)kLag;
         }
-        if (__any_sync(0xffffffffu, above)) {
+        if (__any_sync(0xffffffffu, above || odd) || t >= room) {
+          const uint32_t big = __reduce_max_sync(0xffffffffu, max(hi & 0xffffu, hi >> 16));
+          const uint32_t least = __reduce_min_sync(0xffffffffu, min(lo & 0xffffu, lo >> 16));
+          const bool set = __any_sync(0xffffffffu, above);
+          const int e0 = ev;
+          if (big < 253u << 7) ev = max(ev, (int)(big >> 7));  // else the second path looks for the largest finite
+          const uint32_t from_v = (uint32_t)(ev - kSpan) << 7;
+          wide = big >= 253u << 7 || least < from_v;
+          from = (0x8000u - from_v) * 0x10001u;
+          const float up = ex2((float)(e0 - ev));
+          if (set) low = min(low, least < 0x80u ? -255 : (int)(least >> 7));
+          float al[HV];
 #pragma unroll
           for (int e = 0; e < HV; ++e) {
 #pragma unroll
             for (int d = kLow; d < 32; d += d == 1 ? 3 : d) x[e] = fmaxf(x[e], __shfl_xor_sync(0xffffffffu, x[e], d));
-            x[e] = fmaxf(m[e], x[e]);
+            x[e] = set ? fmaxf(m[e], x[e]) : m[e];
             const float f = ex2(m[e] - x[e]);
             m[e] = x[e];
-            l[e] *= f;
-            al[e] *= f;
+            al[e] = set ? f * up : up;
+            l[e] *= set ? f : 1.f;
           }
-          grow = true;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][i] *= al[i % HV];
+          room = cs.t0 + wt + (kv4_room(ev, low) << tsh);
+          wide |= t >= room;
+          if (wide) {
+            if (big >= 253u << 7) {
+              uint32_t f = 0;
+#pragma unroll 1
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t u = *reinterpret_cast<const uint16_t*>(vb + kKv4Codes + 2 * (32 * i + lane)) & 0x7fffu;
+                if (u < 0x7f80u && 8 * i + lane / 4 < lim) f = max(f, u);
+              }
+              const int e = min((int)(__reduce_max_sync(0xffffffffu, f) >> 7), 252);
+              if (e > ev) {
+                const float r = ex2((float)(ev - e));
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) o[j][i] *= r;
+                ev = e;
+                from = 0;  // the next tile sets the limits
+              }
+            }
+            // p s in fp32 as a sum of two bf16: 2^-17 of itself off, over all of fp32's range.  At other places than
+            // its own, a column's B is zero.
+            const float cw = __uint_as_float((uint32_t)(253 - ev) << 23);
+            float* mine = &sm.red_o[warp][0][lane];  // free until the segment ends
+#pragma unroll
+            for (int i = 0; i < 4 * NV; ++i) mine[32 * i] = s[i / NV][i % NV];
+#pragma unroll 1
+            for (int sb = 0; sb < 4; ++sb) {
+              const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);
+              const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);
+              const int t0 = 16 * sb + tok;
+              float p[NV];
+#pragma unroll
+              for (int i = 0; i < NV; ++i)
+                p[i] = t0 + i / HV * 8 < lim ? ex2(fmaf(mine[32 * (sb * NV + i)], sl[i % HV], (float)kUp - m[i % HV])) : 0.f;
+              uint2 sx = *reinterpret_cast<const uint2*>(vb + kKv4Codes + t0 * 8), sy = make_uint2(0, 0);
+              if constexpr (kCols < 4) sy = *reinterpret_cast<const uint2*>(vb + kKv4Codes + (t0 + 8) * 8);
+              if (t0 >= lim) sx = make_uint2(0, 0);
+              if (t0 + 8 >= lim) sy = make_uint2(0, 0);
+              auto group = [&](auto W) {
+                constexpr int w = decltype(W)::value;
+                const float fx = scale_of<w>(sx) * cw, fy = scale_of<w>(sy) * cw;
+                float v[4];
+                if constexpr (kCols == 1)
+                  v[0] = p[0] * fx, v[1] = p[1] * fx, v[2] = p[NV - 2] * fy, v[3] = p[NV - 1] * fy;
+                else if constexpr (kCols == 2)
+                  v[0] = p[0] * fx, v[1] = p[NV - 1] * fy, v[2] = v[3] = 0.f;
+                else
+                  v[0] = v[1] = p[0] * fx, v[2] = v[3] = 0.f;
+                constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
+                const uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
+                const uint32_t y = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
+                const uint32_t a0[4] = {code_bf16(x), code_bf16(x >> 4), code_bf16(y), code_bf16(y >> 4)};
+                const uint32_t a1[4] = {code_bf16(x >> 8), code_bf16(x >> 12), code_bf16(y >> 8), code_bf16(y >> 12)};
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {
+                  const uint32_t u0 = pack_bf16(v[0], v[1]), u1 = pack_bf16(v[2], v[3]);
+                  const float2 r0 = unpack_bf16(u0), r1 = unpack_bf16(u1);
+                  v[0] -= r0.x, v[1] -= r0.y, v[2] -= r1.x, v[3] -= r1.y;
+                  const uint32_t t = movmatrix_trans(u0);
+                  uint32_t b0 = t, b1 = t;
+                  if constexpr (kCols == 1)
+                    b1 = movmatrix_trans(u1);
+                  else if constexpr (kCols == 2)
+                    b0 = g & 1 ? 0u : t, b1 = g & 1 ? t : 0u;
+                  else
+                    b0 = (g & 3) == 0 ? t : 0u, b1 = (g & 3) == 2 ? t : 0u;
+                  mma_bf16_16816(o[2 * w], a0, b0, b1);
+                  mma_bf16_16816(o[2 * w + 1], a1, b0, b1);
+                }
+              };
+              group(std::integral_constant<int, 0>{});
+              group(std::integral_constant<int, 1>{});
+              group(std::integral_constant<int, 2>{});
+              group(std::integral_constant<int, 3>{});
+            }
+          }
+        }
+        {
+          const float cv = wide ? 0.f : __uint_as_float((uint32_t)(253 - ev) << 23);
+          const uint2 ta = make_uint2(vs.x, vs.y), tb = make_uint2(vs.z, vs.w);
+          sm.vpair[warp][lane] = make_uint4(pack_f16(scale_of<0>(ta) * cv, scale_of<0>(tb) * cv),
+                                            pack_f16(scale_of<1>(ta) * cv, scale_of<1>(tb) * cv),
+                                            pack_f16(scale_of<2>(ta) * cv, scale_of<2>(tb) * cv),
+                                            pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
         }
 #pragma unroll
         for (int sb = 0; sb < 4; ++sb)
 #pragma unroll
-          for (int i = 0; i < NV; ++i) s[sb][i] = ex2(fmaf(s[sb][i], sl[i % HV], 4.f - m[i % HV]));  // 2^4 p
+          for (int i = 0; i < NV; ++i) s[sb][i] = ex2(fmaf(s[sb][i], sl[i % HV], (float)kUp - m[i % HV]));  // 2^kUp p
         if (lim < kKv4Tile) {  // also where a scale of 0 makes -inf * 0 a NaN
 #pragma unroll
           for (int sb = 0; sb < 4; ++sb)
@@ -701,12 +811,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         for (int sb = 0; sb < 4; ++sb)
 #pragma unroll
           for (int i = 0; i < NV; ++i) l[i % HV] += s[sb][i];
-        if (grow) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[j][i] *= al[i % HV];
-        }
         __syncwarp();  // vpair is written
 
         // ---- O^T += V^T P^T
@@ -759,7 +863,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       Kv4Seg nx = cs;
       const bool more = kv4_next(a, sm, nx, uend, tsh);
       if (more) load_q(nx);
-      const float down = __uint_as_float((uint32_t)(ev - 4) << 23) + (ev == 4 ? 0x1p-127f : 0.f);
+      const float down = __uint_as_float((uint32_t)(ev + 1) << 23) * (1.f / (1 << kUp));
 #pragma unroll
       for (int e = 0; e < HV; ++e) {  // dims 16 j + 2g and + 1: o[j][e], o[j][2 + e], summed over a head's columns
         const int hd = (2 * c + e) / kCols;
@@ -777,7 +881,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
             *reinterpret_cast<float2*>(&sm.red_o[warp][hd][16 * j + 2 * g]) = make_float2(y0 * down, y1 * down);
         }
         if (hd < G && g == 0 && (kCols < 4 || (c & 1) == 0))
-          *reinterpret_cast<float2*>(sm.red_ml[warp][hd]) = make_float2(m[e], l[e]);
+          *reinterpret_cast<float2*>(sm.red_ml[warp][hd]) = make_float2(m[e], l[e] * (1.f / (1 << kUp)));
       }
       team_sync(team, tsh);
       const bool whole = cs.t0 == 0 && cs.t1 == cs.n;

@@ -64,3 +64,129 @@ def test_a_v_group_that_is_not_finite_in_a_split_context(cuda):
         check(out, c)
         bad = torch.isnan(out)
         assert bad[0, :G, 64:96].all() and bad.sum() == 32 * G
+
+
+# --------------------------------------------------------------------------- V scales of very different magnitude
+def check_v(out, c, **kw):
+    """`check` holds every element to 2^-10 sum p|v| (and the roundings of the output and of fp32): a value may lie
+    any way below the largest of its context, its tile or its token."""
+    assert torch.isfinite(out).all()
+    check(out, c, **kw)
+
+
+def with_v(c, v):
+    return dict(c, vp=O.pool_from_rows(v, c["bs"], True))
+
+
+@pytest.mark.parametrize("e", [-10, -16, -24, -30, -45, -60])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_v_scales_across_groups(cuda, G, e):
+    """Groups of 32 dims at 1, 2^e, 2^(e/2) and 2^(e/3) of one another."""
+    c = make_case([200, 64, 1, 130], G, 2, 64, 100 + G)
+    v = rows(c, 101, 2).float().view(-1, 2, 4, 32)
+    v = v * 2.0 ** torch.tensor([0, e, e // 2, e // 3]).view(4, 1)
+    c = with_v(c, v.view(-1, 2, 128).to(BF))
+    check_v(call(c, cuda), c)
+
+
+@pytest.mark.parametrize("e", [-10, -16, -24, -30, -45, -60])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_v_scales_across_tokens(cuda, G, e):
+    """Every third token, whole tiles, or all but one token at 2^e of the rest."""
+    for k, pick in enumerate((lambda t: t % 3 == 0, lambda t: t // 64 == 1, lambda t: t != 77)):
+        c = make_case([200, 130], G, 2, 64, 110 + G)
+        v = rows(c, 111 + k, 2).float()
+        for b in (0, 1):
+            at = slots_of(c, b)
+            small = pick(torch.arange(c["ctx"][b]))
+            v[at[small]] *= 2.0 ** e
+        c = with_v(c, v.to(BF))
+        check_v(call(c, cuda), c)
+
+
+def logits_case(logit, G, hkv, ctx, seed, bs=64):
+    """A case whose logits are near logit(t) (natural log) for token t of every row: q is one direction u for all
+    heads, up to 1 part in 8, and k_t = logit(t) u."""
+    c = make_case(ctx, G, hkv, bs, seed)
+    g = torch.Generator().manual_seed(seed)
+    u = torch.where(torch.rand(128, generator=g) < 0.5, -1.0, 1.0)
+    c["q"] = (u * (1 + 0.125 * torch.rand(c["q"].shape, generator=g))).to(BF)
+    k = torch.zeros((c["nb"] * bs, hkv, 128))
+    for b, n in enumerate(ctx):
+        x = logit(torch.arange(n)).float() / (128 * SCALE)
+        k[slots_of(c, b)] = x.view(-1, 1, 1) * u
+    c["kp"] = O.pool_from_rows(k.to(BF), bs, False)
+    return c
+
+
+@pytest.mark.parametrize("e", [10, 20, 30, 45, 60])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_a_huge_v_of_negligible_or_of_small_probability(cuda, G, e):
+    """Token t0's V is 2^e times the others', its probability 2^-(e + 20) (it adds nothing), 2^-e (it adds as much
+    as another) or 2^-(e - 6) (it is most of the output)."""
+    for t0 in (3, 90, 199):
+        for less in (e + 20, e, e - 6):
+            c = logits_case(lambda t: torch.where(t == t0, -less * math.log(2.0), 0.25 * torch.cos(t.float())), G, 2,
+                            [200], 120 + G)
+            v = rows(c, 121, 2).float()
+            v[slots_of(c, 0)[t0]] *= 2.0 ** e
+            c = with_v(c, v.to(BF))
+            check_v(call(c, cuda), c)
+
+
+@pytest.mark.parametrize("e", [0, 8, 20, 26, 40, 60])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_a_token_of_all_the_probability_and_no_value(cuda, G, e):
+    """An attention sink: one token's V is zero, in all groups or in one, and the others, at 2^-e of its
+    probability, are the whole output."""
+    for groups in ([0, 1, 2, 3], [2]):
+        c = logits_case(lambda t: torch.where(t == 0, 0.0, -e * math.log(2.0) + torch.sin(t.float())), G, 2,
+                        [150, 2], 130 + G)
+        v = rows(c, 131, 2).view(-1, 2, 4, 32)
+        for b in (0, 1):
+            v[slots_of(c, b)[0], :, groups] = 0
+        c = with_v(c, v.view(-1, 2, 128))
+        check_v(call(c, cuda), c)
+
+
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_small_values_over_a_long_context(cuda, G):
+    """Thousands of tokens in one warp's run (1300 queries over the same 4000): a first tile of small V and most of
+    the probability, then large V of little."""
+    B, look = 1300, [0, 650, 1299]
+    for e in (6, 9, 12, 20):
+        c = logits_case(lambda t: torch.where(t < 64, 0.0, -(e + 14) * math.log(2.0)), G, 1, [4000], 140 + G, 256)
+        q = c["q"] * (1 + torch.randint(0, 32, (B, 1, 1), generator=torch.Generator().manual_seed(e)) / 256)
+        v = rows(c, 141, 1).float()
+        v[slots_of(c, 0)[:64]] *= 2.0 ** -e
+        c = with_v(c, v.to(BF))
+        out = call(c, cuda, q=q.to(BF), rows=torch.zeros(B, dtype=torch.int64))
+        check_v(out[look], dict(c, q=q.to(BF)[look], ctx=[4000] * 3, bt=c["bt"].expand(3, -1)))
+
+
+@pytest.mark.parametrize("G", [2, 8])
+def test_v_scales_down_to_2_100_of_the_largest_and_subnormal_ones(cuda, G):
+    for top, low in ((2.0 ** 60, 2.0 ** -40), (2.0 ** -10, 2.0 ** -110), (2.0 ** -100, 2.0 ** -128)):
+        c = make_case([100, 65], G, 2, 64, 150 + G)
+        v = rows(c, 151, 2).float()
+        v[::2] *= low
+        v[1::2] *= top
+        v.view(-1, 2, 4, 32)[1::4, :, 1] *= low / top
+        c = with_v(c, v.to(BF))
+        check_v(call(c, cuda), c)
+
+
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_v_groups_that_are_not_finite_among_scales_of_every_size(cuda, G):
+    """NaN, zero and far-apart scales in the same tiles."""
+    c = make_case([200], G, 2, 64, 160 + G)
+    v = rows(c, 161, 2).float()
+    at = slots_of(c, 0)
+    v[at[::3]] *= 2.0 ** -40
+    v[at[5::7]] = 0
+    v[at[100], 1, 40] = math.inf
+    c = with_v(c, v.to(BF))
+    out = call(c, cuda).cpu()
+    check(out, c)
+    bad = torch.isnan(out)
+    assert bad[0, G:, 32:64].all() and bad.sum() == 32 * G
