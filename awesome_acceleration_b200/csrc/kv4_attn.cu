@@ -45,8 +45,9 @@
 // put right in the softmax scale, the 16 in q, and the offset of 8 through the
 // accumulator's start, -8 sum(q) of the group; the group's scale multiplies
 // the fp32 sum.  q is scaled by a power of two per head to a largest element
-// in [2^14, 2^15), so that bf16 values go into fp16 unrounded down to 2^-24 of
-// the largest.
+// in [2^14, 2^15), so that bf16 values go into fp16 unrounded down to 2^-27 of
+// the largest.  Items with smaller ones, or with q or a softmax scale for which
+// fp32 has no room, take the second path below.
 // P.V: O^T = V^T P^T with V^T (dims x tokens) as the A operand.  Here the sum
 // over thousands of tokens would cancel against its offset, so u - 8 is made
 // exactly, by one more fp16x2 add or fma.  P^T is 2^kUp p in fp16, p <= 2^kLag,
@@ -64,11 +65,14 @@
 // on, and n tiles of 64 tokens lose at most 2^-16 D while
 // n <= 2^(kUp + 1 + low - e): 2^7 tiles, 8192 tokens of one warp, for scales
 // within 2^6 of one another.  Later tiles, and tiles with a scale below
-// 2^-kSpan of the largest (zero among them) or a NaN, take a second path: p s
-// in fp32, cut into two bf16 that two MMAs on bf16 codes add up.  O is held
-// relative to the largest scale, so that what lies 2^-100 below it still counts in
-// full.  A tile takes 2.5 times as long on it (256 rows with one token in 16 at
-// 2^-20 of the others: 287 us, without 119).
+// 2^-kSpan of the largest (zero among them) or a NaN, take a second path: codes
+// and q in bf16, no product rounded; p s in fp32, cut into two bf16 that two
+// MMAs add up.  O is held relative to the largest scale and q to its largest
+// element, so that what lies 2^-100 below them still counts in full.  A tile takes
+// 3.6 times as long on it, in loops that are rolled so that the first path keeps
+// its registers (256 rows with one token in 16 at 2^-20 of the others: 433 us,
+// without 119; with the loops unrolled, or in a function of its own, 256 x 1500
+// at 64/8 heads take 99 or 105 us on the first path, and so 96).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -87,6 +91,7 @@ constexpr int kLag = 3;           // the softmax reference follows a score that 
 constexpr int kUp = 15 - kLag;    // P is held times 2^kUp: at most 2^15 in fp16
 constexpr int kSpan = 16;         // powers of two that V scales in fp16 may lie below the largest
 constexpr int kRoom = kUp + 1;    // see kv4_room
+constexpr int kNone = -512;       // instead of an exponent: no tile has room
 // less `from` and a scale: bits 15 and 31 where the scale is below 2^(ev + 1)
 constexpr uint32_t kUpTo = (0x807fu + 0x8000u + (kSpan << 7)) * 0x10001u;
 
@@ -249,6 +254,15 @@ __device__ __forceinline__ uint32_t code_bf16(uint32_t x) {
   const uint32_t y = and_or<0x000f000fu>(x, 0x43004300u);
   const __nv_bfloat162 r = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&y), __float2bfloat162_rn(-136.f));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Power of two by which the second path multiplies q: the softmax scale's if that is below 1, and less where q's
+// largest element (bf16 bits mx) would pass 2^101.
+__device__ __forceinline__ int kv4_q_exp(float scale, uint32_t mx) {
+  const int e = (int)(__float_as_uint(fabsf(scale) * kLog2e) >> 23) - 127;
+  return min(min(max(e, -120), 0), 227 - (int)(mx >> 7));
 }
 
 // Tiles that may hold p s in fp16 (see the head of the file) for the largest V scale in [2^ev, 2^(ev + 1)) and none
@@ -561,9 +575,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       uint32_t qf[4][4];
       float sl[HV];       // log2 softmax scale of the raw scores of this lane's heads
       float corr[4][HV];  // -8 times 2^-24 times the sum of their q over group w
+      bool fits;          // q into fp16
       {
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns q's sign
-        uint32_t mx = 0;
+        uint32_t hi = 0, lo = 0x7fff7fffu;  // in pairs: largest |q|; smallest above zero, plus 0x7fff
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           qf[w][0] = xq[w].x ^ flip;
@@ -571,10 +586,21 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
           qf[w][2] = xq[w].z ^ flip;
           qf[w][3] = xq[w].w ^ flip;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) mx = max(mx, max(qf[w][r] & 0x7fffu, (qf[w][r] >> 16) & 0x7fffu));
+          for (int r = 0; r < 4; r += 2) {
+            const uint32_t y = qf[w][r] & 0x7fff7fffu, z = qf[w][r + 1] & 0x7fff7fffu;
+            hi = __vimax3_u16x2(hi, y, z);
+            lo = __vimin3_s16x2(lo, y + 0x7fff7fffu, z + 0x7fff7fffu);
+          }
         }
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // largest, and 2^16 less the smallest above zero (0: there is none)
+        uint32_t both = max(hi & 0xffffu, hi >> 16) |
+                        (uint32_t)(0x7fff - min((int)(int16_t)lo, (int)lo >> 16)) << 16;
+        both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 1));
+        both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, 2));
+        const uint32_t mx = both & 0xffffu, mn = 0x10000u - (both >> 16);
+        // If not, or if fp32 has no room for the raw scores, the second path takes all of the item.
+        fits = !__any_sync(0xffffffffu, mx >> 7 > 200 || (int)(mx >> 7) - (int)(mn >> 7) > (mn < 0x80u ? 20 : 27) ||
+                                                   !(fabsf(a.scale) < 0x1p40f));
         // 2^(14 - e) for a largest element in [2^e, 2^(e + 1)), as far as fp32 goes
         const int f = min(268 - (int)(mx >> 7), 254);
         const float up = __uint_as_float((uint32_t)f << 23);
@@ -608,255 +634,336 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
       for (int e = 0; e < HV; ++e) m[e] = -INFINITY, l[e] = 0.f;
       // Biased exponents of the largest V scale so far (at least this) and of the smallest in the tiles that set the
       // softmax reference; tiles from `room` on are left to the second path.  O is kept times 2^(kUp + 126 - ev).
-      int ev = kSpan + 1, low = 255, room = 0;
+      int ev = kSpan + 1, low = 255, room = fits ? 0 : -1;
       uint32_t from = 0;  // and a scale: bits 15 and 31 where the scale is at least 2^(ev - kSpan); 0: not set
 
-      for (int t = cs.t0 + wt; t < cs.t1 && !dead; t += T) {
-        const uint32_t st = used % kStages;
-        if (!warp_wait(&sm.full[warp][st], used / kStages & 1, a.err, abort)) {
-          dead = true;
-          break;
-        }
-        ++used;
-        const uint8_t* kb = sm.kv[warp][st][0];
-        const uint8_t* vb = sm.kv[warp][st][1];
-        const int lim = cs.ctx - t * kKv4Tile;  // tokens from here to the end of the context
-
-        // ---- S = K Q^T
-        float s[4][NV];
-#pragma unroll
-        for (int sb = 0; sb < 4; ++sb) {
-          const uint4 x4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + lane * 16);        // token g
-          const uint4 y4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + 512 + lane * 16);  // token g + 8
-          const uint2 sx = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + tok) * 8);
-          const uint2 sy = kCols == 4 ? sx : *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + tok + 8) * 8);
-          auto group = [&](auto W, uint32_t x, uint32_t y) {
-            constexpr int w = decltype(W)::value;
-            float acc[4];
-            const uint32_t a0[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
-            mma_f16_16816_from(acc, a0, qf[w][0], qf[w][1], corr[w][0], corr[w][HV - 1]);
-            x >>= 8;
-            y >>= 8;
-            const uint32_t a1[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
-            mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
-            const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-              const float v = kCols == 1 ? acc[i] : kCols == 2 ? acc[2 * i] : c & 1 ? acc[2] : acc[0];
-              const float f = i < HV ? fx : fy;
-              s[sb][i] = w == 0 ? v * f : fmaf(v, f, s[sb][i]);
-            }
-          };
-          group(std::integral_constant<int, 0>{}, x4.x, y4.x);
-          group(std::integral_constant<int, 1>{}, x4.y, y4.y);
-          group(std::integral_constant<int, 2>{}, x4.z, y4.z);
-          group(std::integral_constant<int, 3>{}, x4.w, y4.w);
-        }
-
-        // ---- the tile's V scales; lane: tokens 2 lane and 2 lane + 1.  Behind the context a scale may be anything:
-        // it becomes that of the tile's first token, and p zero.
-        uint4 vs = *(reinterpret_cast<const uint4*>(vb + kKv4Codes) + lane);
-        if (lim < kKv4Tile) {
-          const uint2 first = *reinterpret_cast<const uint2*>(vb + kKv4Codes);
-          if (2 * lane >= lim) vs.x = first.x, vs.y = first.y;
-          if (2 * lane + 1 >= lim) vs.z = first.x, vs.w = first.y;
-#pragma unroll
-          for (int sb = 0; sb < 4; ++sb)
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-              if (16 * sb + tok + i / HV * 8 >= lim) s[sb][i] = -INFINITY;
-        }
-        // Scales are not negative, so their bits order as they do: bits 15 and 31 stay where all are in range.
-        const uint32_t hi = __vmaxu2(__vimax3_u16x2(vs.x, vs.y, vs.z), vs.w);
-        const uint32_t lo = __vminu2(__vimin3_u16x2(vs.x, vs.y, vs.z), vs.w);
-        const bool odd = ~((lo + from) & (kUpTo - from - hi)) & 0x80008000u;
-
-        // ---- online softmax in the log2 domain.  The reference of the exponentials follows the maximum only when a
-        // score passes it by 2^kLag: p stays below that, and most tiles need no shuffles and no rescaling.
-        float x[HV];
-        bool above = false, wide = false;
-#pragma unroll
-        for (int e = 0; e < HV; ++e) {
-          x[e] = s[0][e];
-#pragma unroll
-          for (int i = 1; i < 4 * NV / HV; ++i) x[e] = fmaxf(x[e], s[i % 4][i / 4 * HV + e]);
-          x[e] *= sl[e];
-          above |= x[e] > m[e] + (float)kLag;
-        }
-        if (__any_sync(0xffffffffu, above || odd) || t >= room) {
-          const uint32_t big = __reduce_max_sync(0xffffffffu, max(hi & 0xffffu, hi >> 16));
-          const uint32_t least = __reduce_min_sync(0xffffffffu, min(lo & 0xffffu, lo >> 16));
-          const bool set = __any_sync(0xffffffffu, above);
-          const int e0 = ev;
-          if (big < 253u << 7) ev = max(ev, (int)(big >> 7));  // else the second path looks for the largest finite
-          const uint32_t from_v = (uint32_t)(ev - kSpan) << 7;
-          wide = big >= 253u << 7 || least < from_v;
-          from = (0x8000u - from_v) * 0x10001u;
-          const float up = ex2((float)(e0 - ev));
-          if (set) low = min(low, least < 0x80u ? -255 : (int)(least >> 7));
-          float al[HV];
-#pragma unroll
-          for (int e = 0; e < HV; ++e) {
-#pragma unroll
-            for (int d = kLow; d < 32; d += d == 1 ? 3 : d) x[e] = fmaxf(x[e], __shfl_xor_sync(0xffffffffu, x[e], d));
-            x[e] = set ? fmaxf(m[e], x[e]) : m[e];
-            const float f = ex2(m[e] - x[e]);
-            m[e] = x[e];
-            al[e] = set ? f * up : up;
-            l[e] *= set ? f : 1.f;
+      for (int t = cs.t0 + wt;; t += T) {
+        for (; t < cs.t1 && !dead; t += T) {
+          const uint32_t st = used % kStages;
+          if (!warp_wait(&sm.full[warp][st], used / kStages & 1, a.err, abort)) {
+            dead = true;
+            break;
           }
+          if (room < 0) break;
+          const uint8_t* kb = sm.kv[warp][st][0];
+          const uint8_t* vb = sm.kv[warp][st][1];
+          const int lim = cs.ctx - t * kKv4Tile;  // tokens from here to the end of the context
+
+          // ---- S = K Q^T
+          float s[4][NV];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int sb = 0; sb < 4; ++sb) {
+            const uint4 x4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + lane * 16);        // token g
+            const uint4 y4 = *reinterpret_cast<const uint4*>(kb + sb * 1024 + 512 + lane * 16);  // token g + 8
+            const uint2 sx = *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + tok) * 8);
+            const uint2 sy =
+                kCols == 4 ? sx : *reinterpret_cast<const uint2*>(kb + kKv4Codes + (16 * sb + tok + 8) * 8);
+            auto group = [&](auto W, uint32_t x, uint32_t y) {
+              constexpr int w = decltype(W)::value;
+              float acc[4];
+              const uint32_t a0[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
+              mma_f16_16816_from(acc, a0, qf[w][0], qf[w][1], corr[w][0], corr[w][HV - 1]);
+              x >>= 8;
+              y >>= 8;
+              const uint32_t a1[4] = {code_sub<false>(x), code_sub<false>(y), code_sub<true>(x), code_sub<true>(y)};
+              mma_f16_16816(acc, a1, qf[w][2], qf[w][3]);
+              const float fx = scale_of<w>(sx), fy = scale_of<w>(sy);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[j][i] *= al[i % HV];
-          room = cs.t0 + wt + (kv4_room(ev, low) << tsh);
-          wide |= t >= room;
-          if (wide) {
-            if (big >= 253u << 7) {
-              uint32_t f = 0;
-#pragma unroll 1
-              for (int i = 0; i < 8; ++i) {
-                const uint32_t u = *reinterpret_cast<const uint16_t*>(vb + kKv4Codes + 2 * (32 * i + lane)) & 0x7fffu;
-                if (u < 0x7f80u && 8 * i + lane / 4 < lim) f = max(f, u);
+              for (int i = 0; i < NV; ++i) {
+                const float v = kCols == 1 ? acc[i] : kCols == 2 ? acc[2 * i] : c & 1 ? acc[2] : acc[0];
+                const float f = i < HV ? fx : fy;
+                s[sb][i] = w == 0 ? v * f : fmaf(v, f, s[sb][i]);
               }
-              const int e = min((int)(__reduce_max_sync(0xffffffffu, f) >> 7), 252);
-              if (e > ev) {
-                const float r = ex2((float)(ev - e));
+            };
+            group(std::integral_constant<int, 0>{}, x4.x, y4.x);
+            group(std::integral_constant<int, 1>{}, x4.y, y4.y);
+            group(std::integral_constant<int, 2>{}, x4.z, y4.z);
+            group(std::integral_constant<int, 3>{}, x4.w, y4.w);
+          }
+
+          // ---- the tile's V scales; lane: tokens 2 lane and 2 lane + 1.  Behind the context a scale may be anything:
+          // it becomes that of the tile's first token, and p zero.
+          uint4 vs = *(reinterpret_cast<const uint4*>(vb + kKv4Codes) + lane);
+          if (lim < kKv4Tile) {
+            const uint2 first = *reinterpret_cast<const uint2*>(vb + kKv4Codes);
+            if (2 * lane >= lim) vs.x = first.x, vs.y = first.y;
+            if (2 * lane + 1 >= lim) vs.z = first.x, vs.w = first.y;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) o[j][i] *= r;
-                ev = e;
-                from = 0;  // the next tile sets the limits
-              }
-            }
-            // p s in fp32 as a sum of two bf16: 2^-17 of itself off, over all of fp32's range.  At other places than
-            // its own, a column's B is zero.
-            const float cw = __uint_as_float((uint32_t)(253 - ev) << 23);
-            float* mine = &sm.red_o[warp][0][lane];  // free until the segment ends
-#pragma unroll
-            for (int i = 0; i < 4 * NV; ++i) mine[32 * i] = s[i / NV][i % NV];
-#pragma unroll 1
-            for (int sb = 0; sb < 4; ++sb) {
-              const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);
-              const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);
-              const int t0 = 16 * sb + tok;
-              float p[NV];
+            for (int sb = 0; sb < 4; ++sb)
 #pragma unroll
               for (int i = 0; i < NV; ++i)
-                p[i] = t0 + i / HV * 8 < lim ? ex2(fmaf(mine[32 * (sb * NV + i)], sl[i % HV], (float)kUp - m[i % HV])) : 0.f;
-              uint2 sx = *reinterpret_cast<const uint2*>(vb + kKv4Codes + t0 * 8), sy = make_uint2(0, 0);
-              if constexpr (kCols < 4) sy = *reinterpret_cast<const uint2*>(vb + kKv4Codes + (t0 + 8) * 8);
-              if (t0 >= lim) sx = make_uint2(0, 0);
-              if (t0 + 8 >= lim) sy = make_uint2(0, 0);
-              auto group = [&](auto W) {
-                constexpr int w = decltype(W)::value;
-                const float fx = scale_of<w>(sx) * cw, fy = scale_of<w>(sy) * cw;
-                float v[4];
-                if constexpr (kCols == 1)
-                  v[0] = p[0] * fx, v[1] = p[1] * fx, v[2] = p[NV - 2] * fy, v[3] = p[NV - 1] * fy;
-                else if constexpr (kCols == 2)
-                  v[0] = p[0] * fx, v[1] = p[NV - 1] * fy, v[2] = v[3] = 0.f;
-                else
-                  v[0] = v[1] = p[0] * fx, v[2] = v[3] = 0.f;
-                constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
-                const uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
-                const uint32_t y = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
-                const uint32_t a0[4] = {code_bf16(x), code_bf16(x >> 4), code_bf16(y), code_bf16(y >> 4)};
-                const uint32_t a1[4] = {code_bf16(x >> 8), code_bf16(x >> 12), code_bf16(y >> 8), code_bf16(y >> 12)};
-#pragma unroll 1
-                for (int part = 0; part < 2; ++part) {
-                  const uint32_t u0 = pack_bf16(v[0], v[1]), u1 = pack_bf16(v[2], v[3]);
-                  const float2 r0 = unpack_bf16(u0), r1 = unpack_bf16(u1);
-                  v[0] -= r0.x, v[1] -= r0.y, v[2] -= r1.x, v[3] -= r1.y;
-                  const uint32_t t = movmatrix_trans(u0);
-                  uint32_t b0 = t, b1 = t;
-                  if constexpr (kCols == 1)
-                    b1 = movmatrix_trans(u1);
-                  else if constexpr (kCols == 2)
-                    b0 = g & 1 ? 0u : t, b1 = g & 1 ? t : 0u;
-                  else
-                    b0 = (g & 3) == 0 ? t : 0u, b1 = (g & 3) == 2 ? t : 0u;
-                  mma_bf16_16816(o[2 * w], a0, b0, b1);
-                  mma_bf16_16816(o[2 * w + 1], a1, b0, b1);
-                }
-              };
-              group(std::integral_constant<int, 0>{});
-              group(std::integral_constant<int, 1>{});
-              group(std::integral_constant<int, 2>{});
-              group(std::integral_constant<int, 3>{});
-            }
+                if (16 * sb + tok + i / HV * 8 >= lim) s[sb][i] = -INFINITY;
           }
-        }
-        {
-          const float cv = wide ? 0.f : __uint_as_float((uint32_t)(253 - ev) << 23);
-          const uint2 ta = make_uint2(vs.x, vs.y), tb = make_uint2(vs.z, vs.w);
-          sm.vpair[warp][lane] = make_uint4(pack_f16(scale_of<0>(ta) * cv, scale_of<0>(tb) * cv),
-                                            pack_f16(scale_of<1>(ta) * cv, scale_of<1>(tb) * cv),
-                                            pack_f16(scale_of<2>(ta) * cv, scale_of<2>(tb) * cv),
-                                            pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
-        }
+          // Scales are not negative, so their bits order as they do: bits 15 and 31 stay where all are in range.
+          const uint32_t hi = __vmaxu2(__vimax3_u16x2(vs.x, vs.y, vs.z), vs.w);
+          const uint32_t lo = __vminu2(__vimin3_u16x2(vs.x, vs.y, vs.z), vs.w);
+          const bool odd = ~((lo + from) & (kUpTo - from - hi)) & 0x80008000u;
+
+          // ---- online softmax in the log2 domain.  The reference of the exponentials follows the maximum only when a
+          // score passes it by 2^kLag: p stays below that, and most tiles need no shuffles and no rescaling.
+          float x[HV];
+          bool above = false;
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
+          for (int e = 0; e < HV; ++e) {
+            x[e] = s[0][e];
 #pragma unroll
-          for (int i = 0; i < NV; ++i) s[sb][i] = ex2(fmaf(s[sb][i], sl[i % HV], (float)kUp - m[i % HV]));  // 2^kUp p
-        if (lim < kKv4Tile) {  // also where a scale of 0 makes -inf * 0 a NaN
+            for (int i = 1; i < 4 * NV / HV; ++i) x[e] = fmaxf(x[e], s[i % 4][i / 4 * HV + e]);
+            x[e] *= sl[e];
+            above |= x[e] > m[e] + (float)kLag;
+          }
+          if (__any_sync(0xffffffffu, above || odd) || t >= room) {
+            const uint32_t big = __reduce_max_sync(0xffffffffu, max(hi & 0xffffu, hi >> 16));
+            const uint32_t least = __reduce_min_sync(0xffffffffu, min(lo & 0xffffu, lo >> 16));
+            const bool set = __any_sync(0xffffffffu, above);
+            const int e0 = ev;
+            if (big < 253u << 7) ev = max(ev, (int)(big >> 7));  // else the second path does
+            const uint32_t from_v = (uint32_t)(ev - kSpan) << 7;
+            const bool wide = big >= 253u << 7 || least < from_v;
+            from = (0x8000u - from_v) * 0x10001u;
+            const float up = ex2((float)(e0 - ev));
+            if (set) low = min(low, least < 0x80u ? kNone : (int)(least >> 7));
+            float al[HV];
+#pragma unroll
+            for (int e = 0; e < HV; ++e) {
+#pragma unroll
+              for (int d = kLow; d < 32; d += d == 1 ? 3 : d) x[e] = fmaxf(x[e], __shfl_xor_sync(0xffffffffu, x[e], d));
+              x[e] = set ? fmaxf(m[e], x[e]) : m[e];
+              const float f = ex2(m[e] - x[e]);
+              m[e] = x[e];
+              al[e] = set ? f * up : up;
+              l[e] *= set ? f : 1.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[j][i] *= al[i % HV];
+            room = cs.t0 + wt + (kv4_room(ev, low) << tsh);
+            if (wide || t >= room) break;
+          }
+          {
+            const float cv = __uint_as_float((uint32_t)(253 - ev) << 23);
+            const uint2 ta = make_uint2(vs.x, vs.y), tb = make_uint2(vs.z, vs.w);
+            sm.vpair[warp][lane] = make_uint4(pack_f16(scale_of<0>(ta) * cv, scale_of<0>(tb) * cv),
+                                              pack_f16(scale_of<1>(ta) * cv, scale_of<1>(tb) * cv),
+                                              pack_f16(scale_of<2>(ta) * cv, scale_of<2>(tb) * cv),
+                                              pack_f16(scale_of<3>(ta) * cv, scale_of<3>(tb) * cv));
+          }
 #pragma unroll
           for (int sb = 0; sb < 4; ++sb)
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-              if (16 * sb + tok + i / HV * 8 >= lim) s[sb][i] = 0.f;
+            for (int i = 0; i < NV; ++i) s[sb][i] = ex2(fmaf(s[sb][i], sl[i % HV], (float)kUp - m[i % HV]));  // 2^kUp p
+          if (lim < kKv4Tile) {  // also where a scale of 0 makes -inf * 0 a NaN
+#pragma unroll
+            for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+              for (int i = 0; i < NV; ++i)
+                if (16 * sb + tok + i / HV * 8 >= lim) s[sb][i] = 0.f;
+          }
+#pragma unroll
+          for (int sb = 0; sb < 4; ++sb)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) l[i % HV] += s[sb][i];
+          __syncwarp();  // vpair is written
+
+          // ---- O^T += V^T P^T
+          uint32_t pt = 0;
+#pragma unroll
+          for (int sb = 0; sb < 4; ++sb) {
+            const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
+            const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
+            const uint4 sx = sm.vpair[warp][sb * 8 + c], sy = sm.vpair[warp][sb * 8 + 4 + c];
+            uint32_t px, py;  // column g: its head's tokens 2c, 2c + 1 and ... + 8
+            if constexpr (kCols == 1) {
+              px = movmatrix_trans(pack_f16(s[sb][0], s[sb][1]));
+              py = movmatrix_trans(pack_f16(s[sb][NV - 2], s[sb][NV - 1]));
+            } else if constexpr (kCols == 2) {
+              // A head's even column takes tokens 0 .. 7, its odd one 8 .. 15: one transpose for both.
+              const uint32_t y = movmatrix_trans(pack_f16(s[sb][0], s[sb][NV - 1]));
+              px = g & 1 ? 0u : y;
+              py = g & 1 ? y : 0u;
+            } else {
+              // Columns 4 h and 4 h + 1 take tokens 0 .. 7 of even and of odd sb, + 2 and + 3 tokens 8 .. 15.
+              if (sb % 2 == 0) pt = movmatrix_trans(pack_f16(s[sb][0], s[(sb + 1) % 4][0]));
+              px = (g & 3) == sb % 2 ? pt : 0u;
+              py = (g & 3) == sb % 2 + 2 ? pt : 0u;
+            }
+            auto group = [&](auto W) {  // 32 dims: j = 2w and 2w + 1
+              constexpr int w = decltype(W)::value;
+              const uint32_t b0 = mul_f16(px, w == 0 ? sx.x : w == 1 ? sx.y : w == 2 ? sx.z : sx.w);
+              const uint32_t b1 = mul_f16(py, w == 0 ? sy.x : w == 1 ? sy.y : w == 2 ? sy.z : sy.w);
+              // 16 bits of tokens 2c | 2c + 1 each: four nibbles = dims 16 j + 2g, + 1 of j = 2w, 2w + 1
+              constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
+              uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
+              uint32_t y = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
+              const uint32_t a0[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
+              mma_f16_16816(o[2 * w], a0, b0, b1);
+              x >>= 8;
+              y >>= 8;
+              const uint32_t a1[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
+              mma_f16_16816(o[2 * w + 1], a1, b0, b1);
+            };
+            group(std::integral_constant<int, 0>{});
+            group(std::integral_constant<int, 1>{});
+            group(std::integral_constant<int, 2>{});
+            group(std::integral_constant<int, 3>{});
+          }
+          __syncwarp();  // every lane has read the stage
+          if (lane == 0) mbar_arrive(&sm.empty[warp][st]);
+          ++used;
+        }
+        if (t >= cs.t1 || dead) break;
+        // ---- this tile on the second path: the scores first
+        const uint32_t st = used % kStages;
+        const uint8_t* kb = sm.kv[warp][st][0];
+        const uint8_t* vb = sm.kv[warp][st][1];
+        const int lim = cs.ctx - t * kKv4Tile;
+        float* mine = &sm.red_o[warp][0][lane];  // free until the segment ends: this lane's scores, then p
+        float x[HV];
+#pragma unroll
+        for (int e = 0; e < HV; ++e) x[e] = -INFINITY;
+        {
+          const uint4* qp = reinterpret_cast<const uint4*>(a.q + (qh0 + min(qh, G - 1)) * 128 + 8 * c);
+          uint32_t mx = 0;
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {
+            const uint4 y = qp[4 * w];
+            mx = __vimax3_u16x2(mx, __vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu),
+                                __vmaxu2(y.z & 0x7fff7fffu, y.w & 0x7fff7fffu));
+          }
+          mx = max(mx & 0xffffu, mx >> 16);
+          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const int by = kv4_q_exp(a.scale, mx);
+          const float up = copysignf(exp2i(by), a.scale);
+          float sw[HV];
+#pragma unroll
+          for (int e = 0; e < HV; ++e)
+            sw[e] = __shfl_sync(0xffffffffu, fabsf(a.scale) * kLog2e * exp2i(-by), 8 * c + 4 * e);
+#pragma unroll 1
+          for (int sb = 0; sb < 4; ++sb) {
+            float y[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) y[i] = 0.f;
+#pragma unroll 1
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t u = *reinterpret_cast<const uint32_t*>(kb + sb * 1024 + lane * 16 + 4 * w);
+              const uint32_t v = *reinterpret_cast<const uint32_t*>(kb + sb * 1024 + 512 + lane * 16 + 4 * w);
+              const uint8_t* sp = kb + kKv4Codes + (16 * sb + tok) * 8 + 2 * w;
+              const float fx = bf16_bits(*reinterpret_cast<const uint16_t*>(sp));
+              const float fy = kCols == 4 ? fx : bf16_bits(*reinterpret_cast<const uint16_t*>(sp + 64));
+              const uint4 qw = qp[4 * w];
+              auto pair = [&](uint32_t z) {
+                const float2 f = unpack_bf16(z);
+                return pack_bf16(f.x * up, f.y * up);
+              };
+              float acc[4] = {0.f, 0.f, 0.f, 0.f};
+              const uint32_t a0[4] = {code_bf16(u), code_bf16(v), code_bf16(u >> 4), code_bf16(v >> 4)};
+              mma_bf16_16816(acc, a0, pair(qw.x), pair(qw.y));
+              const uint32_t a1[4] = {code_bf16(u >> 8), code_bf16(v >> 8), code_bf16(u >> 12), code_bf16(v >> 12)};
+              mma_bf16_16816(acc, a1, pair(qw.z), pair(qw.w));
+#pragma unroll
+              for (int i = 0; i < NV; ++i) {
+                const float z = kCols == 1 ? acc[i] : kCols == 2 ? acc[2 * i] : c & 1 ? acc[2] : acc[0];
+                y[i] = fmaf(z, i < HV ? fx : fy, y[i]);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              const float z = 16 * sb + tok + i / HV * 8 < lim ? y[i] * sw[i % HV] : -INFINITY;
+              mine[32 * (sb * NV + i)] = z;
+              x[i % HV] = fmaxf(x[i % HV], z);
+            }
+          }
+        }
+        // the reference of the softmax, and the largest finite V scale
+        bool above = false;
+#pragma unroll
+        for (int e = 0; e < HV; ++e) above |= x[e] > m[e] + (float)kLag;
+        const bool set = __any_sync(0xffffffffu, above);
+        if (set) low = kNone;
+        uint32_t top = 0;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t u = *reinterpret_cast<const uint16_t*>(vb + kKv4Codes + 2 * (32 * i + lane)) & 0x7fffu;
+          if (u < 0x7f80u && 8 * i + lane / 4 < lim) top = max(top, u);
+        }
+        const int e0 = ev;
+        ev = max(ev, min((int)(__reduce_max_sync(0xffffffffu, top) >> 7), 252));
+        if (ev > e0) from = 0;  // the next tile sets its limits
+        const float up = ex2((float)(e0 - ev));
+        float al[HV];
+#pragma unroll
+        for (int e = 0; e < HV; ++e) {
+#pragma unroll
+          for (int d = kLow; d < 32; d += d == 1 ? 3 : d) x[e] = fmaxf(x[e], __shfl_xor_sync(0xffffffffu, x[e], d));
+          x[e] = set ? fmaxf(m[e], x[e]) : m[e];
+          const float f = set ? ex2(m[e] - x[e]) : 1.f;
+          m[e] = x[e];
+          al[e] = f * up;
+          l[e] *= f;
         }
 #pragma unroll
-        for (int sb = 0; sb < 4; ++sb)
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int i = 0; i < NV; ++i) l[i % HV] += s[sb][i];
-        __syncwarp();  // vpair is written
-
-        // ---- O^T += V^T P^T
-        uint32_t pt = 0;
-#pragma unroll
+          for (int i = 0; i < 4; ++i) o[j][i] *= al[i % HV];
+        // p s as a sum of two bf16: 2^-17 of itself off, over all of fp32's range.  A column's B is zero at the places
+        // of tokens that are another's.
+        const float cw = __uint_as_float((uint32_t)(253 - ev) << 23);
+#pragma unroll 1
         for (int sb = 0; sb < 4; ++sb) {
-          const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);        // tokens 2c, 2c + 1
-          const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);  // ... + 8
-          const uint4 sx = sm.vpair[warp][sb * 8 + c], sy = sm.vpair[warp][sb * 8 + 4 + c];
-          uint32_t px, py;  // column g: its head's tokens 2c, 2c + 1 and ... + 8
-          if constexpr (kCols == 1) {
-            px = movmatrix_trans(pack_f16(s[sb][0], s[sb][1]));
-            py = movmatrix_trans(pack_f16(s[sb][NV - 2], s[sb][NV - 1]));
-          } else if constexpr (kCols == 2) {
-            // A head's even column takes tokens 0 .. 7, its odd one 8 .. 15: one transpose for both.
-            const uint32_t y = movmatrix_trans(pack_f16(s[sb][0], s[sb][NV - 1]));
-            px = g & 1 ? 0u : y;
-            py = g & 1 ? y : 0u;
-          } else {
-            // Columns 4 h and 4 h + 1 take tokens 0 .. 7 of even and of odd sb, + 2 and + 3 tokens 8 .. 15.
-            if (sb % 2 == 0) pt = movmatrix_trans(pack_f16(s[sb][0], s[(sb + 1) % 4][0]));
-            px = (g & 3) == sb % 2 ? pt : 0u;
-            py = (g & 3) == sb % 2 + 2 ? pt : 0u;
+          const uint4 x4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + lane * 16);
+          const uint4 y4 = *reinterpret_cast<const uint4*>(vb + sb * 1024 + 512 + lane * 16);
+          const int t0 = 16 * sb + tok;
+          float p[NV];
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            p[i] = t0 + i / HV * 8 < lim ? ex2(mine[32 * (sb * NV + i)] + ((float)kUp - m[i % HV])) : 0.f;
+            l[i % HV] += p[i];
           }
-          auto group = [&](auto W) {  // 32 dims: j = 2w and 2w + 1
+          uint2 sx = *reinterpret_cast<const uint2*>(vb + kKv4Codes + t0 * 8), sy = make_uint2(0, 0);
+          if constexpr (kCols < 4) sy = *reinterpret_cast<const uint2*>(vb + kKv4Codes + (t0 + 8) * 8);
+          if (t0 >= lim) sx = make_uint2(0, 0);
+          if (t0 + 8 >= lim) sy = make_uint2(0, 0);
+          auto group = [&](auto W) {
             constexpr int w = decltype(W)::value;
-            const uint32_t b0 = mul_f16(px, w == 0 ? sx.x : w == 1 ? sx.y : w == 2 ? sx.z : sx.w);
-            const uint32_t b1 = mul_f16(py, w == 0 ? sy.x : w == 1 ? sy.y : w == 2 ? sy.z : sy.w);
-            // 16 bits of tokens 2c | 2c + 1 each: four nibbles = dims 16 j + 2g, + 1 of j = 2w, 2w + 1
+            const float fx = scale_of<w>(sx) * cw, fy = scale_of<w>(sy) * cw;
+            float v[4];
+            if constexpr (kCols == 1)
+              v[0] = p[0] * fx, v[1] = p[1] * fx, v[2] = p[NV - 2] * fy, v[3] = p[NV - 1] * fy;
+            else if constexpr (kCols == 2)
+              v[0] = p[0] * fx, v[1] = p[NV - 1] * fy, v[2] = v[3] = 0.f;
+            else
+              v[0] = v[1] = p[0] * fx, v[2] = v[3] = 0.f;
             constexpr uint32_t sel = (w & 1) ? 0x7632u : 0x5410u;
-            uint32_t x = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
-            uint32_t y = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
-            const uint32_t a0[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
-            mma_f16_16816(o[2 * w], a0, b0, b1);
-            x >>= 8;
-            y >>= 8;
-            const uint32_t a1[4] = {code<false>(x), code<true>(x), code<false>(y), code<true>(y)};
-            mma_f16_16816(o[2 * w + 1], a1, b0, b1);
+            const uint32_t y = w < 2 ? __byte_perm(x4.x, x4.z, sel) : __byte_perm(x4.y, x4.w, sel);
+            const uint32_t z = w < 2 ? __byte_perm(y4.x, y4.z, sel) : __byte_perm(y4.y, y4.w, sel);
+            const uint32_t a0[4] = {code_bf16(y), code_bf16(y >> 4), code_bf16(z), code_bf16(z >> 4)};
+            const uint32_t a1[4] = {code_bf16(y >> 8), code_bf16(y >> 12), code_bf16(z >> 8), code_bf16(z >> 12)};
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+              const uint32_t u0 = pack_bf16(v[0], v[1]), u1 = pack_bf16(v[2], v[3]);
+              const float2 r0 = unpack_bf16(u0), r1 = unpack_bf16(u1);
+              v[0] -= r0.x, v[1] -= r0.y, v[2] -= r1.x, v[3] -= r1.y;
+              const uint32_t u = movmatrix_trans(u0);
+              uint32_t b0 = u, b1 = u;
+              if constexpr (kCols == 1)
+                b1 = movmatrix_trans(u1);
+              else if constexpr (kCols == 2)
+                b0 = g & 1 ? 0u : u, b1 = g & 1 ? u : 0u;
+              else
+                b0 = (g & 3) == 0 ? u : 0u, b1 = (g & 3) == 2 ? u : 0u;
+              mma_bf16_16816(o[2 * w], a0, b0, b1);
+              mma_bf16_16816(o[2 * w + 1], a1, b0, b1);
+            }
           };
           group(std::integral_constant<int, 0>{});
           group(std::integral_constant<int, 1>{});
           group(std::integral_constant<int, 2>{});
           group(std::integral_constant<int, 3>{});
         }
-        __syncwarp();  // every lane has read the stage
+        __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[warp][st]);
+        ++used;
       }
 
       // ---- end of the segment: the team's warps meet in shared memory

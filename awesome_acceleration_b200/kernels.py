@@ -292,7 +292,8 @@ def kv4_decode_attention(q, k_cache, v_cache, block_tables, rows, seqlens, *, ct
                          max_context: int, workspace: torch.Tensor, out=None) -> torch.Tensor:
     """q [B, Hq, 128] -> out [B, Hq, 128] over seqlens[rows[b]] + ctx_add
     tokens of the 4-bit pools (paged_decode_attention over the bf16 cache).
-    V scales count in full down to 2^-100 of the largest of a row's context.
+    V scales count in full down to 2^-100 of the largest of a row's context, elements of q down to 2^-100 of the
+    largest of their head.
     Calls that share `workspace` (uint8) must be ordered on one stream."""
     what = "kv4_decode_attention"
     if out is None:

@@ -218,8 +218,9 @@ int64_t aacc_kv4_decode_workspace_bytes(int num_q_heads, int num_kv_heads);
  * aacc_paged_decode_attention.  A context longer than max_context is cut
  * there (error word bit 32); an empty one, a padding row (negative slot
  * index) or one outside [0, num_rows) (bit 2) gives zeros.  V scales count in
- * full down to 2^-100 of the largest that a row's context has in that head; a
- * NaN scale of V spoils its 32 dims, one of K the heads that attend to it.
+ * full down to 2^-100 of the largest that a row's context has in that head,
+ * and the elements of q down to 2^-100 of their head's largest.  A NaN scale
+ * of V spoils its 32 dims, one of K the heads that attend to it.
  * Calls that share a workspace must be ordered on one stream. */
 int aacc_kv4_decode_attention(const void* q, void* out, const void* k_cache, const void* v_cache, int64_t num_blocks,
                               const int32_t* block_tables, int64_t num_rows, int64_t max_blocks,

@@ -190,3 +190,60 @@ def test_v_groups_that_are_not_finite_among_scales_of_every_size(cuda, G):
     check(out, c)
     bad = torch.isnan(out)
     assert bad[0, G:, 32:64].all() and bad.sum() == 32 * G
+
+
+# --------------------------------------------------------------------------- queries of very different magnitude
+@pytest.mark.parametrize("e", [-20, -28, -40, -60, -90])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_small_query_elements_that_meet_large_keys(cuda, G, e):
+    """One group of q at 2^e of the others, where K is 2^-e times the others': all groups count alike in a logit."""
+    c = make_case([200, 65, 2], G, 2, 64, 170 + G)
+    up = torch.ones(4, 32)
+    up[G % 4] = 2.0 ** -e
+    k = rows(c, 171, 2).float().view(-1, 2, 4, 32) * up
+    c["kp"] = O.pool_from_rows(k.view(-1, 2, 128).to(BF), 64, False)
+    c["q"] = (c["q"].float().view(3, -1, 4, 32) / up).view(3, -1, 128).to(BF)
+    for scale in (SCALE, -SCALE, 2.0):
+        check_v(call(c, cuda, scale=scale), c, scale=scale)
+
+
+@pytest.mark.parametrize("top", [110, 125, -100, -124])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_queries_at_the_ends_of_bf16(cuda, G, top):
+    """q near 2^top and K near 2^-top: ordinary logits.  Other heads of the same kv head have q of zero or tiny q."""
+    c = make_case([130, 1], G, 2, 64, 180 + G)
+    low = max(-top, -120)
+    k = rows(c, 181, 2).float() * 2.0 ** low
+    c["kp"] = O.pool_from_rows(k.to(BF), 64, False)
+    q = c["q"].float().clamp(-3, 3) * 2.0 ** (min(-low, 125))
+    if G > 1:
+        q[:, 1] = 0
+        q[:, 2 * G - 1] *= 2.0 ** -60
+    c["q"] = q.to(BF)
+    check_v(call(c, cuda), c)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-38, 1e30, 0.0])
+def test_softmax_scales_of_every_size(cuda, scale):
+    """A scale that q or K makes up for."""
+    for G in (2, 8):
+        c = make_case([130, 3], G, 2, 64, 190 + G)
+        f = 1.0 if scale == 0 else 0.1 / scale
+        a = 2.0 ** round(math.log2(f) / 2)
+        k = rows(c, 191, 2).float() * a
+        c["kp"] = O.pool_from_rows(k.to(BF), 64, False)
+        c["q"] = (c["q"].float() * a).to(BF)
+        check_v(call(c, cuda, scale=scale), c, scale=scale)
+
+
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_a_query_that_is_not_finite_spoils_its_own_head_only(cuda, G):
+    c = make_case([150, 20], G, 2, 64, 200 + G)
+    clean = c["q"].clone()
+    for bad in (math.nan, math.inf, -math.inf):
+        c["q"] = clean.clone()
+        c["q"][0, G, 17] = bad
+        out = call(c, cuda).cpu()
+        nan = torch.isnan(out)
+        assert nan[0, G].all() and nan.sum() == 128
+        check(out, c)
