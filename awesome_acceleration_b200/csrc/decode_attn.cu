@@ -15,6 +15,7 @@
 //
 // The kernel is HBM-bound: each K/V byte of the context is read once per
 // kv head.  Algorithmic bytes per call = sum(ctx) * Hkv * 128 * 2 * 2.
+#include <algorithm>
 #include <mutex>
 
 #include "common.cuh"
@@ -288,13 +289,15 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
 // A/B): cfg2 engine step, attention only, ctx 1536: 7.70 ms at 512-token
 // splits, 6.76 ms at 2048; cfg3 (ctx U[512,4096]): 6.02 / 6.40 / 6.45 /
 // 6.36 TB/s at 512 / 1024 / 2048 / unsplit.
+constexpr int64_t kTargetCtas = 148 * 8;  // to keep every SM busy (two resident, several waves)
+constexpr int kMaxSplit = 2048;
+
 static int default_split(int64_t batch, int Hkv, int64_t max_ctx) {
-  const int64_t target = 148 * 8;  // CTAs to keep every SM busy (two resident, several waves)
-  int64_t want = (target + batch * Hkv - 1) / (batch * Hkv);
+  int64_t want = (kTargetCtas + batch * Hkv - 1) / (batch * Hkv);
   int64_t split = (max_ctx + want - 1) / want;
   split = ((split + kTile - 1) / kTile) * kTile;
   if (split < kTile) split = kTile;
-  if (split > 2048) split = 2048;
+  if (split > kMaxSplit) split = kMaxSplit;
   return (int)split;
 }
 
@@ -324,12 +327,16 @@ using namespace aacc;
 extern "C" {
 
 int64_t aacc_paged_decode_workspace_bytes(int64_t batch, int num_q_heads, int64_t max_context, int split_tokens) {
-  if (split_tokens <= 0) split_tokens = default_split(batch, 1, max_context);  // upper bound on splits
-  int64_t max_splits = (max_context + split_tokens - 1) / split_tokens;
-  if (max_splits < 1) max_splits = 1;
-  // partial O | partial (max, sum) | one merge counter per (row, kv head) (<= q heads)
-  return batch * num_q_heads * max_splits * (kD + 2) * (int64_t)sizeof(float) +
-         batch * num_q_heads * (int64_t)sizeof(int);
+  if (batch <= 0 || num_q_heads <= 0) return 0;
+  auto splits = [&](int64_t split) { return (max_context + split - 1) / split; };
+  // Rows x splits of any call of 1 .. batch rows: by default a call has no more splits than CTAs to aim at, rounded up
+  // for each row, unless they would be longer than kMaxSplit.
+  int64_t parts = split_tokens > 0 ? batch * splits(split_tokens)
+                                   : std::min(batch * splits(kTile),
+                                              std::max(kTargetCtas + batch, batch * splits(kMaxSplit)));
+  parts = std::max(parts, batch);
+  // partial O and (max, sum); at the end one merge counter per (row, kv head) (<= q heads)
+  return parts * num_q_heads * (kD + 2) * (int64_t)sizeof(float) + batch * num_q_heads * (int64_t)sizeof(int);
 }
 
 int aacc_paged_decode_attention(const void* q, void* out, const void* k_cache, const void* v_cache, int64_t num_blocks,
@@ -348,7 +355,7 @@ int aacc_paged_decode_attention(const void* q, void* out, const void* k_cache, c
   const int max_splits = (int)((max_context + split_tokens - 1) / split_tokens);
   if (max_splits > 1) {
     const int64_t need = batch * num_q_heads * (int64_t)max_splits * (kD + 2) * (int64_t)sizeof(float) +
-                         batch * num_kv_heads * (int64_t)sizeof(int);
+                         batch * num_kv_heads * (int64_t)sizeof(int) + (workspace_bytes & 3);
     if (!workspace || workspace_bytes < need)
       return set_error(AACC_ERR_INVALID, "paged_decode_attention: workspace %lld < %lld bytes",
                        (long long)workspace_bytes, (long long)need);
@@ -360,7 +367,11 @@ int aacc_paged_decode_attention(const void* q, void* out, const void* k_cache, c
   if (st) return st;
   float* ws_o = static_cast<float*>(workspace);
   float* ws_ml = ws_o ? ws_o + batch * num_q_heads * (int64_t)max_splits * kD : nullptr;
-  int* cnt = ws_ml ? reinterpret_cast<int*>(ws_ml + batch * num_q_heads * (int64_t)max_splits * 2) : nullptr;
+  // The counters lie at the workspace's end, so that where they are does not depend on the call's shape: a call of
+  // other rows or splits must not find partials of an earlier one in their place.
+  int* cnt = ws_o && workspace_bytes >= batch * num_kv_heads * (int64_t)sizeof(int)
+                 ? reinterpret_cast<int*>(static_cast<char*>(workspace) + workspace_bytes / 4 * 4) - batch * num_kv_heads
+                 : nullptr;
   const float scale_log2 = scale * kLog2e;
   unsigned* err = device_error_ptr();
   dim3 grid(max_splits, num_kv_heads, (unsigned)batch);
@@ -462,7 +473,8 @@ int aacc_paged_decode_attention_noalloc(const void* q, void* out, const void* k_
   st = noalloc_scratch(&scratch);
   if (st) return st;
   if (max_splits > 1) {
-    cudaError_t e = cudaMemsetAsync(static_cast<char*>(scratch) + partial_bytes, 0, counter_bytes, stream);
+    cudaError_t e = cudaMemsetAsync(static_cast<char*>(scratch) + kNoAllocScratchBytes - counter_bytes, 0,
+                                    counter_bytes, stream);
     if (e != cudaSuccess)
       return set_error(AACC_ERR_CUDA, "paged_decode_attention_noalloc: clearing counters: %s", cudaGetErrorString(e));
   }

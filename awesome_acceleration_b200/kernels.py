@@ -65,6 +65,8 @@ def gather_rows(src: torch.Tensor, idx: torch.Tensor, out: torch.Tensor | None =
 
 # ---------------------------------------------------------------- attention
 def decode_workspace_bytes(batch: int, num_q_heads: int, max_context: int, split_tokens: int = 0) -> int:
+    """Workspace of paged_decode_attention (zero-filled before its first use) for calls of up to `batch` rows and
+    `max_context` tokens, which may share it in turn."""
     return int(_lib_().aacc_paged_decode_workspace_bytes(batch, num_q_heads, max_context, split_tokens))
 
 

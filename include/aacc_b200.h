@@ -87,9 +87,11 @@ int aacc_gather_rows(const void* src, int64_t n_src, int64_t row_bytes, const in
 
 /* ---- attention ----------------------------------------------------------- */
 
-/* Workspace bytes aacc_paged_decode_attention needs for `batch` rows with at
- * most `max_context` tokens each.  The workspace must be zero-filled before
- * its first use (it holds merge counters that every call leaves at zero). */
+/* Workspace bytes aacc_paged_decode_attention needs for calls of up to `batch`
+ * rows with at most `max_context` tokens each.  The workspace must be
+ * zero-filled before its first use (its end holds merge counters that every
+ * call leaves at zero).  Calls of up to that many rows, of any number, may
+ * share it in turn. */
 int64_t aacc_paged_decode_workspace_bytes(int64_t batch, int num_q_heads, int64_t max_context,
                                           int split_tokens);
 
