@@ -704,6 +704,7 @@ class Qwen3Runtime:
             xs, rs, ds = x[:Tc], res[:Tc], delta[:Tc]
             K.embed_rmsnorm(ids_d[t0:t0 + Tc], self.embed, self.layers[0].in_ln, self.eps, rs, xs)
 
+            attend = None  # with it goes the chunk before's scratch
             slots, attend = self._prefill_chunk(seq_rows, cu_q, ctx0, [e for _, _, e in ch], max_q,
                                                 meta[2:, t0:t0 + Tc])
             self._layer_chain(xs, rs, ds, q[:Tc], attn[:Tc], act[:Tc], attend, pos_d[t0:t0 + Tc], slots)
@@ -786,6 +787,7 @@ class Qwen3RuntimeKV4(Qwen3Runtime):
         _, _, dst = K.build_slot_maps(total, tables, num_tokens=n_ctx, block_size=bs, num_blocks=n_blk)
         rows = torch.arange(len(ends), dtype=torch.int64, device=self.device)
         if self._stage is self._stage_decode or self._stage[0].shape[0] < n_new:
+            self._stage = self._stage_decode  # not two of a prefill's at once
             self._stage = self._staging(n_new)
         # Zero-filled: the attention multiplies the tail of a sequence's last tile by p = 0.
         k, v = torch.zeros((2, n_blk, self.Hkv, bs, 128), dtype=torch.bfloat16, device=self.device)
