@@ -161,3 +161,25 @@ def test_sizing_leaves_room_for_a_chunk_of_many_short_prompts(monkeypatch):
     scratch = n * Qwen3RuntimeKV4.SCRATCH_BLOCK * 4 * 128 * 2 * 2  # n prompts of one token in one chunk
     rows = chunk * 4 * 128 * 2 * 2
     assert 1 < n < want and pool + scratch + rows <= free - (1 << 30)
+
+
+def test_tensor_parallel_cache_has_its_ranks_heads():
+    """A rank's 4-bit cache holds its share of the kv heads, and its runtime is the 4-bit one."""
+    from awesome_acceleration_b200 import runtime as R
+    from awesome_acceleration_b200.kv_cache import PagedKV4Cache
+    from awesome_acceleration_b200.model import model_tp
+    from awesome_acceleration_b200.model.model import Qwen3Config
+    cfg = Qwen3Config(hidden_size=512, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=4, head_dim=128,
+                      intermediate_size=1024, vocab_size=256)
+    with torch.device("meta"):
+        m = model_tp.Qwen3ForCausalLMTP(cfg)
+    m.tp_size = 2
+    m.init_kv_cache(3, 500, "cpu", torch.bfloat16, block_size=128, kv_bits=4)
+    assert isinstance(m.kv, PagedKV4Cache) and m.kv.num_kv_heads == 2
+    assert m.kv.k.shape == (2, m.kv.num_blocks, 2, 2, 4608) and m.max_batch == 3
+    assert m.model.layers[1].self_attn._kv_cache.data_ptr() == m.kv.k[1].data_ptr()
+    assert R.runtime_class(m.kv) is R.Qwen3RuntimeKV4
+    m.init_kv_cache(3, 500, "cpu", torch.bfloat16, block_size=128)
+    assert m.kv.bits == 16 and R.runtime_class(m.kv) is R.Qwen3Runtime
+    with pytest.raises(ValueError, match="kv_bits"):
+        m.init_kv_cache(3, 500, "cpu", torch.bfloat16, kv_bits=8)
