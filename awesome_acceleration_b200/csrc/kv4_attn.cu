@@ -65,14 +65,14 @@
 // on, and n tiles of 64 tokens lose at most 2^-16 D while
 // n <= 2^(kUp + 1 + low - e): 2^7 tiles, 8192 tokens of one warp, for scales
 // within 2^6 of one another.  Later tiles, and tiles with a scale below
-// 2^-kSpan of the largest (zero among them) or a NaN, take a second path: codes
-// and q in bf16, no product rounded; p s in fp32, cut into two bf16 that two
-// MMAs add up.  O is held relative to the largest scale and q to its largest
-// element, so that what lies 2^-100 below them still counts in full.  A tile takes
-// 3.6 times as long on it, in loops that are rolled so that the first path keeps
-// its registers (256 rows with one token in 16 at 2^-20 of the others: 433 us,
-// without 119; with the loops unrolled, or in a function of its own, 256 x 1500
-// at 64/8 heads take 99 or 105 us on the first path, and so 96).
+// 2^-kSpan of the largest (zero among others) or a NaN, take a second path:
+// codes and q in bf16, no product rounded; p s in fp32, cut into two bf16 that
+// two MMAs add up.  O is held relative to the largest scale and q to its
+// largest element, so that what lies 2^-100 below them still counts in full.  A
+// tile takes 3.6 times as long on it, in loops that are rolled so that the first
+// path keeps its registers (256 rows with one token in 16 at 2^-20 of the
+// others: 433 us, without 119; with the loops unrolled, or in a function of its
+// own, 256 x 1500 at 64/8 heads take 99 or 105 us on the first path, and so 96).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -738,7 +738,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
 #pragma unroll
               for (int i = 0; i < 4; ++i) o[j][i] *= al[i % HV];
             room = cs.t0 + wt + (kv4_room(ev, low) << tsh);
-            if (wide || t >= room) break;
+            if ((wide || t >= room) && big) break;  // fp16 loses nothing of zeros
           }
           {
             const float cv = __uint_as_float((uint32_t)(253 - ev) << 23);

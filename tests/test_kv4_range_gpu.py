@@ -247,3 +247,19 @@ def test_a_query_that_is_not_finite_spoils_its_own_head_only(cuda, G):
         nan = torch.isnan(out)
         assert nan[0, G].all() and nan.sum() == 128
         check(out, c)
+
+
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_tiles_of_zeros(cuda, G):
+    """A pool never written reads as zeros; tiles and tokens of zero V before, between and after others, with most of
+    the probability or little of it."""
+    for e in (0, 30):
+        for pick in (lambda t: t < 64, lambda t: (t >= 64) & (t < 128), lambda t: t >= 190, lambda t: t % 5 == 0,
+                     lambda t: t < 130, lambda t: t >= 0):
+            c = logits_case(lambda t: torch.where(pick(t), 0.0, -e * math.log(2.0)) + torch.sin(t.float()), G, 2,
+                            [200, 70], 220 + G)
+            v = rows(c, 221, 2)
+            for b in (0, 1):
+                v[slots_of(c, b)[pick(torch.arange(c["ctx"][b]))]] = 0
+            c = with_v(c, v)
+            check_v(call(c, cuda), c)
