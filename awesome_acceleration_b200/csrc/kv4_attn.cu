@@ -7,11 +7,12 @@
 // not the memory, is what bounds the kernel (with the arithmetic taken out
 // 256 rows take 110 us).
 //
-// Measured (B200, bf16 q, floor at a copy's 6.45 TB/s): 256 rows of 512..4096
-// tokens at 16/8 heads 120 to 130 us (up to 5.6 TB/s, floor 106); 256 of
-// 1024..2047 at 64/8 heads 95 us (floor 71); 40 of 1..3001 at 64/8 heads 27.5
-// us (floor 10); 1 row of 40960 at 32/8 heads 20 us (floor 7.3), of 333 at 16/8
-// 6.2 us: a launch, the plan and the merge are about 6 us of each.
+// Measured (B200, bf16 q, replayed from a graph; floor at a copy's 6.45 TB/s):
+// 256 rows of 512..4096 tokens at 16/8 heads 120 us (5.7 TB/s, floor 106; called
+// one by one over changing inputs 131); 256 of 1024..2047 at 64/8 heads 96 us
+// (floor 71); 40 of 1..3001 at 64/8 heads 28.4 us (floor 10); 1 row of 40960 at
+// 32/8 heads 20 us (floor 7.3), of 333 at 16/8 6.2 us: a launch, the plan and the
+// merge are about 6 us of each.
 //
 // Work: the kernel is persistent, one CTA per SM of 8 warps that compute and 8
 // that load, grouped into teams of T = 1, 2, 4 or 8.  An item is one (row, kv
@@ -426,8 +427,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
     }
   }
   __syncthreads();
-  // Lane i weighs T = 2^i, in units of a model fitted to runs of 24 shapes with each T (B200; on average within 1 %
-  // of the best T, at most 6 %; T = 1, 2, 4 or 8 for all would cost 95, 22, 19 or 23 % on average): 3 for a round of
+  // Lane i weighs T = 2^i, in units of a model fitted to runs of 24 shapes with each T (B200; on average within 2 %
+  // of the best T, at most 11 %; T = 1, 2, 4 or 8 for all would cost 112, 28, 13 or 19 % on average): 3 for a round of
   // tiles; for each segment of a run 0.14 per head and warp that meets the first; where items are shared, 1.2, and
   // for each part of an item 0.93 and 0.25 for each of the heads that a warp adds.
   if (warp == 0) {
