@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv4_decode_kernel(const Kv4Arg
         const uint8_t* kb = sm.kv[warp][st][0];
         const uint8_t* vb = sm.kv[warp][st][1];
         const int lim = cs.ctx - t * kKv4Tile;
-        float* mine = &sm.red_o[warp][0][lane];  // free until the segment ends: this lane's scores, then p
+        float* mine = &sm.red_o[warp][0][lane];  // free until the segment ends: this lane's scores
         float x[HV];
 #pragma unroll
         for (int e = 0; e < HV; ++e) x[e] = -INFINITY;

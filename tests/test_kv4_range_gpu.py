@@ -263,3 +263,23 @@ def test_tiles_of_zeros(cuda, G):
                 v[slots_of(c, b)[pick(torch.arange(c["ctx"][b]))]] = 0
             c = with_v(c, v)
             check_v(call(c, cuda), c)
+
+
+@pytest.mark.parametrize("level", [-90, -40, 60])
+@pytest.mark.parametrize("scale", [2.0 ** -80, SCALE, 2.0 ** 45])
+def test_small_query_elements_at_every_scale(cuda, scale, level):
+    """Query elements near 2^level and 2^-70 of that, K to make up for both, so that logits are ordinary whatever the
+    softmax scale."""
+    low = round(-level - math.log2(scale / SCALE))
+    if low + 70 > 120:
+        level, low = level + (low - 50), 50
+    for G in (1, 8):
+        c = make_case([130, 3], G, 2, 64, 230 + G)
+        k = rows(c, 231, 2).float().view(-1, 2, 4, 32) * 2.0 ** max(low, -120)
+        k[:, :, 1] *= 2.0 ** 70
+        q = c["q"].float().view(2, -1, 4, 32) * 2.0 ** level
+        q[:, :, 1] *= 2.0 ** -70
+        c["kp"] = O.pool_from_rows(k.view(-1, 2, 128).to(BF), 64, False)
+        c["q"] = q.view(2, -1, 128).to(BF)
+        assert c["q"].isfinite().all() and k.isfinite().all()
+        check_v(call(c, cuda, scale=scale), c, scale=scale)
